@@ -13,6 +13,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libforgeserve_hip.so")
 
 F32, BF16, F16 = 0, 1, 2
+STORE_E4M3 = 16   # a pool of 8-bit codes (fs_kv_layout): added to the dtype of the rows written and read
 DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 c_i32, c_i64, c_f32, c_p = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p

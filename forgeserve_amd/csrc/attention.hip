@@ -26,7 +26,7 @@
 #include <math.h>
 #include <stdlib.h>
 
-#include "common.h"
+#include "e4m3.h"
 
 namespace {
 
@@ -1499,6 +1499,103 @@ __global__ void __launch_bounds__(64) attn_f32_kernel(AttnParams P) {
   }
 }
 
+// The scalar kernel over a pool of e4m3 codes (float32 rows, and what the matrix kernels do not take): a lane per key,
+// its codes 16 at a time, then a lane per dim, four keys to a word. A key's scale multiplies its score, a value's its
+// probability, both in float32. A score that is NaN stays one, and its row's output is NaN.
+template <int DT>
+__global__ void __launch_bounds__(64) attn_generic_e4m3_kernel(AttnParams P) {
+  typedef Elem<DT> E;
+  typedef typename E::T T_;
+  __shared__ float qs[256];
+  __shared__ float ps[64];
+  const int lane = threadIdx.x;
+  const int s = blockIdx.y;
+  const int64_t R = blockIdx.x;  // (b, t, h)
+  const int h = (int)(R % P.H);
+  const int bt = (int)(R / P.H);
+  const int b = bt / P.T, t = bt - b * P.T;
+  const int pos = P.pos[bt];
+  const int kbeg = s * P.split;
+  if (pos < kbeg) return;
+  const int kend = min(kbeg + P.split, pos + 1);
+  const int D = P.kv.head_dim, BS = P.kv.block_size;
+  const int hkv = h / P.G;
+  const T_* qrow = reinterpret_cast<const T_*>(P.q) + q_offset(P, b, t) + (int64_t)h * P.q_sh;
+  for (int d = lane; d < D; d += 64) qs[d] = E::load(qrow, d);
+  __syncthreads();
+  const int32_t* trow = P.table + (int64_t)b * P.table_stride;
+  auto block_of = [&](int j) {   // -1: unmapped
+    const int bi = j / BS;
+    const int v = bi < P.max_blocks ? trow[bi] : -1;
+    return v >= 0 && v < P.kv.num_blocks ? v : -1;
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = kbeg; j0 < kend; j0 += 64) {
+    const int j = j0 + lane;
+    float sv = -INFINITY, vs = 0.f;
+    if (j < kend) {
+      const int blk = block_of(j), slot = j % BS;
+      if (blk >= 0) {
+        const uint8_t* kt = key_tile(P.kv, blk, hkv);
+        const uint8_t* sc = tile_scales(P.kv, blk, hkv);
+        float dot = 0.f;
+        for (int d = 0; d < D; d += 16) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(kt + key_code(P.kv, slot, d));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float f[4];
+            decode4(w[c], f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dot = fmaf(qs[d + 4 * c + e], f[e], dot);
+          }
+        }
+        sv = dot * scale_value(sc[slot]) * P.scale_log2;
+        vs = scale_value(sc[BS + slot]);
+      }
+    }
+    const float m_new = fmaxf(m_run, wave_max(sv));
+    const float alpha = (m_new == -INFINITY) ? 1.f : exp2f(m_run - m_new);
+    const float p = (sv == -INFINITY) ? 0.f : exp2f(sv - m_new);
+    l_run = l_run * alpha + wave_sum(p);
+    m_run = m_new;
+    __syncthreads();
+    ps[lane] = p * vs;
+    __syncthreads();
+    const int nj = min(64, kend - j0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int d = lane + 64 * c;
+      if (d >= D) break;
+      float a = acc[c] * alpha;
+      for (int jj = 0; jj < nj; jj += 4) {   // four keys of one block (block_size % 4 == 0, j0 % 64 == 0)
+        const int blk = block_of(j0 + jj);
+        if (blk < 0) continue;   // (their weights are zeros)
+        float f[4];
+        decode4(*reinterpret_cast<const uint32_t*>(value_tile(P.kv, blk, hkv) + value_code(P.kv, (j0 + jj) % BS, d)), f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pj = ps[jj + e];
+          if (pj == 0.f) continue;   // a masked key, or one past kend: whatever lies there adds nothing
+          a = fmaf(pj, f[e], a);
+        }
+      }
+      acc[c] = a;
+    }
+  }
+  float* pa = P.ws_acc + (R * P.nsplit + s) * D;
+  for (int c = 0; c < 4; ++c) {
+    const int d = lane + 64 * c;
+    if (d < D) pa[d] = acc[c];
+  }
+  if (lane == 0) {
+    float* pm = P.ws_ml + (R * P.nsplit + s) * 2;
+    pm[0] = m_run;
+    pm[1] = l_run;
+  }
+}
+
 // Whole 16-byte pieces of queries, keys and values, head_dim <= 128, four consecutive keys in one block.
 bool f32_eligible(const fs_kv_layout& kv, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh) {
   if (kv.dtype != FS_F32 || kv.head_dim % 4 || kv.head_dim > 128 || kv.block_size % 4) return false;
@@ -1533,6 +1630,7 @@ __global__ void __launch_bounds__(64 * COMBINE_ROWS) attn_combine_kernel(AttnPar
     return;
   }
   const int ns = min(pos / P.split + 1, P.nsplit);  // keys past the table were never visible
+  const bool keep_nan = stores_e4m3(P.kv);
   const float* ml = P.ws_ml + R * P.nsplit * 2;
   const float* pa = P.ws_acc + R * P.nsplit * D;
   float M = -INFINITY;
@@ -1573,7 +1671,7 @@ __global__ void __launch_bounds__(64 * COMBINE_ROWS) attn_combine_kernel(AttnPar
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int d = lane + 64 * c;
-    if (d < D) E::store(orow, d, L > 0.f ? acc[c] / L : 0.f);
+    if (d < D) E::store(orow, d, L > 0.f || (keep_nan && L != 0.f) ? acc[c] / L : 0.f);
   }
 }
 
@@ -1688,9 +1786,12 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
   FS_CHECK_ARG(kv->block_size > 0 && max_blocks > 0 && table_stride >= max_blocks,
                "paged_attention: block_size %d max_blocks %d", kv->block_size, max_blocks);
   FS_CHECK_ARG(kv->num_blocks > 0, "paged_attention: num_blocks");
-  FS_CHECK_ARG(kv->dtype == FS_F32 || kv->dtype == FS_BF16 || kv->dtype == FS_F16, "paged_attention: dtype %d",
-               kv->dtype);
-  FS_CHECK_ARG(kv->k_group == 0 || (kv->k_group > 0 && kv->k_dim == 1 && kv->head_dim % 8 == 0),
+  const bool e4m3 = stores_e4m3(*kv);
+  const int32_t dtype = row_dtype(*kv);
+  FS_CHECK_ARG(dtype == FS_F32 || dtype == FS_BF16 || dtype == FS_F16, "paged_attention: dtype %d", kv->dtype);
+  if (e4m3)
+    if (int e = check_e4m3_layout(*kv, "paged_attention")) return e;
+  FS_CHECK_ARG(e4m3 || kv->k_group == 0 || (kv->k_group > 0 && kv->k_dim == 1 && kv->head_dim % 8 == 0),
                "paged_attention: grouped keys need k_group > 0, k_dim == 1 and head_dim %% 8 == 0");
   const int64_t need = fs_paged_attention_workspace_size(B, T, n_heads, kv->head_dim, max_blocks, kv->block_size);
   FS_CHECK_ARG(workspace_bytes >= need, "paged_attention: workspace %lld < %lld bytes", (long long)workspace_bytes,
@@ -1808,6 +1909,12 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
       else attn_f32_kernel<8><<<fgrid, 64, 0, st>>>(P);
       if (int e = fs::launch_status("paged_attention")) return e;
       if (P.nsplit == 1) return 0;   // every output is written
+    } else if (e4m3) {
+      switch (dtype) {
+        case FS_F32: attn_generic_e4m3_kernel<FS_F32><<<grid, 64, 0, st>>>(P); break;
+        case FS_BF16: attn_generic_e4m3_kernel<FS_BF16><<<grid, 64, 0, st>>>(P); break;
+        default: attn_generic_e4m3_kernel<FS_F16><<<grid, 64, 0, st>>>(P); break;
+      }
     } else switch (kv->dtype) {
       case FS_F32: attn_generic_kernel<FS_F32><<<grid, 64, 0, st>>>(P); break;
       case FS_BF16: attn_generic_kernel<FS_BF16><<<grid, 64, 0, st>>>(P); break;
@@ -1817,7 +1924,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
   if (int e = fs::launch_status("paged_attention")) return e;
   if (P.direct && P.nsplit == 1) return 0;   // every query sees one chunk: all outputs are written
   dim3 cgrid((unsigned)((rows + COMBINE_ROWS - 1) / COMBINE_ROWS));
-  switch (kv->dtype) {
+  switch (dtype) {
     case FS_F32: attn_combine_kernel<FS_F32><<<cgrid, 64 * COMBINE_ROWS, 0, st>>>(P, out, o_sb, o_st, o_sh); break;
     case FS_BF16: attn_combine_kernel<FS_BF16><<<cgrid, 64 * COMBINE_ROWS, 0, st>>>(P, out, o_sb, o_st, o_sh); break;
     default: attn_combine_kernel<FS_F16><<<cgrid, 64 * COMBINE_ROWS, 0, st>>>(P, out, o_sb, o_st, o_sh); break;

@@ -8,13 +8,14 @@
 // for the host. Launched from here: 16 rows of one token through 4 blocks (d = 2048, bf16) 440 -> 330 us, which
 // are the kernels'; one row through 4 float32 blocks (d = 256) 520 -> 303; four rows of 160 tokens through
 // those 707 -> 467.
-#include "common.h"
+#include "e4m3.h"
 
 namespace {
 
 struct Shape {
   int64_t m, d, qn, qkv_n, f;   // rows, d_model, query columns, QKV columns, hidden columns
   int32_t hd, dtype;
+  bool e4m3;                    // the caches hold 8-bit codes
 };
 
 // The projection's K splits are left as partials for the kernel that follows it (their sum is that kernel's).
@@ -22,7 +23,10 @@ bool partials_ok(const Shape& s, int64_t n, int64_t k) {
   return s.dtype == FS_BF16 && k % 64 == 0 && n % 8 == 0 && fs_gemm_splits(n, k, s.dtype) > 1 &&
          !fs_gemm_serial(s.m, n, k, s.dtype);
 }
-bool qkv_partials(const Shape& s) { return partials_ok(s, s.qkv_n, s.d) && s.hd % 16 == 0; }
+bool qkv_partials(const Shape& s) {
+  const int32_t groups = s.hd / 16;   // (into a pool of codes: a power of two of them)
+  return partials_ok(s, s.qkv_n, s.d) && s.hd % 16 == 0 && !(s.e4m3 && (groups & (groups - 1)));
+}
 bool norm_partials(const Shape& s, int64_t k) { return s.d <= 8192 && partials_ok(s, s.d, k); }
 bool fused_swiglu(const Shape& s) {
   return s.dtype == FS_BF16 && s.f % 2 == 0 && s.d % 64 == 0 && fs_gemm_splits(2 * s.f, s.d, s.dtype) == 1;
@@ -59,11 +63,12 @@ int64_t partials_bytes(const Shape& s, int64_t n, int64_t k) {
 }
 
 bool make_shape(Shape& s, int32_t B, int32_t T, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t d_model,
-                int64_t ffn, int32_t dtype) {
+                int64_t ffn, int32_t kv_dtype) {
+  const int32_t dtype = kv_dtype & ~FS_STORE_E4M3;
   if (B < 0 || T < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || d_model <= 0 || ffn <= 0) return false;
   if (dtype != FS_F32 && dtype != FS_BF16 && dtype != FS_F16) return false;
   s = Shape{(int64_t)B * T, d_model, (int64_t)n_heads * head_dim, (int64_t)(n_heads + 2 * n_kv_heads) * head_dim, ffn,
-            head_dim, dtype};
+            head_dim, dtype, dtype != kv_dtype};
   return true;
 }
 
@@ -76,10 +81,11 @@ bool make_shape(Shape& s, int32_t B, int32_t T, int32_t n_heads, int32_t n_kv_he
 }  // namespace
 
 extern "C" int fs_run_blocks_workspace(int32_t B, int32_t T, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
-                                       int64_t d_model, int64_t ffn, int32_t dtype, int32_t max_blocks,
+                                       int64_t d_model, int64_t ffn, int32_t kv_dtype, int32_t max_blocks,
                                        int32_t block_size, int64_t* bytes) {
   Shape s;
-  FS_CHECK_ARG(bytes && make_shape(s, B, T, n_heads, n_kv_heads, head_dim, d_model, ffn, dtype), "run_blocks_workspace: shapes");
+  FS_CHECK_ARG(bytes && make_shape(s, B, T, n_heads, n_kv_heads, head_dim, d_model, ffn, kv_dtype), "run_blocks_workspace: shapes");
+  const int32_t dtype = s.dtype;
   int64_t g = 0;
   auto need = [&](bool partials, int64_t n, int64_t k) {
     const int64_t b = partials ? partials_bytes(s, n, k) : fs_gemm_workspace_size(s.m, n, k, dtype);
@@ -97,22 +103,24 @@ extern "C" int fs_run_blocks_workspace(int32_t B, int32_t T, int32_t n_heads, in
 }
 
 extern "C" int fs_run_blocks(const fs_block* blocks, int32_t n_blocks, int32_t B, int32_t T, int32_t n_heads,
-                             int64_t d_model, int64_t ffn, int32_t dtype, const int32_t* positions,
+                             int64_t d_model, int64_t ffn, int32_t kv_dtype, const int32_t* positions,
                              const float* rope_cos, const float* rope_sin, int32_t rope_len, float scale, const void* x,
                              const void* h, void* x_out, void* y_out, void* gemm_ws, int64_t gemm_ws_bytes,
                              void* attn_ws, int64_t attn_ws_bytes, void* scratch, int64_t scratch_bytes, void* stream) {
   FS_CHECK_ARG(blocks && n_blocks > 0 && x && h && x_out && scratch, "run_blocks: null pointer");
   Shape s;
-  FS_CHECK_ARG(make_shape(s, B, T, n_heads, blocks[0].kv.n_kv_heads, blocks[0].kv.head_dim, d_model, ffn, dtype),
+  FS_CHECK_ARG(make_shape(s, B, T, n_heads, blocks[0].kv.n_kv_heads, blocks[0].kv.head_dim, d_model, ffn, kv_dtype),
                "run_blocks: shapes");
+  const int32_t dtype = s.dtype;
   FS_CHECK_ARG(positions && rope_cos && rope_sin && attn_ws, "run_blocks: null pointer");
   for (int32_t i = 0; i < n_blocks; ++i) {   // all of them before the first launch writes to a cache
     const fs_block& b = blocks[i];
-    FS_CHECK_ARG(b.kv.n_kv_heads == blocks[0].kv.n_kv_heads && b.kv.head_dim == s.hd && b.kv.dtype == dtype,
+    FS_CHECK_ARG(b.kv.n_kv_heads == blocks[0].kv.n_kv_heads && b.kv.head_dim == s.hd && b.kv.dtype == kv_dtype,
                  "run_blocks: block %d: its cache's heads, head_dim or dtype", (int)i);
     FS_CHECK_ARG(b.w_qkv && b.w_o && b.w_gate_up && b.w_down && b.mlp_norm && b.kv.k && b.kv.v && b.tables && b.visible &&
                      (b.next_norm || i == n_blocks - 1),
                  "run_blocks: block %d: null pointer", (int)i);
+    if (s.e4m3) FS_TRY(check_e4m3_layout(b.kv, "run_blocks"));
   }
   FS_CHECK_ARG(blocks[n_blocks - 1].next_norm == nullptr || y_out, "run_blocks: null y_out");
   const Scratch sc(reinterpret_cast<char*>(scratch), s);

@@ -3,8 +3,10 @@
 // Reference: paged.py:71-82 (PagedLayerView.update) and model.py:40-45 (apply_rope).
 // Pool layout is described by fs_kv_layout; one (block, kv-head) tile of keys is block_size*head_dim
 // contiguous elements (slot-major, or as 8-dim groups of every slot), and values are stored dim-major
-// so the attention kernel reads 16 keys of one dim as one contiguous run.
-#include "common.h"
+// so the attention kernel reads 16 keys of one dim as one contiguous run. A pool of 8-bit codes has kernels of its
+// own (kv_e4m3.hip).
+#include "e4m3.h"
+#include "kv.h"
 
 namespace {
 
@@ -22,95 +24,9 @@ FS_DEVICE void rope_pair(float x1, float x2, float c, float s, float& o1, float&
   o2 = E::round(d + e);
 }
 
-FS_DEVICE bool slot_of(int pos, const int32_t* table, int64_t table_stride, int b, int max_blocks,
-                       const fs_kv_layout& kv, int64_t& blk, int& slot) {
-  if (pos < 0) return false;
-  int bi = pos / kv.block_size;
-  if (bi >= max_blocks) return false;
-  blk = table[(int64_t)b * table_stride + bi];
-  if (blk < 0 || blk >= kv.num_blocks) return false;
-  slot = pos - bi * kv.block_size;
-  return true;
-}
-
-typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4_t;
-
-template <int DT>
-FS_DEVICE void unpack8(const u32x4_t& w, float (&v)[8]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = Elem<DT>::to_f32((uint16_t)(w[j] & 0xffffu));
-    v[2 * j + 1] = Elem<DT>::to_f32((uint16_t)(w[j] >> 16));
-  }
-}
-
-template <int DT>
-FS_DEVICE u32x4_t pack8(const float (&v)[8]) {
-  u32x4_t w;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    w[j] = (uint32_t)Elem<DT>::store_bits(v[2 * j]) | ((uint32_t)Elem<DT>::store_bits(v[2 * j + 1]) << 16);
-  return w;
-}
-
 // The same as qkv_rope_write_kernel for 16-bit dtypes whose rows split into 16-byte groups (D/2 % 8 == 0,
 // aligned rows, each 8-dim group of a key contiguous): a thread rotates 8 pairs at once (two 16-byte loads of the halves,
 // 16-byte loads of cos/sin, 16-byte stores of q and k); values keep the dim-major element stores.
-// Eight consecutive qkv elements as floats: the 16-bit row itself, or (PART) the split-K partials of
-// the QKV projection [splits][rows][cols] added in increasing split order and rounded to DT, exactly the
-// values the GEMM's own reduction would have stored.
-struct QkvPart {
-  const float* part;   // null: read the 16-bit qkv rows
-  int32_t splits;
-  int64_t stride;      // elements between consecutive splits (rows * cols)
-};
-
-// PART: 0 reads the 16-bit row; > 0 adds that many partials, all loaded before the first add; < 0
-// adds pp.splits partials one at a time.
-template <int DT, int PART>
-FS_DEVICE void load8(const uint16_t* qkv, const QkvPart& pp, int64_t e, float (&v)[8]) {
-  if (PART == 0) {
-    unpack8<DT>(*reinterpret_cast<const u32x4_t*>(qkv + e), v);
-    return;
-  }
-  float4_t a, b;
-  if (PART > 0) {
-    constexpr int NS = PART > 0 ? PART : 1;
-    float4_t qa[NS], qb[NS];
-#pragma unroll
-    for (int sp = 0; sp < NS; ++sp) {
-      qa[sp] = *reinterpret_cast<const float4_t*>(pp.part + sp * pp.stride + e);
-      qb[sp] = *reinterpret_cast<const float4_t*>(pp.part + sp * pp.stride + e + 4);
-    }
-    a = qa[0];
-    b = qb[0];
-#pragma unroll
-    for (int sp = 1; sp < NS; ++sp)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] += qa[sp][j];
-        b[j] += qb[sp][j];
-      }
-  } else {
-    a = *reinterpret_cast<const float4_t*>(pp.part + e);
-    b = *reinterpret_cast<const float4_t*>(pp.part + e + 4);
-    for (int sp = 1; sp < pp.splits; ++sp) {
-      const float4_t a2 = *reinterpret_cast<const float4_t*>(pp.part + sp * pp.stride + e);
-      const float4_t b2 = *reinterpret_cast<const float4_t*>(pp.part + sp * pp.stride + e + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] += a2[j];
-        b[j] += b2[j];
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = Elem<DT>::round(a[j]);
-    v[j + 4] = Elem<DT>::round(b[j]);
-  }
-}
-
 // Verify windows: T consecutive tokens of a table row (rows back to back, T <= VWIN_MAX_T) sit in
 // consecutive pool slots, so a dim's values of the window are one short run of the dim-major value
 // tile. Their values are written by the grid's last row of workgroups through LDS, lanes taking
@@ -388,6 +304,7 @@ __global__ void __launch_bounds__(256) gather_kernel(fs_kv_layout kv, const int3
 
 int check_layout(const fs_kv_layout* kv) {
   FS_CHECK_ARG(kv != nullptr && kv->k != nullptr && kv->v != nullptr, "kv layout: null pool");
+  if (stores_e4m3(*kv)) return check_e4m3_layout(*kv, "kv layout");
   FS_CHECK_ARG(kv->dtype == FS_F32 || kv->dtype == FS_BF16 || kv->dtype == FS_F16, "kv layout: bad dtype %d",
                kv->dtype);
   FS_CHECK_ARG(kv->block_size > 0 && kv->n_kv_heads > 0 && kv->head_dim > 0 && kv->head_dim % 2 == 0,
@@ -421,6 +338,10 @@ int qkv_rope_write(const void* qkv, int64_t qkv_stride, int64_t n_tokens, int32_
   FS_CHECK_ARG(qkv_stride >= (int64_t)(n_heads + 2 * kv->n_kv_heads) * kv->head_dim, "qkv_rope_write: qkv stride");
   if (n_tokens == 0) return 0;
   hipStream_t s = fs::as_stream(stream);
+  if (stores_e4m3(*kv))
+    return fs::qkv_rope_write_e4m3(qkv, pp.part, pp.splits, pp.stride, qkv_stride, n_tokens, T, n_heads, positions, slots,
+                                   token_row, n_rows, rope_cos, rope_sin, rope_len, block_tables, table_stride, max_blocks,
+                                   *kv, q_out, q_stride, s);
   dim3 grid((unsigned)n_tokens);
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = kv->dtype != FS_F32 && (kv->head_dim / 2) % 8 == 0 && kv->head_dim % 2 == 0 &&
@@ -523,6 +444,9 @@ extern "C" int fs_paged_kv_write(const void* k_new, const void* v_new, int64_t s
                (long long)table_stride);
   if (B == 0 || T == 0) return 0;
   hipStream_t s = fs::as_stream(stream);
+  if (stores_e4m3(*kv))
+    return fs::paged_kv_write_e4m3(k_new, v_new, s_b, s_h, s_t, B, T, positions, block_tables, table_stride, max_blocks,
+                                   *kv, s);
   dim3 grid((unsigned)(B * T));
 #define FS_LAUNCH(DT)                                                                                            \
   kv_write_kernel<DT><<<grid, 256, 0, s>>>((const typename Elem<DT>::T*)k_new, (const typename Elem<DT>::T*)v_new, \
@@ -545,6 +469,7 @@ extern "C" int fs_paged_gather(const fs_kv_layout* kv, const int32_t* block_tabl
   const int64_t total = (int64_t)B * kv->n_kv_heads * max_blocks * kv->block_size * kv->head_dim;
   if (total == 0) return 0;
   hipStream_t s = fs::as_stream(stream);
+  if (stores_e4m3(*kv)) return fs::paged_gather_e4m3(*kv, block_tables, table_stride, B, max_blocks, k_out, v_out, s);
   int64_t blocks = (total + 255) / 256;
   if (blocks > 65536) blocks = 65536;
   dim3 grid((unsigned)blocks);

@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, KVLayout, check, ptr, require_device, stream_ptr
+from ._lib import DTYPE_CODE, STORE_E4M3, KVLayout, check, ptr, require_device, stream_ptr
 
 I32 = torch.int32
 
@@ -69,6 +69,44 @@ def kv_layout(k: torch.Tensor, v: torch.Tensor) -> KVLayout:
         raise ValueError(f"k/v pool views must match: {tuple(k.shape)} vs {tuple(v.shape)}")
     nb, h, bs, d = v.shape
     return KVLayout(k.data_ptr(), v.data_ptr(), *k_strides, *v.stride(), bs, h, d, _dt(k), nb, k_group)
+
+
+def kv_layout_e4m3(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> KVLayout:
+    """Layout of one layer whose keys and values are 8-bit floating point (e4m3 codes, torch.float8_e4m3fn or
+    uint8) with one power of two per token, KV head and side as their scale. Every call that takes a layout takes
+    this one: the writes encode rows of `dtype`, the gather and the attention decode, with queries and outputs of
+    `dtype` (float32, bfloat16, float16).
+
+    k: (num_blocks, n_kv_heads, head_dim // 16, block_size, 16); v: (num_blocks, n_kv_heads, block_size // 4,
+    head_dim, 4), the dims of each 64 (or what is left of them) ordered by d % 16 first; scales: uint8
+    (num_blocks, n_kv_heads, 2, block_size), the exponent bytes e of the keys', then of the values' scales
+    2^(e - 127). The blocks and heads may have any strides; a tile, and a pair of scale rows, is contiguous.
+    head_dim is a multiple of 16 and at most 256, block_size a multiple of 4. The scale is the smallest power of
+    two that brings a group's largest magnitude to 448 or less (fs_kv_layout says what lies beyond the limits);
+    attention is fast for bfloat16 and float16 with head_dim 64 or 128 and block_size % 16 == 0."""
+    if any(t.dtype not in (torch.uint8, torch.float8_e4m3fn) for t in (k, v)) or scales.dtype != torch.uint8:
+        raise ValueError(f"8-bit pool: codes must be float8_e4m3fn or uint8, scales uint8: {k.dtype}, {v.dtype}, "
+                         f"{scales.dtype}")
+    if k.device != v.device or k.device != scales.device:
+        raise ValueError("8-bit pool: codes and scales must be on one device")
+    if k.dim() != 5 or v.dim() != 5 or scales.dim() != 4:
+        raise ValueError(f"8-bit pool: shapes {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)}")
+    nb, h, c, bs, w = k.shape
+    d = 16 * c
+    if w != 16 or v.shape != (nb, h, bs // 4, d, 4) or scales.shape != (nb, h, 2, bs) or bs % 4 or d > 256:
+        raise ValueError(f"8-bit pool: shapes {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)} (head_dim a "
+                         "multiple of 16 up to 256, block_size a multiple of 4)")
+    if not (k[0, 0].is_contiguous() and v[0, 0].is_contiguous() and scales[0, 0].is_contiguous()):
+        raise ValueError("8-bit pool: a tile's codes and its scales must be contiguous")
+    return KVLayout(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), scales.stride(0), scales.stride(1), v.stride(0),
+                    v.stride(1), 0, 0, bs, h, d, _dt(torch.empty(0, dtype=dtype)) | STORE_E4M3, nb,
+                    scales.data_ptr() - k.data_ptr())
+
+
+def _check_rows(what: str, t_dtype: torch.dtype, layout: KVLayout) -> None:
+    """A pool of codes takes and gives rows of its own dtype only."""
+    if layout.dtype & STORE_E4M3 and DTYPE_CODE.get(t_dtype) != layout.dtype & ~STORE_E4M3:
+        raise ValueError(f"{what}: {t_dtype} rows and an 8-bit pool of another dtype")
 
 
 # ------------------------------------------------------------------------------------------------
@@ -265,6 +303,7 @@ def qkv_rope_write(qkv: torch.Tensor, positions: torch.Tensor, T: int, n_heads: 
     qkv: (B*T, (n_heads + 2*n_kv_heads) * head_dim); positions/slots: int32 (B*T,);
     tables: int32 (B, max_blocks). Returns the rotated queries (B*T, n_heads * head_dim)."""
     require_device(qkv, positions, tables)
+    _check_rows("qkv_rope_write", qkv.dtype, layout)
     m, ld = _rows(qkv)
     d = layout.head_dim
     if q_out is None:
@@ -290,7 +329,8 @@ def qkv_rope_gemm(h: torch.Tensor, w: torch.Tensor, positions: torch.Tensor, T: 
     k = h.shape[1]
     lib = _lib.load()
     d = layout.head_dim
-    if (h.dtype == torch.bfloat16 and w.dtype == h.dtype and w.shape[1] == k and layout.dtype == _dt(h)
+    if (h.dtype == torch.bfloat16 and w.dtype == h.dtype and w.shape[1] == k and layout.dtype & ~STORE_E4M3 == _dt(h)
+            and not (layout.dtype & STORE_E4M3 and d // 16 & (d // 16 - 1))
             and k % 64 == 0 and lda % 8 == 0 and ldb % 8 == 0 and n % 8 == 0 and (d // 2) % 8 == 0
             and lib.fs_gemm_splits(n, k, _dt(h)) > 1 and not lib.fs_gemm_serial(m, n, k, _dt(h))
             and positions.dtype == I32 and tables.dtype == I32
@@ -316,6 +356,7 @@ def qkv_rope_write_varlen(qkv: torch.Tensor, positions: torch.Tensor, token_row:
     qkv: (n_tokens, (n_heads + 2*n_kv_heads) * head_dim); positions, token_row: int32 (n_tokens,);
     tables: int32 (rows, max_blocks). Returns the rotated queries (n_tokens, n_heads * head_dim)."""
     require_device(qkv, positions, token_row, tables)
+    _check_rows("qkv_rope_write_varlen", qkv.dtype, layout)
     m, ld = _rows(qkv)
     d = layout.head_dim
     if positions.dtype != I32 or token_row.dtype != I32 or tables.dtype != I32:
@@ -337,6 +378,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, ta
                    layout: KVLayout) -> None:
     """Scatter k, v (B, n_kv_heads, T, head_dim) to the pool slots of positions (B, T) (paged.py:74-78)."""
     require_device(k, v, positions, tables)
+    _check_rows("paged_kv_write", k.dtype, layout)
     if k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
         raise ValueError("paged_kv_write: k and v must share shape and strides, head_dim contiguous")
     b, h, t, d = k.shape
@@ -349,6 +391,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, ta
 
 def paged_gather(layout: KVLayout, tables: torch.Tensor, dtype, device) -> Tuple[torch.Tensor, torch.Tensor]:
     """Every block of every table row, in table order: (B, n_kv_heads, max_blocks*block_size, head_dim)."""
+    _check_rows("paged_gather", dtype, layout)
     b, nb = tables.shape
     shape = (b, layout.n_kv_heads, nb * layout.block_size, layout.head_dim)
     k_all = torch.empty(shape, dtype=dtype, device=device)
@@ -385,6 +428,7 @@ def paged_attention(q: torch.Tensor, layout: KVLayout, tables: torch.Tensor, pos
     plan_key: an object that stands for these positions (the forward step): consecutive calls with the
     same key reuse the work plan of the first (the positions must not change between them)."""
     require_device(q, tables, positions)
+    _check_rows("paged_attention", q.dtype, layout)
     b, t, h, d = q.shape
     if q.stride(3) != 1:
         raise ValueError("paged_attention: head_dim must be contiguous")
@@ -413,6 +457,7 @@ def paged_attention_varlen(q: torch.Tensor, layout: KVLayout, tables: torch.Tens
     sequence's tokens; tables int32 (S, max_blocks). Returns out (n_tokens, n_heads, head_dim).
     plan_key: as for paged_attention."""
     require_device(q, tables, positions, cu_seqlens)
+    _check_rows("paged_attention_varlen", q.dtype, layout)
     n, h, d = q.shape
     if q.stride(2) != 1:
         raise ValueError("paged_attention_varlen: head_dim must be contiguous")
@@ -449,10 +494,11 @@ def run_blocks(x: torch.Tensor, h: torch.Tensor, b: int, t: int, heads: tuple, f
     m, d = x.shape
     n_heads, nkv, hd = heads
     dt, dev = _dt(x), x.device
+    kv_dt = blocks[0][8][0].dtype   # (with the flag of a pool of codes)
     arr = (_lib.Block * len(blocks))()
     sizes = set()
     for e, (wq, wo, wgu, wd, n1, e1, n2, e2, (lay, tab, slots, vis), _) in zip(arr, blocks):
-        if (lay.n_kv_heads, lay.head_dim, lay.dtype) != (nkv, hd, dt):
+        if (lay.n_kv_heads, lay.head_dim, lay.dtype) != (nkv, hd, kv_dt) or kv_dt & ~STORE_E4M3 != dt:
             raise ValueError("run_blocks: the cache's heads, head_dim or dtype are not the model's")
         if (tab.dtype != I32 or vis.dtype != I32 or vis.shape != (b, t) or not vis.is_contiguous()
                 or (slots is not None and (slots.dtype != I32 or slots.numel() != m))):
@@ -463,11 +509,11 @@ def run_blocks(x: torch.Tensor, h: torch.Tensor, b: int, t: int, heads: tuple, f
         e.kv, e.tables, e.table_stride, e.max_blocks = lay, tab.data_ptr(), tab.stride(0), tab.shape[1]
         e.slots, e.visible, e.mlp_eps, e.next_eps = ptr(slots), vis.data_ptr(), e1, e2
         sizes.add((tab.shape[1], lay.block_size))
-    shape = (heads, ffn, frozenset(sizes))
+    shape = (heads, ffn, kv_dt, frozenset(sizes))
     if shape not in buffers:
         need, attn = (_lib.c_i64 * 3)(), 0
         for nb, bs in sizes:
-            check(lib.fs_run_blocks_workspace(b, t, n_heads, nkv, hd, d, ffn, dt, nb, bs, need), "run_blocks_workspace")
+            check(lib.fs_run_blocks_workspace(b, t, n_heads, nkv, hd, d, ffn, kv_dt, nb, bs, need), "run_blocks_workspace")
             attn = max(attn, need[1])
         buffers[shape] = (_persistent_ws("gemm", need[0], dev) if need[0] > 0 else None,
                           _persistent_ws("attention", attn, dev), _ws(need[2], dev))
@@ -479,7 +525,7 @@ def run_blocks(x: torch.Tensor, h: torch.Tensor, b: int, t: int, heads: tuple, f
         key, vis = blk[9], blk[8][3]
         e.reuse_plan = key is not None and before[0] is key and before[1] is vis
         before = key, vis
-    rc = lib.fs_run_blocks(arr, len(blocks), b, t, n_heads, d, ffn, dt, positions.data_ptr(), rope_cos.data_ptr(),
+    rc = lib.fs_run_blocks(arr, len(blocks), b, t, n_heads, d, ffn, kv_dt, positions.data_ptr(), rope_cos.data_ptr(),
                            rope_sin.data_ptr(), rope_cos.shape[0], 1.0 / math.sqrt(hd), x.data_ptr(), h.data_ptr(),
                            x_out.data_ptr(), ptr(y), ptr(gws), 0 if gws is None else gws.numel(), aws.data_ptr(),
                            aws.numel(), scratch.data_ptr(), scratch.numel(), stream_ptr())

@@ -16,6 +16,13 @@ every result are the same.
 `pool.k[layer]` is then a (num_blocks, n_kv_heads, block_size, head_dim/8, 8) view
 (`.flatten(-2)` gives the reference's shape, as a copy).
 
+`cache_dtype=torch.float8_e4m3fn` holds keys and values in 8-bit floating point, about half the bytes of a 16-bit
+pool: e4m3 codes with a power of two per token, KV head and side as their scale. Rows are encoded as they are
+written and decoded by whatever reads them, so everything that takes a pool's views takes these. `pool.k[layer]`,
+`pool.v[layer]` and `pool.scales[layer]` are then the codes and exponent bytes as `ops.kv_layout_e4m3` describes
+them; `ops.paged_gather` gives their values. A value is stored within half a step of e4m3, 2^-4 of it (of values
+below 2^-15 of their group's largest, 2^-19 of that).
+
 The block allocator and the block tables stay on the host, as in the reference; tables are copied
 to the GPU (int32) once per step and shared by every layer's view.
 """
@@ -136,10 +143,13 @@ class BlockAllocator:
 
 class PagedKVPool:
     """The block pool of every layer (paged.py:42-58). key_layout: "slots" (the reference's key shape,
-    the default) or "groups" (keys as 8-dim groups of every slot; see the module docstring)."""
+    the default) or "groups" (keys as 8-dim groups of every slot; see the module docstring). cache_dtype:
+    what keys and values are held in, `dtype` (None) or torch.float8_e4m3fn (codes in tiles of their own
+    order, whatever the key_layout)."""
 
     def __init__(self, cfg: ModelConfig, num_blocks: int, block_size: int = 16, tp: TPContext = SINGLE,
-                 dtype=torch.float32, device=None, key_layout: str = "slots"):
+                 dtype=torch.float32, device=None, key_layout: str = "slots",
+                 cache_dtype: Optional[torch.dtype] = None):
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else "cuda"
         h = cfg.n_kv_heads // tp.size
@@ -149,29 +159,53 @@ class PagedKVPool:
         self.num_blocks = num_blocks
         self.dtype = dtype
         self.device = torch.device(device)
-        if key_layout == "slots":
+        self.cache_dtype = dtype if cache_dtype is None else cache_dtype
+        self.scales = None
+        if key_layout not in ("slots", "groups"):
+            raise ValueError(f"key_layout must be 'slots' or 'groups', not {key_layout!r}")
+        if self.cache_dtype == torch.float8_e4m3fn:
+            self._store_e4m3(h, d)
+        elif self.cache_dtype != dtype:
+            raise ValueError(f"cache_dtype must be the pool's dtype {dtype} or torch.float8_e4m3fn, not {cache_dtype}")
+        elif key_layout == "slots":
             self.k_store = torch.zeros((cfg.n_layers, num_blocks, h, block_size, d), dtype=dtype, device=self.device)
             self.k = [self.k_store[i] for i in range(cfg.n_layers)]
-        elif key_layout == "groups":
+        else:
             if d % 8:
                 raise ValueError(f"grouped keys need head_dim % 8 == 0 (head_dim {d})")
             self.k_store = torch.zeros((cfg.n_layers, num_blocks, h, d // 8, block_size, 8), dtype=dtype,
                                        device=self.device)
             self.k = [self.k_store[i].transpose(2, 3) for i in range(cfg.n_layers)]
-        else:
-            raise ValueError(f"key_layout must be 'slots' or 'groups', not {key_layout!r}")
         self.key_layout = key_layout
-        self.v_store = torch.zeros((cfg.n_layers, num_blocks, h, d, block_size), dtype=dtype, device=self.device)
-        self.v = [self.v_store[i].transpose(-1, -2) for i in range(cfg.n_layers)]
+        if self.scales is None:
+            self.v_store = torch.zeros((cfg.n_layers, num_blocks, h, d, block_size), dtype=dtype, device=self.device)
+            self.v = [self.v_store[i].transpose(-1, -2) for i in range(cfg.n_layers)]
         self.allocator = BlockAllocator(num_blocks)
         self._layouts = None
+
+    def _store_e4m3(self, h: int, d: int) -> None:
+        """Tiles of codes and their scales' exponent bytes (a head's blocks side by side: a block's are 32 bytes at 16
+        slots, and four neighbouring blocks share a cache line), all zeros: every slot stands for zeros."""
+        n, nb, bs = self.cfg.n_layers, self.num_blocks, self.block_size
+        if d % 16 or d > 256 or bs % 4:
+            raise ValueError(f"an 8-bit pool needs head_dim % 16 == 0, at most 256, and block_size % 4 == 0 "
+                             f"(head_dim {d}, block_size {bs})")
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        self.k_store = zeros(n, nb, h, d // 16, bs, 16).view(torch.float8_e4m3fn)
+        self.v_store = zeros(n, nb, h, bs // 4, d, 4).view(torch.float8_e4m3fn)
+        self.scale_store = zeros(n, h, nb, 2, bs)
+        self.k, self.v = ([x[i] for i in range(n)] for x in (self.k_store, self.v_store))
+        self.scales = [self.scale_store[i].transpose(0, 1) for i in range(n)]
 
     def blocks_for(self, n_tokens: int) -> int:
         return -(-n_tokens // self.block_size)
 
     def layout(self, layer: int):
         if self._layouts is None:
-            self._layouts = [ops.kv_layout(self.k[i], self.v[i]) for i in range(len(self.k))]
+            if self.scales is not None:
+                self._layouts = [ops.kv_layout_e4m3(*x, self.dtype) for x in zip(self.k, self.v, self.scales)]
+            else:
+                self._layouts = [ops.kv_layout(self.k[i], self.v[i]) for i in range(len(self.k))]
         return self._layouts[layer]
 
     def views(self, block_tables: torch.Tensor, positions: torch.Tensor) -> List["PagedLayerView"]:

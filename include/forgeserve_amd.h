@@ -29,6 +29,9 @@ extern "C" {
 #define FS_F32 0
 #define FS_BF16 1
 #define FS_F16 2
+/* Added to a layout's dtype: the pool stores 8-bit floating point (see fs_kv_layout). The dtype without it is
+ * that of the rows written to the pool and read from it, of the queries and of the attention's outputs. */
+#define FS_STORE_E4M3 16
 
 #define FS_ERR_ARG (-1)
 
@@ -40,7 +43,20 @@ extern "C" {
  * (v_slot == 1, v_dim == block_size: a block's 16 keys of one dim are 32 contiguous bytes) and either
  * slot-major keys (k_slot == head_dim, k_dim == 1, k_group == 0) or grouped keys (k_slot == 8,
  * k_group == 8*block_size: a block's 16 keys of one 8-dim group are 256 contiguous bytes, so each
- * 16-byte-per-lane load of a key tile is one contiguous 1 KB run). */
+ * 16-byte-per-lane load of a key tile is one contiguous 1 KB run).
+ *
+ * dtype | FS_STORE_E4M3: keys and values are e4m3 codes (4 exponent and 3 mantissa bits, OCP: largest value 448,
+ * no infinities), with one power of two per token, KV head and side as their scale, kept as its biased exponent
+ * byte e: a code c stands for value(c) * 2^(e - 127). The scale is the smallest that brings the finite values'
+ * largest magnitude to 448 or less, from 2^-117 to 2^119 (f16: 2^-15 to 2^7, so that every value is an f16); what lies
+ * beyond the largest scale's 448 is stored as that, a value that is not finite as NaN. All offsets in bytes:
+ *   key (slot, dim)    k + block*k_block + head*k_head + (dim/16)*16*block_size + slot*16 + dim%16
+ *   value (slot, dim)  v + block*v_block + head*v_head + (slot/4)*4*head_dim + place(dim)*4 + slot%4, where
+ *                      place(dim) = dim/64*64 + dim%16*n + dim/16%4, n = min(4, head_dim/16 - dim/64*4)
+ *   scales             k + k_group + block*k_slot + head*k_dim: block_size bytes of the keys', then of the values'
+ * v_slot and v_dim are 0. head_dim % 16 == 0 and at most 256, block_size % 4 == 0; k, v and the tiles' strides are
+ * multiples of 16, those of the scales of 4. The fast attention path takes bf16 and f16 with head_dim 64 or 128 and
+ * block_size % 16 == 0. The rotary write rotates in f32 and rounds once (queries to the dtype, keys to the codes). */
 typedef struct fs_kv_layout {
   void* k;
   void* v;

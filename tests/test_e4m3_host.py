@@ -1,0 +1,140 @@
+"""The 8-bit pool's layout and what the calls refuse, on the CPU: nothing is launched."""
+
+import ctypes
+import os
+
+import pytest
+import torch
+
+import e4m3_reference as ref
+from forgeserve_amd import ModelConfig, PagedKVPool, _lib, ops
+from forgeserve_amd.build import LIB
+
+E4M3 = torch.float8_e4m3fn
+
+
+def config(hd=64, heads=4, kv=2, layers=2):
+    return ModelConfig(vocab_size=32, d_model=hd * heads, n_layers=layers, n_heads=heads, n_kv_heads=kv, ffn_dim=64,
+                       max_seq_len=64)
+
+
+def tensors(nb=3, h=2, hd=64, bs=16):
+    u8 = dict(dtype=torch.uint8)
+    return torch.zeros(nb, h, hd // 16, bs, 16, **u8), torch.zeros(nb, h, bs // 4, hd, 4, **u8), torch.zeros(nb, h, 2, bs, **u8)
+
+
+def test_reference_codes():
+    """The definition's own corners: every code is its own nearest, ties go to the even code, the scale's border is
+    448 itself, what is not finite is NaN."""
+    finite = ref.VALUES[~torch.isnan(ref.VALUES)]
+    one = torch.tensor([448.0])
+    for v in finite.tolist():
+        c, e = ref.encode(torch.cat([one.double(), torch.tensor([v], dtype=torch.float64)]), (10, 246))
+        assert int(e) == 127 and ref.VALUES[int(c[1])] == v
+    c, e = ref.encode(torch.tensor([448.0, 17.0, 19.0, -17.0, 2.0 ** -10, float("inf"), float("nan")]), (10, 246))
+    assert ref.decode(c, e)[:5].tolist() == [448.0, 16.0, 20.0, -16.0, 0.0] and ref.decode(c, e)[5:].isnan().all()
+    assert int(ref.exponents(torch.tensor([448.5]).double(), (10, 246))) == 128
+    assert int(ref.exponents(torch.tensor([224.0]).double(), (10, 246))) == 126
+    assert int(ref.exponents(torch.tensor([0.0]).double(), (112, 134))) == 112
+
+
+def test_codes_agree_with_torch():
+    x = torch.randn(4000, generator=torch.Generator().manual_seed(1)).mul_(60).clamp_(-448, 448)
+    x[0] = 448.0
+    c, _ = ref.encode(x.double(), (10, 246))
+    assert torch.equal(c, x.to(E4M3).view(torch.uint8))
+
+
+@pytest.mark.parametrize("hd", [16, 48, 64, 96, 128, 256])
+def test_value_order_is_a_permutation(hd):
+    p = ref.value_order(hd)
+    assert sorted(p.tolist()) == list(range(hd))
+    if hd % 64 == 0:   # the 16 bytes at a place: four keys of dims d, d + 16, d + 32, d + 48
+        assert p[16] == p[0] + 1 and p[32] == p[0] + 2 and p[1] == p[0] + 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_pool_layout(dtype):
+    pool = PagedKVPool(config(), 6, 16, dtype=dtype, device="cpu", cache_dtype=E4M3)
+    for layer in range(2):
+        lay = pool.layout(layer)
+        assert lay.dtype == _lib.DTYPE_CODE[dtype] | _lib.STORE_E4M3
+        assert (lay.k, lay.v) == (pool.k[layer].data_ptr(), pool.v[layer].data_ptr())
+        assert lay.k + lay.k_group == pool.scales[layer].data_ptr()
+        assert (lay.k_block, lay.k_head, lay.v_block, lay.v_head) == (2 * 1024, 1024, 2 * 1024, 1024)
+        assert (lay.k_slot, lay.k_dim) == pool.scales[layer].stride()[:2] == (32, 6 * 32)
+        assert (lay.v_slot, lay.v_dim, lay.block_size, lay.n_kv_heads, lay.head_dim, lay.num_blocks) == (0, 0, 16, 2, 64, 6)
+    assert pool.k[0].dtype == E4M3 and pool.dtype == dtype and pool.cache_dtype == E4M3
+    plain = PagedKVPool(config(), 6, 16, dtype=dtype, device="cpu")
+    assert plain.cache_dtype == dtype and plain.scales is None and plain.layout(0).dtype == _lib.DTYPE_CODE[dtype]
+
+
+def test_pool_refusals():
+    with pytest.raises(ValueError, match="8-bit pool"):
+        PagedKVPool(config(hd=40), 6, 16, device="cpu", cache_dtype=E4M3)
+    with pytest.raises(ValueError, match="8-bit pool"):
+        PagedKVPool(config(), 6, 6, device="cpu", cache_dtype=E4M3)
+    with pytest.raises(ValueError, match="cache_dtype"):
+        PagedKVPool(config(), 6, 16, device="cpu", cache_dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="key_layout"):
+        PagedKVPool(config(), 6, 16, device="cpu", cache_dtype=E4M3, key_layout="rows")
+
+
+def test_layout_refusals():
+    k, v, s = tensors()
+    assert ops.kv_layout_e4m3(k, v.view(E4M3), s, torch.bfloat16).num_blocks == 3
+    bad = [(k.int(), v, s), (k, v.float(), s), (k, v, s.int()), (k[0], v, s), (k, v[:, :, :, :32], s), (k[:, :, :, :8], v, s),
+           (k, v, s[:, :, :1]), (k, v, s[:, :1]), (k[:2], v, s), (k.transpose(2, 3).contiguous().transpose(2, 3), v, s),
+           (k, v, torch.zeros(3, 2, 2, 32, dtype=torch.uint8)[..., ::2]), tensors(hd=272), tensors(bs=6)]
+    for args in bad:
+        with pytest.raises(ValueError, match="8-bit pool"):
+            ops.kv_layout_e4m3(*args, torch.bfloat16)
+    with pytest.raises(ValueError, match="dtype"):
+        ops.kv_layout_e4m3(k, v, s, torch.int8)
+
+
+def test_calls_refuse_bad_layouts():
+    """The C calls check a pool of codes before anything is launched."""
+    if not os.path.exists(LIB):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    k, v, s = tensors()
+    good = ops.kv_layout_e4m3(k, v, s, torch.bfloat16)
+
+    def calls(lay):
+        p = ctypes.byref(lay)
+        return [lib.fs_paged_kv_write(16, 16, 0, 0, 0, 0, 1, 16, 16, 4, 4, p, None),
+                lib.fs_paged_gather(p, 16, 4, 0, 4, 16, 16, None),
+                lib.fs_qkv_rope_write(16, 4096, 0, 1, 4, 16, None, 16, 16, 8, 16, 4, 4, p, 16, 4096, None),
+                lib.fs_paged_attention(16, 0, 0, 0, p, 16, 4, 4, 16, 1, 1, 4, 1.0, 16, 0, 0, 0, 256, 0, None)]
+
+    assert calls(good)[:3] == [0, 0, 0]   # (nothing to do: no rows)
+    for field, value in [("dtype", 19), ("head_dim", 72), ("head_dim", 272), ("block_size", 6), ("k_block", 8), ("v_head", 4),
+                         ("k_group", 0), ("k_slot", 2), ("v_dim", 4), ("v_slot", 1), ("num_blocks", 0),
+                         ("k", good.k + 8), ("v", good.v + 4), ("k_group", good.k_group + 2)]:
+        lay = _lib.KVLayout.from_buffer_copy(good)
+        setattr(lay, field, value)
+        assert calls(lay) == [-1] * 4, field
+    # an aligned gather's outputs must be aligned too; the workspace is still checked
+    assert lib.fs_paged_gather(ctypes.byref(good), 16, 4, 1, 4, 8, 16, None) == -1 and b"aligned" in lib.fs_last_error()
+    assert calls(good)[3] == -1 and b"workspace" in lib.fs_last_error()
+
+
+def test_rows_of_another_dtype_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "require_device", lambda *t: None)
+    k, v, s = tensors()
+    lay = ops.kv_layout_e4m3(k, v, s, torch.bfloat16)
+    x, i = torch.zeros(1, 512, dtype=torch.float16), torch.zeros(1, 4, dtype=torch.int32)
+    f = torch.zeros(8, 32)
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.qkv_rope_write(x, i[0, :1], 1, 4, f, f, i, lay)
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.qkv_rope_write_varlen(x, i[0, :1], i[0, :1], 4, f, f, i, lay)
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.paged_kv_write(x.view(1, 2, 4, 64), x.view(1, 2, 4, 64), i, i, lay)
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.paged_gather(lay, i, torch.float32, "cpu")
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.paged_attention(x.view(1, 1, 8, 64), lay, i, i[:, :1], 1.0)
+    with pytest.raises(ValueError, match="another dtype"):
+        ops.paged_attention_varlen(x.view(1, 8, 64), lay, i, i[:, :1], i[0, :2], 1.0)
