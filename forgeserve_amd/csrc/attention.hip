@@ -502,8 +502,8 @@ FS_DEVICE float fold_value(float x, float cM, float y, float cm) { return fmaf(x
 // Two waves on a CU (four parts) want two (3 rows of 8000-30000 keys: 68 -> 64 us); four want one (16 rows of
 // 128-1280 keys, 64 dims: 12.3 against 13.4). The last pair is consumed with nothing left to load: prefetching
 // past the end cost 64 rows of 1000-2000 keys 7 us.
-constexpr int UNIT_PAIRS = 1;
-constexpr int part_pairs(int parts) { return parts == 4 ? 2 : 1; }
+constexpr int unit_pairs(int store) { return store == FS_BF16 ? 1 : 2; }
+constexpr int part_pairs(int store, int parts) { return store == FS_BF16 ? (parts == 4 ? 2 : 1) : (parts == 4 ? 4 : 2); }
 
 // TWO: the tile has a second 16-row half. NP: pair buffers in registers.
 template <int D, int BSZ, bool TWO, int NP>
@@ -702,11 +702,18 @@ __device__ __attribute__((always_inline)) inline void attn_wave_tiles(const Attn
   }
 }
 
+}  // namespace
+
+#include "attention_e4m3.h"
+
+namespace {
+
 // Row `rr` of the query rows (token rr / G, head hkv*G + rr % G), dims 16*(mt + i) + 4g .. +4 for i < N, from its
 // folded chunk-s state (M, L, o): a query that sees one chunk only is finished here (a padding query,
 // position < 0, gets zeros from chunk 0); any other query gets this chunk's partial for attn_combine
 // if the chunk holds keys it sees.
-template <int D, int N>
+// ST: the pool's dtype; over codes the row may be f16, and a NaN stays one.
+template <int D, int N, int ST = FS_BF16>
 FS_DEVICE void attn_emit(const AttnParams& P, int b, int s, int kbeg, int hkv, int rr, int rp, int mt, float M,
                          float L, const float4_t (&o)[N]) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -718,8 +725,19 @@ FS_DEVICE void attn_emit(const AttnParams& P, int b, int s, int kbeg, int hkv, i
     // o / L, rounded to bf16. o times L's reciprocal, which the row's outputs share, is within 2 ulps of it, and rounds
     // to the same bf16 unless a tie is that near: then the wave divides (one time in thirty for N = 1, in nine for
     // 4). Prompts of 817-4096 tokens: every output divided 402 us, products with N = 1 397, with N = 4 362.
-    const float inv = 1.f / L;
     float f[N][4];
+    uint16_t* orow = reinterpret_cast<uint16_t*>(P.out) + o_offset(P, b, t, P.o_sb, P.o_st) + (int64_t)h * P.o_sh;
+    if constexpr (ST == (FS_F16 | FS_STORE_E4M3)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[i][c] = L == 0.f ? 0.f : o[i][c] / L;
+        *reinterpret_cast<u32x2_t*>(orow + 16 * (mt + i) + 4 * g) =
+            u32x2_t{Operand<FS_F16>::round2(f[i][0], f[i][1]), Operand<FS_F16>::round2(f[i][2], f[i][3])};
+      }
+      return;
+    }
+    const float inv = 1.f / L;
     uint16_t near = 0xffff;   // the products' smallest distance above four ulps below a tie
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -732,9 +750,8 @@ FS_DEVICE void attn_emit(const AttnParams& P, int b, int s, int kbeg, int hkv, i
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) f[i][c] = L > 0.f ? o[i][c] / L : 0.f;
+        for (int c = 0; c < 4; ++c) f[i][c] = L > 0.f || ((ST & FS_STORE_E4M3) && L != 0.f) ? o[i][c] / L : 0.f;
     }
-    uint16_t* orow = reinterpret_cast<uint16_t*>(P.out) + o_offset(P, b, t, P.o_sb, P.o_st) + (int64_t)h * P.o_sh;
 #pragma unroll
     for (int i = 0; i < N; ++i) *reinterpret_cast<short4_t*>(orow + 16 * (mt + i) + 4 * g) = bf16_rne4(f[i]);
     return;
@@ -750,7 +767,19 @@ FS_DEVICE void attn_emit(const AttnParams& P, int b, int s, int kbeg, int hkv, i
   }
 }
 
-template <int D, int BSZ, bool TWO>
+// The share of class w of a unit, by the pool's dtype (ST).
+template <int ST, int D, int BSZ, bool TWO, int NP>
+__device__ __attribute__((always_inline)) inline void wave_tiles(const AttnParams& P, int b, int kbeg, int kend, int qmax,
+                                                                 int row0, int nrows, const int (&rpos)[2], int hkv, int w,
+                                                                 float4_t (*red_acc)[64], float* red_m, float* red_l) {
+  if constexpr (ST == FS_BF16)
+    attn_wave_tiles<D, BSZ, TWO, NP>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc, red_m, red_l);
+  else
+    attn_wave_tiles_e4m3<ST & ~FS_STORE_E4M3, D, BSZ, TWO, NP>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc,
+                                                               red_m, red_l);
+}
+
+template <int ST, int D, int BSZ, bool TWO>
 __global__ void __launch_bounds__(64 * UNIT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 attn_unit_kernel(AttnParams P) {
   constexpr int MT = D / 16, NG = (TWO ? 2 : 1) * MT;
@@ -777,7 +806,7 @@ attn_unit_kernel(AttnParams P) {
   const int kbeg = s * P.split;
   const int kend = min(kbeg + P.split, qmax + 1);
 
-  attn_wave_tiles<D, BSZ, TWO, UNIT_PAIRS>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc[w], red_m[w], red_l[w]);
+  wave_tiles<ST, D, BSZ, TWO, unit_pairs(ST)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc[w], red_m[w], red_l[w]);
   __syncthreads();
 
   // fold the waves' partials in wave order; wave w takes the (query half, 16-dim tile) pairs w,
@@ -798,7 +827,7 @@ attn_unit_kernel(AttnParams P) {
       for (int c = 0; c < 4; ++c) o[c] = fold_value(o[c], cM, a[c], cm);
       M = Mn;
     }
-    attn_emit<D, 1>(P, b, s, kbeg, hkv, row0 + r, rpos[nt], mt, M, L, {o});
+    attn_emit<D, 1, ST>(P, b, s, kbeg, hkv, row0 + r, rpos[nt], mt, M, L, {o});
   }
 }
 
@@ -830,7 +859,7 @@ FS_DEVICE float ld1_dev(__amdgpu_buffer_rsrc_t r, int off) {
 // its classes folded, (M, L, O), every other part its class partials one by one, and the part that arrives
 // last folds them in order and emits the rows. The arrival is counted (an agent-scope atomic), never awaited;
 // the published values cross XCDs through device-coherent accesses.
-template <int D, int BSZ, bool TWO, int PARTS>
+template <int ST, int D, int BSZ, bool TWO, int PARTS>
 __global__ void __launch_bounds__(64 * UNIT_WAVES / PARTS) __attribute__((amdgpu_waves_per_eu(1)))
 attn_unit_part_kernel(AttnParams P) {
   constexpr int WPP = UNIT_WAVES / PARTS;
@@ -864,8 +893,8 @@ attn_unit_part_kernel(AttnParams P) {
   const int kbeg = s * P.split;
   const int kend = min(kbeg + P.split, qmax + 1);
 
-  attn_wave_tiles<D, BSZ, TWO, part_pairs(PARTS)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, WPP * part + w,
-                                                         red_acc[w], red_m[w], red_l[w]);
+  wave_tiles<ST, D, BSZ, TWO, part_pairs(ST, PARTS)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, WPP * part + w,
+                                                     red_acc[w], red_m[w], red_l[w]);
   __syncthreads();
 
   // this unit's published partials, SLOT floats each
@@ -933,7 +962,7 @@ attn_unit_part_kernel(AttnParams P) {
       for (int c = 0; c < 4; ++c) o[c] = fold_value(o[c], cM, a[v][c], cm);
       M = Mn;
     }
-    if (r < nrows) attn_emit<D, 1>(P, b, s, kbeg, hkv, row0 + r, nt ? rpos[1] : rpos[0], mt, M, L, {o});
+    if (r < nrows) attn_emit<D, 1, ST>(P, b, s, kbeg, hkv, row0 + r, nt ? rpos[1] : rpos[0], mt, M, L, {o});
   }
 }
 
@@ -1676,6 +1705,9 @@ __global__ void __launch_bounds__(64 * COMBINE_ROWS) attn_combine_kernel(AttnPar
 }
 
 bool mfma_eligible(const fs_kv_layout& kv, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh) {
+  if (stores_e4m3(kv))   // (check_e4m3_layout has seen to the pool)
+    return row_dtype(kv) != FS_F32 && (kv.head_dim == 64 || kv.head_dim == 128) && kv.block_size % 16 == 0 &&
+           (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ((q_sb | q_st | q_sh) & 7) == 0;
   if (kv.dtype != FS_BF16) return false;
   if (kv.head_dim != 64 && kv.head_dim != 128) return false;
   if (kv.block_size % 16 != 0) return false;  // a 16-key tile never straddles two blocks
@@ -1837,7 +1869,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
   P.row_start = row_start;
   const int64_t qtiles = ((int64_t)T * P.G + QTILE - 1) / QTILE;
   // many query tiles per row (a prompt): groups of PF_WAVES tiles share their key/value reads
-  const bool prefill = mfma && qtiles >= PF_MIN_QTILES;
+  const bool prefill = mfma && qtiles >= PF_MIN_QTILES && !e4m3;
   P.zgroup = prefill ? PF_WAVES : 1;
 
   hipStream_t st = fs::as_stream(stream);
@@ -1878,21 +1910,28 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
       const bool two = (int64_t)T * P.G > 16;   // else no tile has a second half of query rows
       const int parts = split_parts(units, (int64_t)max_blocks * kv->block_size, two);
       const unsigned pgrid = grid * (unsigned)parts, pthreads = 64 * UNIT_WAVES / (unsigned)parts;
-#define FS_ATTN_LAUNCH(D_, BS_, TWO_)                                                     \
-  do {                                                                                    \
-    if (parts == 4) attn_unit_part_kernel<D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
-    else if (parts == 2) attn_unit_part_kernel<D_, BS_, TWO_, 2><<<pgrid, pthreads, 0, st>>>(P); \
-    else attn_unit_kernel<D_, BS_, TWO_><<<grid, 64 * UNIT_WAVES, 0, st>>>(P);                   \
+#define FS_ATTN_LAUNCH(ST_, D_, BS_, TWO_)                                                     \
+  do {                                                                                         \
+    if (parts == 4) attn_unit_part_kernel<ST_, D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
+    else if (parts == 2) attn_unit_part_kernel<ST_, D_, BS_, TWO_, 2><<<pgrid, pthreads, 0, st>>>(P); \
+    else attn_unit_kernel<ST_, D_, BS_, TWO_><<<grid, 64 * UNIT_WAVES, 0, st>>>(P);              \
   } while (0)
-#define FS_ATTN_LAUNCH_D(D_)                                                              \
+#define FS_ATTN_LAUNCH_D(ST_, D_)                                                         \
   do {                                                                                    \
-    if (bs16 && two) FS_ATTN_LAUNCH(D_, 16, true);                                        \
-    else if (bs16) FS_ATTN_LAUNCH(D_, 16, false);                                         \
-    else if (two) FS_ATTN_LAUNCH(D_, 0, true);                                            \
-    else FS_ATTN_LAUNCH(D_, 0, false);                                                    \
+    if (bs16 && two) FS_ATTN_LAUNCH(ST_, D_, 16, true);                                   \
+    else if (bs16) FS_ATTN_LAUNCH(ST_, D_, 16, false);                                    \
+    else if (two) FS_ATTN_LAUNCH(ST_, D_, 0, true);                                       \
+    else FS_ATTN_LAUNCH(ST_, D_, 0, false);                                               \
   } while (0)
-      if (kv->head_dim == 128) FS_ATTN_LAUNCH_D(128);
-      else FS_ATTN_LAUNCH_D(64);
+#define FS_ATTN_LAUNCH_ST(ST_)                                                            \
+  do {                                                                                    \
+    if (kv->head_dim == 128) FS_ATTN_LAUNCH_D(ST_, 128);                                  \
+    else FS_ATTN_LAUNCH_D(ST_, 64);                                                       \
+  } while (0)
+      if (kv->dtype == FS_BF16) FS_ATTN_LAUNCH_ST(FS_BF16);
+      else if (dtype == FS_BF16) FS_ATTN_LAUNCH_ST(FS_BF16 | FS_STORE_E4M3);
+      else FS_ATTN_LAUNCH_ST(FS_F16 | FS_STORE_E4M3);
+#undef FS_ATTN_LAUNCH_ST
 #undef FS_ATTN_LAUNCH_D
 #undef FS_ATTN_LAUNCH
     }
