@@ -1000,6 +1000,11 @@ FS_DEVICE void pf_dma16(const void* sbase, uint32_t voff, uint32_t lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(l) : "memory", "m0");
 }
+// 4 bytes per lane from an address of its own; lane l lands at lds + 4 * l.
+FS_DEVICE void pf_dma4(const void* src, uint32_t lds) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(l) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 template <int N>
 FS_DEVICE void pf_wait_vm() {
@@ -1270,6 +1275,12 @@ attn_prefill_kernel(AttnParams P) {
                       {O[mt][nt], O[mt + 1][nt], O[mt + 2][nt], O[mt + 3][nt]});
   }
 }
+
+}  // namespace
+
+#include "attention_prefill_e4m3.h"
+
+namespace {
 
 // ------------------------------------------------------------------------------------------------
 // generic kernel (any dtype, head_dim <= 256, any strides and block size)
@@ -1869,7 +1880,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
   P.row_start = row_start;
   const int64_t qtiles = ((int64_t)T * P.G + QTILE - 1) / QTILE;
   // many query tiles per row (a prompt): groups of PF_WAVES tiles share their key/value reads
-  const bool prefill = mfma && qtiles >= PF_MIN_QTILES && !e4m3;
+  const bool prefill = mfma && qtiles >= PF_MIN_QTILES;
   P.zgroup = prefill ? PF_WAVES : 1;
 
   hipStream_t st = fs::as_stream(stream);
@@ -1898,13 +1909,22 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
     const unsigned grid = (unsigned)units;
     if (prefill) {
       const unsigned threads = 64 * PF_WAVES;
-      if (kv->head_dim == 128) {
-        if (bs16) attn_prefill_kernel<128, 16><<<grid, threads, 0, st>>>(P);
-        else attn_prefill_kernel<128, 0><<<grid, threads, 0, st>>>(P);
-      } else {
-        if (bs16) attn_prefill_kernel<64, 16><<<grid, threads, 0, st>>>(P);
-        else attn_prefill_kernel<64, 0><<<grid, threads, 0, st>>>(P);
-      }
+#define FS_PREFILL(KERNEL, ...)                                                        \
+  do {                                                                                 \
+    if (kv->head_dim == 128) {                                                         \
+      if (bs16) KERNEL<__VA_ARGS__ 128, 16><<<grid, threads, 0, st>>>(P);              \
+      else KERNEL<__VA_ARGS__ 128, 0><<<grid, threads, 0, st>>>(P);                    \
+    } else {                                                                           \
+      if (bs16) KERNEL<__VA_ARGS__ 64, 16><<<grid, threads, 0, st>>>(P);               \
+      else KERNEL<__VA_ARGS__ 64, 0><<<grid, threads, 0, st>>>(P);                     \
+    }                                                                                  \
+  } while (0)
+#define FS_COMMA ,
+      if (!e4m3) FS_PREFILL(attn_prefill_kernel, );
+      else if (dtype == FS_BF16) FS_PREFILL(attn_prefill_e4m3_kernel, FS_BF16 FS_COMMA);
+      else FS_PREFILL(attn_prefill_e4m3_kernel, FS_F16 FS_COMMA);
+#undef FS_COMMA
+#undef FS_PREFILL
     } else {
       // few, possibly long units: several workgroups each, to keep more CUs reading
       const bool two = (int64_t)T * P.G > 16;   // else no tile has a second half of query rows
