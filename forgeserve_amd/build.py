@@ -28,7 +28,7 @@ FLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
 
-SOURCES = ["abi.hip", "kv.hip", "kv_e4m3.hip", "attention.hip", "norm.hip", "gemm.hip", "gemm_f32.hip", "sample.hip", "rng.hip",
+SOURCES = ["abi.hip", "kv.hip", "kv_e4m3.hip", "attention.hip", "norm.hip", "gemm.hip", "gemm_f32.hip", "gemm_e4m3.hip", "sample.hip", "rng.hip",
            "blocks.hip"]
 
 

@@ -1,0 +1,580 @@
+// Projections in 8-bit floating point: C[M,N] = X[M,K] . W[N,K]^T (+ R), W held as e4m3 codes with a power of two per row
+// and 128 of K as their scale, X (bf16 or f16) brought to the same form within the call (e4m3.h has the format).
+//
+//   C[m][n] = round(sum over groups g of 2^(ex[m][g] + ew[n][g] - 254) * sum over k in g of cx[m][k] cw[n][k] (+ R[m][n]))
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 128 of K at a time and applies both scales itself, so a group is one
+// instruction's depth, the chain of a sum over K stays in one f32 accumulator, and the only roundings are the codes', the
+// sum's and the result's (product and residual together, once). One such product is within 2.5e-5 of its operands' norm
+// of the exact one (measured; the matrix core aligns its 128 products before it adds them), far below a 16-bit result's
+// half step, which is why 32-bit results are not offered.
+//
+// The scales of a matrix of r rows lie as [ceil(K / 512)][r][4]: a word per row holds four groups' bytes, one per stage
+// of 128, and the words of consecutive rows lie side by side.
+//
+// The kernel depends on M (the sums' order over K with it, so a row's last bit may differ between a short and a long
+// batch): up to 16 rows one launch does everything; beyond that X is encoded first, then multiplied in LDS-fed tiles.
+#include "e4m3.h"
+
+namespace {
+
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((__vector_size__(2 * sizeof(short)))) short s16x2_t;
+typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2_t;
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
+
+constexpr int GROUP = 128;        // K per scale, and per matrix instruction
+constexpr int SHORT_ROWS = 16;    // rows that one launch takes
+
+// D = A . B^T of 16 x 128 codes each: a lane holds 32 of its row's (two 16-byte chunks: any two, the same for A and B).
+// BYTE: which of the four groups in the scale words.
+template <int BYTE>
+FS_DEVICE float4_t mfma_codes(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, float4_t c, uint32_t sa, uint32_t sb) {
+  struct Two { u32x4 x, y; };
+  const Two a = {a0, a1}, b = {b0, b1};
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(float4_t, __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                          __builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b),
+                                          __builtin_bit_cast(f32x4, c), 0, 0, BYTE, (int)sa, BYTE, (int)sb));
+}
+
+// ------------------------------------------------------------------------------------------------
+// encoding rows of 16-bit values
+// ------------------------------------------------------------------------------------------------
+// Largest |x| of N words of two 16-bit values each, as bits (both types' magnitudes order as integers do).
+template <int N>
+FS_DEVICE uint32_t magnitude_bits(const uint32_t (&w)[N]) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  return m[0] > m[1] ? m[0] : m[1];
+}
+template <int DT>
+FS_DEVICE float half_of(uint32_t w, int hi) { return Elem<DT>::to_f32((uint16_t)(w >> (16 * hi))); }
+
+// Magnitudes above this are not finite, or (bf16) more than the largest scale's 448.
+template <int DT> constexpr uint32_t LARGEST = DT == FS_BF16 ? 0x7f60u : 0x7bffu;
+
+// The exponent byte of a group whose largest magnitude has these bits (at most LARGEST).
+template <int DT>
+FS_DEVICE int exponent_of_bits(uint32_t m) {
+  return scale_exponent<FS_F32>(Elem<DT>::to_f32((uint16_t)m));
+}
+
+// Two 16-bit values' codes under the scale 2^(e - 127) = s: one conversion, which divides by the scale and rounds to
+// nearest even (each bf16 and f16 gives the definition's code).
+template <int DT, bool HI>
+FS_DEVICE s16x2_t encode_pair(s16x2_t old, uint32_t w, float s) {
+  typedef short v2s __attribute__((ext_vector_type(2)));
+  if constexpr (DT == FS_BF16) {
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(s16x2_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(v2s, old),
+                                                                                 __builtin_bit_cast(v2b, w), s, HI));
+  } else {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(s16x2_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(v2s, old),
+                                                                                __builtin_bit_cast(v2h, w), s, HI));
+  }
+}
+// Four values' codes. FAR: some of the wave's are above LARGEST (saturated, or NaN where not finite).
+template <int DT>
+FS_DEVICE uint32_t encode_words(uint32_t a, uint32_t b, int e, bool far) {
+  if (far) return encode4(half_of<DT>(a, 0), half_of<DT>(a, 1), half_of<DT>(b, 0), half_of<DT>(b, 1), scale_inverse(e));
+  const float s = scale_value(e);
+  s16x2_t c = {0, 0};
+  c = encode_pair<DT, false>(c, a, s);
+  c = encode_pair<DT, true>(c, b, s);
+  return __builtin_bit_cast(uint32_t, c);
+}
+// Largest finite magnitude of N words.
+template <int DT, int N>
+FS_DEVICE float finite_max(const uint32_t (&w)[N]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fmaxf(finite_magnitude(half_of<DT>(w[i], 0)), finite_magnitude(half_of<DT>(w[i], 1))));
+  return m;
+}
+
+// A wave per 512 columns of a row: 16 lanes of 8 values share a group. VEC: rows of aligned 16-byte pieces.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) quantize_e4m3_kernel(const typename Elem<DT>::T* __restrict__ X, int64_t ldx,
+                                                            int64_t rows, int64_t K, uint8_t* __restrict__ codes,
+                                                            int64_t ldc, uint32_t* __restrict__ scales, int64_t kw) {
+  typedef Elem<DT> E;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= rows * kw) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = unit / kw, k4 = unit - row * kw, k = k4 * 512 + lane * 8;
+  const bool in = k < K;   // (whole groups: K % 128 == 0)
+  float v[8];
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  int e;
+  u32x2_t out;
+  if constexpr (DT == FS_F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = in ? E::load(X, row * ldx + k + j) : 0.f;
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_magnitude(v[j]));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    e = scale_exponent<FS_F32>(m);
+    const float inv = scale_inverse(e);
+    out = u32x2_t{encode4(v[0], v[1], v[2], v[3], inv), encode4(v[4], v[5], v[6], v[7], inv)};
+  } else {
+    if (in) {
+      if (VEC) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(X + row * ldx + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = x[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = (uint32_t)X[row * ldx + k + 2 * j] | ((uint32_t)X[row * ldx + k + 2 * j + 1] << 16);
+      }
+    }
+    uint32_t m = magnitude_bits(w);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    const bool far = __any(m > LARGEST<DT>);
+    if (far) {
+      float f = finite_max<DT>(w);
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) f = fmaxf(f, __shfl_xor(f, o, 64));
+      e = scale_exponent<FS_F32>(f);
+    } else {
+      e = exponent_of_bits<DT>(m);
+    }
+    out = u32x2_t{encode_words<DT>(w[0], w[1], e, far), encode_words<DT>(w[2], w[3], e, far)};
+  }
+  if (in) *reinterpret_cast<u32x2_t*>(codes + row * ldc + k) = out;
+  // the row's word: lane 16 g holds byte g (zeros past K)
+  uint32_t word = (lane & 15) == 0 && in ? (uint32_t)e << (8 * (lane >> 4)) : 0u;
+  word |= (uint32_t)__shfl_xor((int)word, 16, 64);
+  word |= (uint32_t)__shfl_xor((int)word, 32, 64);
+  if (lane == 0) scales[k4 * rows + row] = word;
+}
+
+// ------------------------------------------------------------------------------------------------
+// results
+// ------------------------------------------------------------------------------------------------
+// Four finished columns C[row][col0 ..]: the residual added in f32, rounded once.
+template <int DT>
+FS_DEVICE void store_row4(float4_t a, int64_t row, int64_t col0, uint16_t* C, int64_t ldc, const uint16_t* R, int64_t ldr,
+                          int64_t N, bool vec) {
+  if (vec && col0 + 4 <= N) {
+    if (R) {
+      const u32x2_t r = *reinterpret_cast<const u32x2_t*>(R + row * ldr + col0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] += half_of<DT>(r[e >> 1], e & 1);
+    }
+    *reinterpret_cast<u32x2_t*>(C + row * ldc + col0) =
+        u32x2_t{(uint32_t)Elem<DT>::store_bits(a[0]) | ((uint32_t)Elem<DT>::store_bits(a[1]) << 16),
+                (uint32_t)Elem<DT>::store_bits(a[2]) | ((uint32_t)Elem<DT>::store_bits(a[3]) << 16)};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (col0 + e < N) C[row * ldc + col0 + e] = Elem<DT>::store_bits(R ? a[e] + Elem<DT>::to_f32(R[row * ldr + col0 + e]) : a[e]);
+}
+// Whether rows of C (and R) can be stored and read eight bytes at a time.
+inline bool rows_by_8(const void* C, int64_t ldc, const void* R, int64_t ldr) {
+  return ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(R)) & 7) == 0 && ldc % 4 == 0 && (!R || ldr % 4 == 0);
+}
+
+// ------------------------------------------------------------------------------------------------
+// up to 16 rows: one launch, bound by the weights' bytes
+// ------------------------------------------------------------------------------------------------
+// A workgroup takes 16 TN columns of C; its eight waves split K and are joined in order through LDS. Weights go straight
+// from HBM to registers in the instruction's own shape (a lane's two 16-byte chunks of a row's 128; a wave's load covers
+// whole lines), DEPTH stages ahead. Each wave encodes its part of the rows itself while its weights are on their way:
+// 32 values a lane and stage, 16 words of magnitudes and 16 conversions.
+template <int DT, int TN, int DEPTH>
+__global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __restrict__ X, int64_t ldx,
+                                                              const uint8_t* __restrict__ W, int64_t ldw,
+                                                              const uint8_t* __restrict__ wsc, uint16_t* __restrict__ C,
+                                                              int64_t ldc, const uint16_t* __restrict__ R, int64_t ldr,
+                                                              int M, int64_t N, int nk, bool vec) {
+  __shared__ float4_t red[8][TN][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * TN);
+  const int k0 = (int)((int64_t)w * nk / 8), k1 = (int)((int64_t)(w + 1) * nk / 8);
+  struct Stage {
+    u32x4 c[TN][2];
+    uint32_t s[TN];
+  } ring[DEPTH];
+  const uint8_t* wrow[TN];
+  int64_t srow[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t n = min(n0 + 16 * j + l16, N - 1);
+    wrow[j] = W + n * ldw + 16 * g;
+    srow[j] = 4 * n;
+  }
+  auto load = [&](int kt, Stage& x) {
+    const int k = min(kt, nk - 1);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      x.c[j][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP));
+      x.c[j][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP + 64));
+      x.s[j] = wsc[(int64_t)(k >> 2) * 4 * N + srow[j] + (k & 3)];
+    }
+  };
+  // the row's values of stage kt: chunks g and 4 + g of 16
+  const bool row_in = l16 < M;
+  const uint16_t* xrow = X + (row_in ? l16 : 0) * ldx + 16 * g;
+  auto load_x = [&](int kt, uint32_t (&x)[16]) {
+    const int k = min(kt, nk - 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 v = *reinterpret_cast<const u32x4*>(xrow + (int64_t)k * GROUP + 64 * (i >> 1) + 8 * (i & 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = row_in ? v[e] : 0u;
+    }
+  };
+  uint32_t xn[16];
+  load_x(k0, xn);
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) load(k0 + d, ring[d]);
+  float4_t acc[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int kt = k0; kt < k1; kt += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (kt + d >= k1) break;   // (wave-uniform)
+      uint32_t m = magnitude_bits(xn);
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+      int e = exponent_of_bits<DT>(m);
+      const bool far = __any(m > LARGEST<DT>);
+      if (far) {
+        float f = finite_max<DT>(xn);
+        f = fmaxf(f, __shfl_xor(f, 16, 64));
+        f = fmaxf(f, __shfl_xor(f, 32, 64));
+        e = scale_exponent<FS_F32>(f);
+      }
+      u32x4 xc[2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) xc[i >> 2][i & 3] = encode_words<DT>(xn[2 * i], xn[2 * i + 1], e, far);
+      load_x(kt + d + 1, xn);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[j] = mfma_codes<0>(ring[d].c[j][0], ring[d].c[j][1], xc[0], xc[1], acc[j], ring[d].s[j], (uint32_t)e);
+      load(kt + d + DEPTH, ring[d]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < TN; ++j) red[w][j][lane] = acc[j];
+  __syncthreads();
+  if (w >= TN) return;
+  // wave j joins its columns' eight sums in order: lane (l16, g) has row l16, columns 16 j + 4 g ..
+  float4_t a = red[0][w][lane];
+#pragma unroll
+  for (int v = 1; v < 8; ++v) {
+    const float4_t b = red[v][w][lane];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] += b[r];
+  }
+  if (row_in) store_row4<DT>(a, l16, n0 + 16 * w + 4 * g, C, ldc, R, ldr, N, vec);
+}
+
+// ------------------------------------------------------------------------------------------------
+// LDS-fed tiles
+// ------------------------------------------------------------------------------------------------
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// Copies straight into LDS, 16 or 4 bytes a lane at a wave-uniform base plus the lane's offset; lane l lands at
+// lds + 16 l (4 l). Counted by vmcnt; the waits are explicit.
+FS_DEVICE void dma16_at(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+FS_DEVICE void dma4_at(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int N>
+FS_DEVICE void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Which tile a workgroup takes: workgroup ids go round the 8 XCDs; each gets a contiguous range of tiles, rows fastest
+// inside groups of at most 8 row tiles, so that the tiles it runs at once share their panels through its L2.
+FS_DEVICE bool tile_of(int tiles_m, int ntiles, int bm, int bn, int64_t& m0, int64_t& n0) {
+  const int per_xcd = (ntiles + 7) / 8;
+  const int tile = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+  if (tile >= ntiles) return false;
+  const int tiles_n = ntiles / tiles_m;
+  const int grp = tile / (8 * tiles_n), first = 8 * grp, gm = min(tiles_m - first, 8);
+  const int in_grp = tile - grp * 8 * tiles_n;
+  m0 = (int64_t)(first + in_grp % gm) * bm;
+  n0 = (int64_t)(in_grp / gm) * bn;
+  return true;
+}
+
+struct Operands {
+  const uint8_t *x, *w;          // codes
+  const uint8_t *xs, *ws;        // scale words
+  int64_t ldx, ldw;              // bytes from row to row
+  int64_t M, N;
+  int nk;                        // stages of 128
+  int tiles_m, ntiles;
+};
+
+// BM x BN tiles, WGM x WGN waves, NS stages of 128 in LDS, NS - 1 of them on their way. A stage's rows are 128 bytes,
+// their 16-byte chunks swapped by (row & 7), so that the operand reads meet no bank twice. The words of the rows' scales
+// come with every fourth stage (one copy per 64 rows), into one of two places.
+template <int DT, int BM, int BN, int WGM, int WGN, int NS>
+__global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands P, uint16_t* __restrict__ C, int64_t ldc,
+                                                                        const uint16_t* __restrict__ R, int64_t ldr,
+                                                                        bool vec, float* __restrict__ part) {
+  constexpr int NW = WGM * WGN, XB = BM * GROUP, STAGE = (BM + BN) * GROUP;
+  constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16;
+  constexpr int CPW = STAGE / 1024 / NW;               // copies of codes per wave and stage
+  constexpr int SW = (BM + BN) / 64;                   // copies of scale words per four stages
+  static_assert(STAGE / 1024 % NW == 0 && SW <= NW && BM % 64 == 0, "whole copies, evenly");
+  static_assert(NS >= 2 && NS <= 4, "wait_stages covers two stages behind the awaited one; scale words have two places");
+  __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
+  __shared__ __attribute__((aligned(256))) uint32_t words[2][BM + BN];
+  int64_t m0, n0;
+  if (!tile_of(P.tiles_m, P.ntiles, BM, BN, m0, n0)) return;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem, words0 = (uint32_t)(uintptr_t)words;
+  const int split = blockIdx.y, nk = P.nk / (int)gridDim.y, first = split * nk;   // (nk % 4 == 0 where K is split)
+  // copy q of a stage: rows 8 q .. of the X block, then of the W block; lane l takes row l >> 3, physical chunk l & 7
+  const int cr = lane >> 3;
+  const char* base[CPW];
+  uint32_t off[CPW];
+#pragma unroll
+  for (int i = 0; i < CPW; ++i) {
+    const int q = i * NW + wave, row = 8 * q + cr, c = (lane & 7) ^ (row & 7);
+    const bool in_x = 8 * q < BM;
+    const int64_t lead = in_x ? m0 : n0, last = (in_x ? P.M : P.N) - 1, ld = in_x ? P.ldx : P.ldw;
+    const int64_t r = min(lead + (in_x ? row : row - BM), last) - lead;
+    base[i] = reinterpret_cast<const char*>((in_x ? P.x : P.w) + lead * ld);
+    off[i] = (uint32_t)(r * ld + 16 * c);
+  }
+  const char* sbase = nullptr;
+  uint32_t soff = 0;
+  if (wave < SW) {
+    const bool in_x = 64 * wave < BM;
+    const int64_t lead = in_x ? m0 : n0, rows = in_x ? P.M : P.N;
+    const int64_t r = min(lead + (in_x ? 64 * wave : 64 * wave - BM) + lane, rows - 1);
+    sbase = reinterpret_cast<const char*>(in_x ? P.xs : P.ws);
+    soff = (uint32_t)(4 * r);
+  }
+  auto issue = [&](int kt) {   // kt: the split's stage
+    const int k = first + kt;
+    if ((k & 3) == 0 || kt == 0) {
+      if (wave < SW)
+        dma4_at(sbase + (int64_t)(k >> 2) * 4 * (64 * wave < BM ? P.M : P.N), soff,
+                words0 + (uint32_t)(4 * ((k >> 2 & 1) * (BM + BN) + 64 * wave)));
+    }
+    const uint32_t to = lds0 + (uint32_t)((kt % NS) * STAGE);
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) dma16_at(base[i] + (int64_t)k * GROUP, off[i], to + (uint32_t)((i * NW + wave) * 1024));
+  };
+  auto wait_stages = [&](int later) {   // (a copy of scale words among the later ones only makes the wait longer)
+    if (later >= 2) wait_vm<2 * CPW>();
+    else if (later == 1) wait_vm<CPW>();
+    else wait_vm<0>();
+  };
+  float4_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  uint32_t xs[TM], ws[TN];
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < nk) issue(s);
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_stages(min(NS - 2, nk - 1 - kt));
+    __syncthreads();   // stage kt has landed for every wave; stage kt-1 is no longer being read
+    if (kt + NS - 1 < nk) issue(kt + NS - 1);
+    const int k = first + kt;
+    if ((k & 3) == 0 || kt == 0) {
+      const uint32_t* p = words[k >> 2 & 1];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) xs[i] = p[wm * (BM / WGM) + 16 * i + l16];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) ws[j] = p[BM + wn * (BN / WGN) + 16 * j + l16];
+    }
+    const char* st = smem + (kt % NS) * STAGE;
+    u32x4 xf[TM][2], wf[TN][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r = wm * (BM / WGM) + 16 * i + l16;
+        xf[i][h] = *reinterpret_cast<const u32x4*>(st + r * GROUP + 16 * ((4 * h + g) ^ (r & 7)));
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int r = wn * (BN / WGN) + 16 * j + l16;
+        wf[j][h] = *reinterpret_cast<const u32x4*>(st + XB + r * GROUP + 16 * ((4 * h + g) ^ (r & 7)));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = mfma_codes<0>(wf[j][0], wf[j][1], xf[i][0], xf[i][1], acc[i][j], ws[j], xs[i]);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xs[i] >>= 8;   // the next group's byte
+#pragma unroll
+    for (int j = 0; j < TN; ++j) ws[j] >>= 8;
+  }
+  // acc[i][j]: lane (l16, g) holds C[16i + l16][16j + 4g + r]
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t row = m0 + wm * (BM / WGM) + 16 * i + l16;
+    if (row >= P.M) continue;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int64_t col0 = n0 + wn * (BN / WGN) + 16 * j + 4 * g;
+      if (part) {   // (N % 4 == 0)
+        if (col0 < P.N) *reinterpret_cast<float4_t*>(part + ((int64_t)split * P.M + row) * P.N + col0) = acc[i][j];
+      } else {
+        store_row4<DT>(acc[i][j], row, col0, C, ldc, R, ldr, P.N, vec);
+      }
+    }
+  }
+}
+
+// C = round(sum of the splits' partials in order (+ R)), four columns a thread.
+template <int DT>
+__global__ void __launch_bounds__(256) gemm_e4m3_join_kernel(const float* __restrict__ part, int splits, int64_t M, int64_t N,
+                                                             uint16_t* __restrict__ C, int64_t ldc,
+                                                             const uint16_t* __restrict__ R, int64_t ldr, bool vec) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= M * N) return;
+  const int64_t row = e / N;
+  float4_t a = *reinterpret_cast<const float4_t*>(part + e);
+  for (int s = 1; s < splits; ++s) {
+    const float4_t b = *reinterpret_cast<const float4_t*>(part + (int64_t)s * M * N + e);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] += b[r];
+  }
+  store_row4<DT>(a, row, e - row * N, C, ldc, R, ldr, N, vec);
+}
+
+struct Plan {
+  int bm, bn, splits;
+};
+// The tile and the K splits of a shape.
+Plan plan_for(int64_t M, int64_t N, int64_t K) {
+  const int bm = M <= 64 ? 64 : 128, bn = M <= 64 ? 64 : 128;
+  const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn), nk = K / GROUP;
+  int s = 1;
+  while (s < 8 && N % 4 == 0 && tiles * s * 2 <= 512 && nk % (8 * s) == 0 && nk / (2 * s) >= 4) s *= 2;
+  return Plan{bm, bn, s};
+}
+
+int64_t scale_bytes(int64_t rows, int64_t K) { return (K + 511) / 512 * rows * 4; }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool short_call(int64_t M, const void* X, int64_t ldx) { return M <= SHORT_ROWS && al16(X) && ldx % 8 == 0; }
+
+void quantize(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, uint8_t* codes, int64_t ldc, uint32_t* scales,
+              hipStream_t s) {
+  const int64_t kw = (K + 511) / 512;
+  const dim3 grid((unsigned)((rows * kw + 3) / 4));
+  const bool vec = al16(X) && ldx % 8 == 0;
+  if (dtype == FS_F32)
+    quantize_e4m3_kernel<FS_F32, false><<<grid, 256, 0, s>>>((const float*)X, ldx, rows, K, codes, ldc, scales, kw);
+  else if (dtype == FS_BF16 && vec)
+    quantize_e4m3_kernel<FS_BF16, true><<<grid, 256, 0, s>>>((const uint16_t*)X, ldx, rows, K, codes, ldc, scales, kw);
+  else if (dtype == FS_BF16)
+    quantize_e4m3_kernel<FS_BF16, false><<<grid, 256, 0, s>>>((const uint16_t*)X, ldx, rows, K, codes, ldc, scales, kw);
+  else if (vec)
+    quantize_e4m3_kernel<FS_F16, true><<<grid, 256, 0, s>>>((const uint16_t*)X, ldx, rows, K, codes, ldc, scales, kw);
+  else
+    quantize_e4m3_kernel<FS_F16, false><<<grid, 256, 0, s>>>((const uint16_t*)X, ldx, rows, K, codes, ldc, scales, kw);
+}
+
+template <int DT>
+int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* ws, uint16_t* C, int64_t ldc,
+         const uint16_t* R, int64_t ldr, int64_t M, int64_t N, int64_t K, char* work, hipStream_t s) {
+  const bool vec = rows_by_8(C, ldc, R, ldr);
+  const int nk = (int)(K / GROUP);
+  if (short_call(M, X, ldx)) {
+    if (N <= 8192)
+      gemm_e4m3_short_kernel<DT, 1, 4><<<dim3((unsigned)((N + 15) / 16)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, R, ldr, (int)M,
+                                                                                     N, nk, vec);
+    else
+      gemm_e4m3_short_kernel<DT, 4, 2><<<dim3((unsigned)((N + 63) / 64)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, R, ldr, (int)M,
+                                                                                     N, nk, vec);
+    return fs::launch_status("gemm_e4m3");
+  }
+  uint8_t* codes = reinterpret_cast<uint8_t*>(work);
+  uint8_t* xs = codes + align256(M * K);
+  float* part = reinterpret_cast<float*>(xs + align256(scale_bytes(M, K)));
+  quantize(X, ldx, M, K, DT, codes, K, reinterpret_cast<uint32_t*>(xs), s);
+  const Plan p = plan_for(M, N, K);
+  Operands P{codes, W, xs, ws, K, ldw, M, N, nk, (int)((M + p.bm - 1) / p.bm), 0};
+  P.ntiles = P.tiles_m * (int)((N + p.bn - 1) / p.bn);
+  const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
+  float* out = p.splits > 1 ? part : nullptr;
+  if (p.bm == 64)
+    gemm_e4m3_tile_kernel<DT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, C, ldc, R, ldr, vec, out);
+  else
+    gemm_e4m3_tile_kernel<DT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
+  if (p.splits > 1) {
+    const int64_t n4 = M * N / 4;
+    gemm_e4m3_join_kernel<DT><<<dim3((unsigned)((n4 + 255) / 256)), 256, 0, s>>>(part, p.splits, M, N, C, ldc, R, ldr, vec);
+  }
+  return fs::launch_status("gemm_e4m3");
+}
+
+}  // namespace
+
+extern "C" int fs_quantize_e4m3(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, int64_t ldc,
+                                void* scales, void* stream) {
+  FS_CHECK_ARG(X && codes && scales, "quantize_e4m3: null pointer");
+  FS_CHECK_ARG(dtype == FS_F32 || dtype == FS_BF16 || dtype == FS_F16, "quantize_e4m3: dtype %d", dtype);
+  FS_CHECK_ARG(rows >= 0 && K > 0 && K % GROUP == 0 && ldx >= K && ldc >= K, "quantize_e4m3: rows %lld K %lld (a multiple of %d)",
+               (long long)rows, (long long)K, GROUP);
+  FS_CHECK_ARG(ldc % 16 == 0 && al16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
+               "quantize_e4m3: codes need 16-byte aligned rows, scales whole words");
+  FS_CHECK_ARG(rows * ((K + 511) / 512) < 0x7fffffffLL, "quantize_e4m3: rows %lld K %lld", (long long)rows, (long long)K);
+  if (rows == 0) return 0;
+  quantize(X, ldx, rows, K, dtype, reinterpret_cast<uint8_t*>(codes), ldc, reinterpret_cast<uint32_t*>(scales), fs::as_stream(stream));
+  return fs::launch_status("quantize_e4m3");
+}
+
+extern "C" int64_t fs_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % GROUP) return 0;
+  const Plan p = plan_for(M, N, K);
+  return align256(M * K) + align256(scale_bytes(M, K)) + (p.splits > 1 ? (int64_t)p.splits * M * N * (int64_t)sizeof(float) : 0);
+}
+
+extern "C" int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* w_scales, void* C, int64_t ldc,
+                            const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K, int32_t dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  FS_CHECK_ARG(X && W && w_scales && C, "gemm_e4m3: null pointer");
+  FS_CHECK_ARG(dtype == FS_BF16 || dtype == FS_F16, "gemm_e4m3: bf16 and f16 rows (dtype %d)", dtype);
+  FS_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K % GROUP == 0, "gemm_e4m3: M %lld N %lld K %lld (K a multiple of %d)", (long long)M,
+               (long long)N, (long long)K, GROUP);
+  FS_CHECK_ARG(ldx >= K && ldw >= K && ldc >= N && (!R || ldr >= N), "gemm_e4m3: leading dimensions");
+  FS_CHECK_ARG(ldw % 16 == 0 && al16(W) && (reinterpret_cast<uintptr_t>(w_scales) & 3) == 0,
+               "gemm_e4m3: codes need 16-byte aligned rows, scales whole words");
+  // a copy's offset inside its tile of rows, and a row's scale word inside its group of K, are 32 bits
+  FS_CHECK_ARG(K <= (1 << 22) && ldw < (1 << 23) && M < (1 << 29) && N < (1 << 29), "gemm_e4m3: M %lld N %lld K %lld ldw %lld",
+               (long long)M, (long long)N, (long long)K, (long long)ldw);
+  if (M == 0) return 0;
+  const int64_t need = fs_gemm_e4m3_workspace_size(M, N, K);
+  FS_CHECK_ARG(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+               "gemm_e4m3: workspace %lld < %lld bytes (or not 256-byte aligned)", (long long)workspace_bytes, (long long)need);
+  hipStream_t s = fs::as_stream(stream);
+  char* work = reinterpret_cast<char*>(workspace);
+  const auto call = dtype == FS_BF16 ? gemm<FS_BF16> : gemm<FS_F16>;
+  return call((const uint16_t*)X, ldx, (const uint8_t*)W, ldw, (const uint8_t*)w_scales, (uint16_t*)C, ldc, (const uint16_t*)R,
+              ldr, M, N, K, work, s);
+}

@@ -137,6 +137,61 @@ def gemm(a: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = None,
     return out
 
 
+def quantize_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x (rows, K) (float32, bfloat16, float16; K a multiple of 128) in 8-bit floating point: (codes, torch.float8_e4m3fn
+    (rows, K); scales, uint8 (ceil(K / 512), rows, 4)). Columns 128g .. of row r stand for
+    codes * 2^(scales[g // 4, r, g % 4] - 127): the smallest power of two that brings the group's largest magnitude to
+    448 or less, so a value is kept within 2^-4 of it (2^-19 of the group's largest, if it is below 2^-15 of that).
+    What is not finite becomes NaN."""
+    require_device(x)
+    m, ldx = _rows(x)
+    k = x.shape[1]
+    if k % 128 or k == 0:
+        raise ValueError(f"quantize_e4m3: K {k} is not a multiple of 128")
+    codes = torch.empty((m, k), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((-(-k // 512), m, 4), dtype=torch.uint8, device=x.device)
+    if m == 0:
+        return codes.view(torch.float8_e4m3fn), scales
+    check(_lib.load().fs_quantize_e4m3(ptr(x), ldx, m, k, _dt(x), ptr(codes), k, ptr(scales), stream_ptr()), "quantize_e4m3")
+    return codes.view(torch.float8_e4m3fn), scales
+
+
+def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Optional[torch.Tensor] = None,
+              residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out = a @ w.T (+ residual) with the weight in 8-bit floating point, as quantize_e4m3 leaves it (w (n, k) codes with
+    16-byte aligned rows, w_scales (ceil(k / 512), n, 4)), and a (bfloat16 or float16) brought to the same form within
+    the call: nn.Linear with half the weight bytes and twice the matrix rate of gemm's. Sums are float32; product and
+    residual are rounded once, to a's dtype. A row's last bit may depend on how many rows the call has."""
+    require_device(a, w, w_scales)
+    m, lda = _rows(a)
+    n, ldb = _rows(w)
+    k = a.shape[1]
+    if a.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"gemm_e4m3: rows must be bfloat16 or float16, not {a.dtype}")
+    if w.shape[1] != k or w.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        raise ValueError(f"gemm_e4m3: {tuple(a.shape)} x {tuple(w.shape)} {w.dtype}")
+    if w_scales.dtype != torch.uint8 or w_scales.shape != (-(-k // 512), n, 4) or not w_scales.is_contiguous():
+        raise ValueError(f"gemm_e4m3: scales must be contiguous uint8 ({-(-k // 512)}, {n}, 4): {tuple(w_scales.shape)}")
+    if out is None:
+        out = torch.empty((m, n), dtype=a.dtype, device=a.device)
+    _, ldc = _rows(out)
+    if out.shape != (m, n) or out.dtype != a.dtype:
+        raise ValueError("gemm_e4m3: out shape/dtype")
+    ldr = 0
+    if residual is not None:
+        require_device(residual)
+        _, ldr = _rows(residual)
+        if residual.shape != out.shape or residual.dtype != a.dtype:
+            raise ValueError("gemm_e4m3: residual shape/dtype")
+    if m == 0 or n == 0:
+        return out
+    lib = _lib.load()
+    ws = _persistent_ws("gemm_e4m3", lib.fs_gemm_e4m3_workspace_size(m, n, k), a.device)
+    check(lib.fs_gemm_e4m3(ptr(a), lda, ptr(w), ldb, ptr(w_scales), ptr(out), ldc, ptr(residual), ldr, m, n, k, _dt(a), ptr(ws),
+                           ws.numel(), stream_ptr()), "gemm_e4m3")
+    return out
+
+
 def gemm_add_rmsnorm(a: torch.Tensor, w: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor,
                      eps: float, x_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """x = a @ w.T + residual (nn.Linear then the residual add, model.py:105-106) and y = RMSNorm(x)

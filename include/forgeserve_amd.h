@@ -275,6 +275,25 @@ int fs_gemm_swiglu(const void* A, int64_t lda, const void* B, int64_t ldb, void*
 int fs_embedding(const int64_t* ids, int64_t M, const void* weight, int64_t d_model, int64_t vocab,
                  void* out, int64_t ldo, int32_t dtype, void* stream);
 
+/* Rows of X as e4m3 codes with a power of two for each 128 columns as their scale, kept as its biased exponent byte
+ * (fs_kv_layout's format and limits, f32's and bf16's for every dtype): code [r][k] at codes + r*ldc + k, the byte of
+ * row r's columns 128g .. at scales + (g/4)*4*rows + 4*r + g%4; bytes past the last group are zeros. K % 128 == 0, code
+ * rows 16-byte aligned, scales 4-byte aligned. No counterpart in the reference: the weights of fs_gemm_e4m3 are laid
+ * out so once. */
+int fs_quantize_e4m3(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, int64_t ldc,
+                     void* scales, void* stream);
+
+/* C[M,N] = X[M,K] . W[N,K]^T (+ R[M,N]) (nn.Linear: model.py:57-60, 88-90, with the residual add of model.py:105-106)
+ * with W as fs_quantize_e4m3 leaves it (ldw bytes from row to row, a multiple of 16) and X encoded in the same way
+ * within the call, f32 accumulation, and one rounding of product and residual to the dtype (bf16 or f16). Rows of X, C
+ * and R may be strided and of any alignment; columns are contiguous. K % 128 == 0. The order of a sum over K goes by M
+ * (as do the tiles), so a row's last bit may differ between a short and a long batch. workspace: at least
+ * fs_gemm_e4m3_workspace_size bytes for this M, 256-byte aligned. */
+int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* w_scales, void* C, int64_t ldc,
+                 const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K, int32_t dtype, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+int64_t fs_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
+
 /* One decoder block of fs_run_blocks: its weights (contiguous rows, the dtype of the run; w_qkv holds wq, wk and
  * wv one below the other, w_gate_up the gate then the up projection), the norm after the attention, the
  * norm that the block's output goes through next (NULL: none; the last block only), its cache layer with

@@ -138,3 +138,47 @@ def test_rows_of_another_dtype_are_refused(monkeypatch):
         ops.paged_attention(x.view(1, 1, 8, 64), lay, i, i[:, :1], 1.0)
     with pytest.raises(ValueError, match="another dtype"):
         ops.paged_attention_varlen(x.view(1, 8, 64), lay, i, i[:, :1], i[0, :2], 1.0)
+
+
+def test_projection_refusals():
+    """The C calls check their arguments before anything is launched."""
+    if not os.path.exists(LIB):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    need = lib.fs_gemm_e4m3_workspace_size(100, 64, 256)
+    assert need >= 100 * 256 + 100 * 4 and lib.fs_gemm_e4m3_workspace_size(1, 64, 200) == 0
+
+    def gemm(x=256, ldx=256, w=256, ldw=256, ws=256, c=256, ldc=64, r=None, ldr=0, m=0, n=64, k=256, dt=_lib.BF16, work=256,
+             size=1 << 40):
+        return lib.fs_gemm_e4m3(x, ldx, w, ldw, ws, c, ldc, r, ldr, m, n, k, dt, work, size, None)
+
+    assert gemm() == 0   # (no rows)
+    for bad in [dict(x=None), dict(w=None), dict(ws=None), dict(c=None), dict(dt=_lib.F32), dict(dt=7), dict(k=200), dict(k=0),
+                dict(m=-1), dict(n=0), dict(ldx=255), dict(ldw=255), dict(ldw=264), dict(ldc=63), dict(r=256, ldr=63),
+                dict(w=264), dict(ws=258), dict(m=100, work=None), dict(m=100, size=need - 1), dict(m=100, work=128),
+                dict(m=1 << 29), dict(n=1 << 29, ldc=1 << 30), dict(k=1 << 23, ldx=1 << 23, ldw=1 << 23), dict(ldw=1 << 23)]:
+        assert gemm(**bad) == -1, bad
+
+    def quantize(x=256, ldx=256, rows=0, k=256, dt=_lib.BF16, codes=256, ldc=256, scales=256):
+        return lib.fs_quantize_e4m3(x, ldx, rows, k, dt, codes, ldc, scales, None)
+
+    assert quantize() == 0
+    for bad in [dict(x=None), dict(codes=None), dict(scales=None), dict(dt=5), dict(k=100), dict(k=0), dict(rows=-1), dict(ldx=255),
+                dict(ldc=255), dict(ldc=264), dict(codes=264), dict(scales=257), dict(rows=1 << 31)]:
+        assert quantize(**bad) == -1, bad
+
+
+def test_projection_wrappers_refuse(monkeypatch):
+    monkeypatch.setattr(ops, "require_device", lambda *t: None)
+    x, w, s = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(8, 256, dtype=torch.uint8), torch.zeros(1, 8, 4, dtype=torch.uint8)
+    for bad in [(x.float(), w, s), (x[:, :128], w, s), (x, w.int(), s), (x, w, s.int()), (x, w, s[:, :7]),
+                (x, w, torch.zeros(2, 8, 4, dtype=torch.uint8)), (x, w, torch.zeros(1, 8, 8, dtype=torch.uint8)[..., ::2]),
+                (x.t(), w, s)]:
+        with pytest.raises(ValueError):
+            ops.gemm_e4m3(*bad)
+    with pytest.raises(ValueError, match="out"):
+        ops.gemm_e4m3(x, w, s, out=torch.zeros(2, 9, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="residual"):
+        ops.gemm_e4m3(x, w, s, residual=torch.zeros(2, 8))
+    with pytest.raises(ValueError, match="128"):
+        ops.quantize_e4m3(torch.zeros(3, 200))

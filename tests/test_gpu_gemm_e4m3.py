@@ -1,0 +1,183 @@
+"""Projections in 8-bit floating point against their definition in 64 bits."""
+
+import pytest
+import torch
+
+import e4m3_reference as ref
+from forgeserve_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+ALL = (10, 246)   # a matrix's scales have the same limits whatever its dtype
+
+
+def values(codes, scales, k):
+    """A matrix's values in 64 bits from its codes (rows, K) and packed scales."""
+    e = scales.cpu().transpose(0, 1).flatten(1)[:, : k // 128]
+    return ref.decode(codes.view(torch.uint8).cpu().unflatten(1, (k // 128, 128)), e).flatten(1)
+
+
+def encoded(x):
+    """x's values as the definition encodes them, in 64 bits."""
+    c, e = ref.encode(x.double().unflatten(1, (-1, 128)), ALL)
+    return ref.decode(c, e).flatten(1)
+
+
+def check(got, x, w, residual=None):
+    """got against x w^T (+ residual), x and w in 64 bits. The result is rounded once, half a step. Below that lie the
+    matrix instruction's own sums: it aligns 128 products before it adds them; 2^-14 of the products' absolute sum is
+    twenty times what it was measured to be off (2.5e-5 of a random result's norm, some 3e-6 of that sum)."""
+    want, mag = x @ w.T, x.abs() @ w.abs().T
+    if residual is not None:
+        want = want + residual.double()
+    tol = torch.finfo(got.dtype).eps / 2 * want.abs() + 2.0 ** -14 * mag + (2.0 ** -25 if got.dtype == F16 else 0)
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,k", [(1, 128), (5, 384), (33, 512), (3, 640), (130, 2048)])
+def test_quantize(dtype, rows, k):
+    g = torch.Generator().manual_seed(rows + k)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(3 * torch.randn(rows, k, generator=g))).to(dtype)
+    x[0, :128] = 0
+    x[-1, 5], x[-1, 6], x[-1, 127] = float("inf"), float("nan"), 448.0
+    c, e = ref.encode(x.double().unflatten(1, (-1, 128)), ALL)
+    want = ref.decode(c, e).flatten(1)
+    wide = torch.zeros(rows, k + 5, dtype=dtype, device=DEV)
+    wide[:, 3: 3 + k] = x.to(DEV)
+    for y in (x.to(DEV), wide[:, 3: 3 + k]):   # aligned rows and others
+        codes, scales = ops.quantize_e4m3(y)
+        assert codes.dtype == torch.float8_e4m3fn and codes.shape == (rows, k) and scales.shape == (-(-k // 512), rows, 4)
+        assert torch.equal(scales.cpu(), ref.packed_scales(e))
+        got = values(codes, scales, k)
+        assert torch.equal(got.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_quantize_every_value(dtype):
+    """Every 16-bit pattern under scales from its own magnitude up: the one conversion is the definition's rounding."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.zeros(65536, 128, dtype=dtype)
+    top = torch.finfo(dtype).max
+    x[:, 0] = bits
+    for i, f in enumerate((1.0, 1.7, 33.0, 1000.0, 3e4)):
+        x[:, 1] = (bits.double().abs() * f).clamp(max=top).nan_to_num(1.0).to(dtype)
+        codes, scales = ops.quantize_e4m3(x.to(DEV))
+        c, e = ref.encode(x.double(), ALL)
+        assert torch.equal(scales[0, :, 0].cpu(), e)
+        got, want = values(codes, scales, 128)[:, :2], ref.decode(c, e)[:, :2]
+        assert torch.equal(got.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0))
+
+
+SIZES = [(1, 16, 128), (1, 7, 384), (3, 130, 640), (8, 6144, 4096), (16, 70, 2048), (16, 9001, 512), (2, 8193, 1024),
+         (17, 64, 128), (64, 130, 512), (33, 7, 1536), (64, 2048, 2048), (65, 64, 256), (130, 300, 640), (300, 128, 4096),
+         (448, 520, 3584), (257, 4100, 1024), (1000, 260, 384), (520, 1, 512), (700, 1537, 896)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gemm(dtype, m, n, k):
+    g = torch.Generator().manual_seed(m + n + k)
+    x = (torch.randn(m, k, generator=g) * torch.exp(0.7 * torch.randn(k, generator=g))).to(dtype)
+    w = torch.randn(n, k, generator=g).mul_(0.02).to(BF16)
+    codes, scales = ops.quantize_e4m3(w.to(DEV))
+    xv, wv = encoded(x), values(codes, scales, k)
+    check(ops.gemm_e4m3(x.to(DEV), codes, scales), xv, wv)
+    # rows, results and residuals with strides and alignments of their own; the space between is left alone
+    for shift in (0, 3):
+        xs = torch.zeros(m, k + 8, dtype=dtype, device=DEV)[:, shift: shift + k].copy_(x)
+        back = torch.full((m, n + 12), 3.0, dtype=dtype, device=DEV)
+        r = torch.randn(m, n, generator=g).to(dtype)
+        rs = torch.zeros(m, n + 5, dtype=dtype, device=DEV)[:, shift: shift + n].copy_(r)
+        out = ops.gemm_e4m3(xs, codes, scales, out=back[:, 4 + shift: 4 + shift + n], residual=rs)
+        check(out, xv, wv, r)
+        assert (back[:, : 4 + shift] == 3).all() and (back[:, 4 + shift + n:] == 3).all()
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 200])
+def test_codes_with_wide_rows(m):
+    g = torch.Generator().manual_seed(m)
+    k, n = 256, 200
+    x = torch.randn(m, k, generator=g).bfloat16()
+    codes, scales = ops.quantize_e4m3(torch.randn(n, k, generator=g).to(DEV))
+    wide = torch.zeros(n, k + 48, dtype=torch.uint8, device=DEV)
+    wide[:, 16: 16 + k] = codes.view(torch.uint8)
+    check(ops.gemm_e4m3(x.to(DEV), wide[:, 16: 16 + k], scales), encoded(x), values(codes, scales, k))
+
+
+@pytest.mark.parametrize("m", [4, 40, 300])
+def test_what_is_not_finite_stays_in_its_row(m):
+    g = torch.Generator().manual_seed(m)
+    k, n = 1024, 96
+    x, w = torch.randn(m, k, generator=g).bfloat16(), torch.randn(n, k, generator=g).to(DEV)
+    codes, scales = ops.quantize_e4m3(w)
+    clean = ops.gemm_e4m3(x.to(DEV), codes, scales)
+    x[1, 700], x[2, 3] = float("nan"), float("-inf")
+    got = ops.gemm_e4m3(x.to(DEV), codes, scales)
+    assert got[1].isnan().all() and got[2].isnan().all()
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert torch.equal(got[keep], clean[keep])
+    bad = codes.view(torch.uint8).clone()
+    bad[5, 300] = 0x7f
+    got = ops.gemm_e4m3(x.to(DEV)[keep].contiguous(), bad, scales)
+    assert got[:, 5].isnan().all() and not got[:, :5].isnan().any() and not got[:, 6:].isnan().any()
+
+
+@pytest.mark.parametrize("m", [3, 64, 200])
+def test_extreme_magnitudes(m):
+    """Rows of the largest and of the smallest bf16 values, and zeros."""
+    g = torch.Generator().manual_seed(m)
+    k, n = 256, 64
+    x = torch.randn(m, k, generator=g)
+    x[0] = 0
+    x[1] *= 1e30
+    x[2] *= 1e-30
+    x = x.bfloat16()
+    codes, scales = ops.quantize_e4m3(torch.randn(n, k, generator=g).to(DEV))
+    check(ops.gemm_e4m3(x.to(DEV), codes, scales), encoded(x), values(codes, scales, k))
+
+
+def test_no_rows():
+    codes, scales = ops.quantize_e4m3(torch.randn(32, 128, device=DEV))
+    assert ops.gemm_e4m3(torch.empty(0, 128, dtype=BF16, device=DEV), codes, scales).shape == (0, 32)
+    assert ops.quantize_e4m3(torch.empty(0, 128, dtype=BF16, device=DEV))[0].shape == (0, 128)
+
+
+@pytest.mark.parametrize("m", [5, 50, 300])
+def test_captured(m):
+    """Replays with new rows between eager calls; two captured calls share the workspace one after the other."""
+    g = torch.Generator().manual_seed(m)
+    k, n = 1024, 512
+    codes, scales = ops.quantize_e4m3(torch.randn(n, k, generator=g).to(DEV))
+    back, bscales = ops.quantize_e4m3(torch.randn(k, n, generator=g).to(DEV))
+    x = torch.randn(m, k, generator=g).bfloat16().to(DEV)
+    step = lambda: ops.gemm_e4m3(ops.gemm_e4m3(x, codes, scales), back, bscales, residual=x)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        x.copy_(torch.randn(m, k, generator=g))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_an_mlp_of_8_bit_projections():
+    """gate | up, the SwiGLU and down with its residual, as a decoder block runs them, against the same chain in 64 bits
+    from each step's own inputs."""
+    g = torch.Generator().manual_seed(21)
+    d, f = 512, 1024
+    wgu, wd = torch.randn(2 * f, d, generator=g).mul_(0.05).to(DEV), torch.randn(d, f, generator=g).mul_(0.05).to(DEV)
+    (cgu, sgu), (cd, sd) = ops.quantize_e4m3(wgu), ops.quantize_e4m3(wd)
+    for m in (1, 20, 90):
+        x = torch.randn(m, d, generator=g).bfloat16().to(DEV)
+        gu = ops.gemm_e4m3(x, cgu, sgu)
+        check(gu, encoded(x.cpu()), values(cgu, sgu, d))
+        h = ops.silu_mul(gu)
+        y = ops.gemm_e4m3(h, cd, sd, residual=x)
+        check(y, encoded(h.cpu()), values(cd, sd, f), x.cpu())
