@@ -20,23 +20,30 @@ namespace {
 
 typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((__vector_size__(2 * sizeof(short)))) short s16x2_t;
 typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2_t;
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
 
 constexpr int GROUP = 128;        // K per scale, and per matrix instruction
 constexpr int SHORT_ROWS = 16;    // rows that one launch takes
+template <int I> struct Int { static constexpr int value = I; };
 
 // D = A . B^T of 16 x 128 codes each: a lane holds 32 of its row's (two 16-byte chunks: any two, the same for A and B).
 // BYTE: which of the four groups in the scale words.
 template <int BYTE>
-FS_DEVICE float4_t mfma_codes(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, float4_t c, uint32_t sa, uint32_t sb) {
-  struct Two { u32x4 x, y; };
-  const Two a = {a0, a1}, b = {b0, b1};
+FS_DEVICE float4_t mfma_codes(i32x8 a, i32x8 b, float4_t c, uint32_t sa, uint32_t sb) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(float4_t, __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                                          __builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b),
-                                          __builtin_bit_cast(f32x4, c), 0, 0, BYTE, (int)sa, BYTE, (int)sb));
+  return __builtin_bit_cast(float4_t, __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, __builtin_bit_cast(f32x4, c), 0, 0,
+                                                                                       BYTE, (int)sa, BYTE, (int)sb));
+}
+// The same of 32 x 64 codes each: a lane holds 32 of row lane % 32.
+template <int BYTE>
+FS_DEVICE f32x16 mfma_codes32(i32x8 a, i32x8 b, f32x16 c, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, BYTE, (int)sa, BYTE, (int)sb);
+}
+FS_DEVICE i32x8 both_chunks(u32x4 a, u32x4 b) {
+  return __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -263,7 +270,8 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
       load_x(kt + d + 1, xn);
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        acc[j] = mfma_codes<0>(ring[d].c[j][0], ring[d].c[j][1], xc[0], xc[1], acc[j], ring[d].s[j], (uint32_t)e);
+        acc[j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), both_chunks(xc[0], xc[1]), acc[j], ring[d].s[j],
+                               (uint32_t)e);
       load(kt + d + DEPTH, ring[d]);
     }
   }
@@ -315,6 +323,11 @@ FS_DEVICE bool tile_of(int tiles_m, int ntiles, int bm, int bn, int64_t& m0, int
   return true;
 }
 
+// A stage's rows in LDS are 128 bytes, eight 16-byte chunks, chunk c at place c ^ swap_of(row): an operand read's 16
+// lanes take one chunk of 16 consecutive rows, which must differ in their place within 256 bytes, two rows' worth.
+// (Swapped by row & 7, as 128-byte banks would have it, half of the LDS port's time went to conflicts.)
+FS_DEVICE int swap_of(int row) { return (row >> 1) & 7; }
+
 struct Operands {
   const uint8_t *x, *w;          // codes
   const uint8_t *xs, *ws;        // scale words
@@ -324,9 +337,8 @@ struct Operands {
   int tiles_m, ntiles;
 };
 
-// BM x BN tiles, WGM x WGN waves, NS stages of 128 in LDS, NS - 1 of them on their way. A stage's rows are 128 bytes,
-// their 16-byte chunks swapped by (row & 7), so that the operand reads meet no bank twice. The words of the rows' scales
-// come with every fourth stage (one copy per 64 rows), into one of two places.
+// BM x BN tiles, WGM x WGN waves, NS stages of 128 in LDS, NS - 1 of them on their way. The words of the rows'
+// scales come with every fourth stage (one copy per 64 rows), into one of two places.
 template <int DT, int BM, int BN, int WGM, int WGN, int NS>
 __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands P, uint16_t* __restrict__ C, int64_t ldc,
                                                                         const uint16_t* __restrict__ R, int64_t ldr,
@@ -352,7 +364,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
   uint32_t off[CPW];
 #pragma unroll
   for (int i = 0; i < CPW; ++i) {
-    const int q = i * NW + wave, row = 8 * q + cr, c = (lane & 7) ^ (row & 7);
+    const int q = i * NW + wave, row = 8 * q + cr, c = (lane & 7) ^ swap_of(row);
     const bool in_x = 8 * q < BM;
     const int64_t lead = in_x ? m0 : n0, last = (in_x ? P.M : P.N) - 1, ld = in_x ? P.ldx : P.ldw;
     const int64_t r = min(lead + (in_x ? row : row - BM), last) - lead;
@@ -406,25 +418,20 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
       for (int j = 0; j < TN; ++j) ws[j] = p[BM + wn * (BN / WGN) + 16 * j + l16];
     }
     const char* st = smem + (kt % NS) * STAGE;
-    u32x4 xf[TM][2], wf[TN][2];
+    auto fragment = [&](const char* rows, int r) {
+      return both_chunks(*reinterpret_cast<const u32x4*>(rows + r * GROUP + 16 * (g ^ swap_of(r))),
+                         *reinterpret_cast<const u32x4*>(rows + r * GROUP + 16 * ((4 + g) ^ swap_of(r))));
+    };
+    i32x8 xf[TM], wf[TN];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int i = 0; i < TM; ++i) xf[i] = fragment(st, wm * (BM / WGM) + 16 * i + l16);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int r = wm * (BM / WGM) + 16 * i + l16;
-        xf[i][h] = *reinterpret_cast<const u32x4*>(st + r * GROUP + 16 * ((4 * h + g) ^ (r & 7)));
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int r = wn * (BN / WGN) + 16 * j + l16;
-        wf[j][h] = *reinterpret_cast<const u32x4*>(st + XB + r * GROUP + 16 * ((4 * h + g) ^ (r & 7)));
-      }
-    }
+    for (int j = 0; j < TN; ++j) wf[j] = fragment(st + XB, wn * (BN / WGN) + 16 * j + l16);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        acc[i][j] = mfma_codes<0>(wf[j][0], wf[j][1], xf[i][0], xf[i][1], acc[i][j], ws[j], xs[i]);
+        acc[i][j] = mfma_codes<0>(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
 #pragma unroll
     for (int i = 0; i < TM; ++i) xs[i] >>= 8;   // the next group's byte
 #pragma unroll
@@ -443,6 +450,272 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
       } else {
         store_row4<DT>(acc[i][j], row, col0, C, ldc, R, ldr, P.N, vec);
       }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// long batches: 256 x 256 tiles, 8 waves of 128 x 64 in two alternating groups
+// ------------------------------------------------------------------------------------------------
+// Bound by the matrix cores with the LDS port close behind: a stage of 128 is 32 instructions of 32 cycles a wave, 2048
+// cycles a SIMD, against 192 KB of operand reads (1536 cycles) and 64 KB of copies (512), the same bytes and cycles as a
+// 16-bit product's stage of 64, for twice the depth. So the loop is that product's (gemm.hip, gemm_bf16_long_kernel): four
+// phases a stage, one 64 x 32 quadrant of the wave's tile each, ordered so that each needs one new operand; the reads and
+// copies of a phase in its first half, the products in its second; waves 4..7 half a phase behind waves 0..3, so that
+// on each SIMD one wave multiplies while the other reads and copies; copies issued five phases before they are read,
+// eight per wave on their way.
+// The scale words of four stages (2 KB) are one more copy per wave, issued four stages before they are read and counted
+// in that stage's waits; a lane keeps its 12 words in registers and each stage's instructions pick their byte.
+template <int DT, bool PARTIAL>
+__global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint16_t* __restrict__ C, int64_t ldc,
+                                                                const uint16_t* __restrict__ R, int64_t ldr, bool vec,
+                                                                float* __restrict__ part) {
+  constexpr int BUF = 256 * GROUP;      // one operand's stage
+  constexpr int PITCH = 64 * 2 + 16;    // a row of a wave's rounded results
+  constexpr int SMEM = 8 * 128 * PITCH;
+  static_assert(SMEM >= 4 * BUF, "the ring fits: X stages 0, 1, then W stages 0, 1");
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM];
+  __shared__ __attribute__((aligned(256))) uint32_t words[2][512];   // X rows', then W rows'
+  int64_t m0, n0;
+  if (!tile_of(P.tiles_m, P.ntiles, 256, 256, m0, n0)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem, words0 = (uint32_t)(uintptr_t)words;
+
+  // Copies: 8 rows of 128 bytes each; lane l takes row l >> 3, physical chunk l & 7 of it, which holds logical chunk
+  // (l & 7) ^ swap_of(row). Quarter q of X: rows 64 q + 8 wave (+ 128); of W: rows 64 (wave >> 2) + 32 q + 8 (wave & 3) (+ 128).
+  const int cr = lane >> 3, cc = (lane & 7) ^ swap_of(8 * (wave & 1) + cr);   // (the quarters' rows add multiples of 16)
+  uint32_t xo[2][2], wo[2][2];
+  const int xrow = 8 * wave, wrow = 64 * (wave >> 2) + 8 * (wave & 3);
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      xo[q][h] = (uint32_t)((min(m0 + xrow + 64 * q + 128 * h + cr, P.M - 1) - m0) * P.ldx + 16 * cc);
+      wo[q][h] = (uint32_t)((min(n0 + wrow + 32 * q + 128 * h + cr, P.N - 1) - n0) * P.ldw + 16 * cc);
+    }
+  const int split = blockIdx.y, nk = P.nk / (int)gridDim.y, first = split * nk;   // (nk % 4 == 0 where K is split)
+  const char* xb = reinterpret_cast<const char*>(P.x + m0 * P.ldx + (int64_t)first * GROUP);
+  const char* wb = reinterpret_cast<const char*>(P.w + n0 * P.ldw + (int64_t)first * GROUP);
+  auto copy_x = [&](int q, int kt, int buf) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      dma16_at(xb + (int64_t)kt * GROUP, xo[q][h], lds0 + (uint32_t)(buf * BUF + (xrow + 64 * q + 128 * h) * GROUP));
+  };
+  auto copy_w = [&](int q, int kt, int buf) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      dma16_at(wb + (int64_t)kt * GROUP, wo[q][h], lds0 + (uint32_t)((2 + buf) * BUF + (wrow + 32 * q + 128 * h) * GROUP));
+  };
+  // 64 rows' words of the four stages from kt (a multiple of 4) on: waves 0..3 X's, 4..7 W's
+  const int64_t srows = wm ? P.N : P.M;
+  const uint32_t so = (uint32_t)(4 * min((wm ? n0 : m0) + 64 * (wave & 3) + lane, srows - 1));
+  const char* sb = reinterpret_cast<const char*>(wm ? P.ws : P.xs) + (int64_t)(first >> 2) * 4 * srows;
+  auto copy_s = [&](int kt) {
+    dma4_at(sb + (int64_t)(kt >> 2) * 4 * srows, so, words0 + (uint32_t)(4 * ((kt >> 2 & 1) * 512 + 64 * wave)));
+  };
+
+  // Operands: lane l holds row l % 32 of a tile of 32 and, of k-step ks, chunks 4 ks + 2 (l / 32) and the next.
+  typedef __attribute__((address_space(3))) const u32x4 LdsFrag;
+  const int l32 = lane & 31, half = lane >> 5;
+  uint32_t xl[4], wl[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t at = 16 * ((4 * (c >> 1) + 2 * half + (c & 1)) ^ swap_of(l32));
+    xl[c] = lds0 + (uint32_t)((wm * 128 + l32) * GROUP) + at;
+    wl[c] = lds0 + 2 * BUF + (uint32_t)((wn * 64 + l32) * GROUP) + at;
+  }
+
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+  i32x8 xf[2][2], w0[2], w1[2];   // [tile][k-step], [k-step]
+  uint32_t xs[4], ws[2];
+
+  auto read_x = [&](int q, int buf) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint32_t at = (uint32_t)(buf * BUF + q * 64 * GROUP + i * 32 * GROUP);
+        xf[i][ks] = both_chunks(*(LdsFrag*)(uintptr_t)(xl[2 * ks] + at), *(LdsFrag*)(uintptr_t)(xl[2 * ks + 1] + at));
+      }
+  };
+  auto read_w = [&](i32x8 (&wf)[2], int q, int buf) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const uint32_t at = (uint32_t)(buf * BUF + q * 32 * GROUP);
+      wf[ks] = both_chunks(*(LdsFrag*)(uintptr_t)(wl[2 * ks] + at), *(LdsFrag*)(uintptr_t)(wl[2 * ks + 1] + at));
+    }
+  };
+  auto read_s = [&](int kt) {
+    const uint32_t* p = words[kt >> 2 & 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xs[i] = p[wm * 128 + 32 * i + l32];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) ws[j] = p[256 + wn * 64 + 32 * j + l32];
+  };
+  auto barrier = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // one phase's second half: 4 products, each as its operands arrive
+  auto mul = [&](auto byte, int qm, int qn, const i32x8 (&wf)[2]) {
+    barrier();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        acc[2 * qm + i][qn] = mfma_codes32<decltype(byte)::value>(wf[ks], xf[i][ks], acc[2 * qm + i][qn], ws[qn], xs[2 * qm + i]);
+    __builtin_amdgcn_s_setprio(0);
+    barrier();
+  };
+  // stage kt, whose groups are byte kt % 4 of the words; buf = kt & 1: it starts with W's quarter buf, and ends reading
+  // the next one's. inner: two more stages follow it, and four behind its group's first (no branches: the compiler moves
+  // these products past them, barriers or not, to the stage's end)
+  auto stage = [&](int kt, auto byte, auto inner) {
+    constexpr int buf = decltype(byte)::value & 1;
+    constexpr bool IN = decltype(inner)::value != 0;
+    i32x8 (&wfirst)[2] = buf ? w1 : w0;
+    i32x8 (&wsecond)[2] = buf ? w0 : w1;
+    const bool next = IN || kt + 1 < nk, next2 = IN || kt + 2 < nk;
+    const bool scales = decltype(byte)::value == 0 && (IN || kt + 4 < nk);   // this stage's waits count one copy more
+    auto wait = [&]() {
+      if (scales) wait_vm<9>();
+      else wait_vm<8>();
+    };
+    if (decltype(byte)::value == 0) read_s(kt);
+    read_x(0, buf);
+    if (scales) copy_s(kt + 4);
+    if (next) {
+      copy_w(buf, kt + 1, buf ^ 1);   // the next stage's second quarter is this stage's first
+      wait();
+    } else {
+      wait_vm<2>();
+    }
+    mul(byte, 0, buf, wfirst);
+    read_w(wsecond, buf ^ 1, buf);
+    if (next) {
+      copy_x(1, kt + 1, buf ^ 1);
+      wait();
+    } else {
+      wait_vm<0>();
+    }
+    mul(byte, 0, buf ^ 1, wsecond);
+    read_x(1, buf);
+    if (next2) {
+      copy_w(buf, kt + 2, buf);
+      wait();
+    } else if (next) {
+      wait_vm<6>();
+    }
+    mul(byte, 1, buf ^ 1, wsecond);
+    if (next) read_w(wsecond, buf ^ 1, buf ^ 1);
+    if (next2) {
+      copy_x(0, kt + 2, buf);
+      wait();
+    } else if (next) {
+      wait_vm<4>();
+    }
+    mul(byte, 1, buf, wfirst);
+  };
+
+  copy_s(0);
+  copy_w(0, 0, 0);
+  copy_x(0, 0, 0);
+  copy_w(1, 0, 0);
+  copy_x(1, 0, 0);
+  if (nk > 1) {
+    copy_w(1, 1, 1);
+    copy_x(0, 1, 1);
+    wait_vm<8>();
+  } else {
+    wait_vm<4>();
+  }
+  barrier();
+  if (wm) barrier();   // the second group runs one barrier behind
+  read_w(w0, 0, 0);
+  int kt = 0;
+  for (; kt + 5 < nk; kt += 4) {
+    stage(kt, Int<0>{}, Int<1>{});
+    stage(kt + 1, Int<1>{}, Int<1>{});
+    stage(kt + 2, Int<2>{}, Int<1>{});
+    stage(kt + 3, Int<3>{}, Int<1>{});
+  }
+  for (; kt < nk; kt += 4) {
+    stage(kt, Int<0>{}, Int<0>{});
+    if (kt + 1 < nk) stage(kt + 1, Int<1>{}, Int<0>{});
+    if (kt + 2 < nk) stage(kt + 2, Int<2>{}, Int<0>{});
+    if (kt + 3 < nk) stage(kt + 3, Int<3>{}, Int<0>{});
+  }
+  if (!wm) barrier();
+
+  // acc[i][j][4 t + r]: the lane holds C[32 i + l32][32 j + 8 t + 4 half + r]
+  auto four = [&](int i, int j, int t) { return float4_t{acc[i][j][4 * t], acc[i][j][4 * t + 1], acc[i][j][4 * t + 2], acc[i][j][4 * t + 3]}; };
+  if (PARTIAL) {   // (N % 4 == 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = m0 + wm * 128 + 32 * i + l32;
+      float* prow = part + ((int64_t)split * P.M + row) * P.N;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int64_t col0 = n0 + wn * 64 + 32 * j + 8 * t + 4 * half;
+          if (row < P.M && col0 < P.N) *reinterpret_cast<float4_t*>(prow + col0) = four(i, j, t);
+        }
+    }
+    return;
+  }
+  // The wave's rounded results (the residual added before) to LDS, then out by whole rows, 16 bytes a lane. Every copy
+  // has landed and, past this barrier, every wave has read its last operands: the ring's space is free.
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  char* out = smem + wave * 128 * PITCH;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = m0 + wm * 128 + 32 * i + l32;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float4_t a = four(i, j, t);
+        const int64_t col0 = n0 + wn * 64 + 32 * j + 8 * t + 4 * half;
+        if (R && row < P.M) {
+          if (vec && col0 + 4 <= P.N) {
+            const u32x2_t r = *reinterpret_cast<const u32x2_t*>(R + row * ldr + col0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] += half_of<DT>(r[e >> 1], e & 1);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col0 + e < P.N) a[e] += Elem<DT>::to_f32(R[row * ldr + col0 + e]);
+          }
+        }
+        *reinterpret_cast<u32x2_t*>(out + (32 * i + l32) * PITCH + 2 * (32 * j + 8 * t + 4 * half)) =
+            u32x2_t{(uint32_t)Elem<DT>::store_bits(a[0]) | ((uint32_t)Elem<DT>::store_bits(a[1]) << 16),
+                    (uint32_t)Elem<DT>::store_bits(a[2]) | ((uint32_t)Elem<DT>::store_bits(a[3]) << 16)};
+      }
+  }
+  const int64_t col = n0 + wn * 64 + 8 * (lane & 7);
+  const bool wide = col + 8 <= P.N && (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
+#pragma unroll 4
+  for (int it = 0; it < 16; ++it) {
+    const int lr = it * 8 + (lane >> 3);
+    const int64_t row = m0 + wm * 128 + lr;
+    const u32x4 o = *reinterpret_cast<const u32x4*>(out + lr * PITCH + 16 * (lane & 7));
+    if (row >= P.M) continue;
+    if (wide) {
+      *reinterpret_cast<u32x4*>(C + row * ldc + col) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < P.N) C[row * ldc + col + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
     }
   }
 }
@@ -469,7 +742,7 @@ struct Plan {
 };
 // The tile and the K splits of a shape.
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
-  const int bm = M <= 64 ? 64 : 128, bn = M <= 64 ? 64 : 128;
+  const int bm = M <= 64 ? 64 : M > 1024 ? 256 : 128, bn = bm;
   const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn), nk = K / GROUP;
   int s = 1;
   while (s < 8 && N % 4 == 0 && tiles * s * 2 <= 512 && nk % (8 * s) == 0 && nk / (2 * s) >= 4) s *= 2;
@@ -524,6 +797,10 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
   float* out = p.splits > 1 ? part : nullptr;
   if (p.bm == 64)
     gemm_e4m3_tile_kernel<DT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, C, ldc, R, ldr, vec, out);
+  else if (p.bm == 256 && out)
+    gemm_e4m3_long_kernel<DT, true><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
+  else if (p.bm == 256)
+    gemm_e4m3_long_kernel<DT, false><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, nullptr);
   else
     gemm_e4m3_tile_kernel<DT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
   if (p.splits > 1) {
