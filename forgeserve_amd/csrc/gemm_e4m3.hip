@@ -484,29 +484,27 @@ __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem, words0 = (uint32_t)(uintptr_t)words;
 
   // Copies: 8 rows of 128 bytes each; lane l takes row l >> 3, physical chunk l & 7 of it, which holds logical chunk
-  // (l & 7) ^ swap_of(row). Quarter q of X: rows 64 q + 8 wave (+ 128); of W: rows 64 (wave >> 2) + 32 q + 8 (wave & 3) (+ 128).
-  const int cr = lane >> 3, cc = (lane & 7) ^ swap_of(8 * (wave & 1) + cr);   // (the quarters' rows add multiples of 16)
-  uint32_t xo[2][2], wo[2][2];
-  const int xrow = 8 * wave, wrow = 64 * (wave >> 2) + 8 * (wave & 3);
+  // (l & 7) ^ swap_of(row). A wave's rows of either operand are 64 i + 8 wave ..; half q of X has i = q and q + 2.
+  const int cr = lane >> 3, cc = (lane & 7) ^ swap_of(8 * (wave & 1) + cr);
+  uint32_t xo[4], wo[4];
+  const int crow = 8 * wave;
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      xo[q][h] = (uint32_t)((min(m0 + xrow + 64 * q + 128 * h + cr, P.M - 1) - m0) * P.ldx + 16 * cc);
-      wo[q][h] = (uint32_t)((min(n0 + wrow + 32 * q + 128 * h + cr, P.N - 1) - n0) * P.ldw + 16 * cc);
-    }
+  for (int i = 0; i < 4; ++i) {
+    xo[i] = (uint32_t)((min(m0 + 64 * i + crow + cr, P.M - 1) - m0) * P.ldx + 16 * cc);
+    wo[i] = (uint32_t)((min(n0 + 64 * i + crow + cr, P.N - 1) - n0) * P.ldw + 16 * cc);
+  }
   const int split = blockIdx.y, nk = P.nk / (int)gridDim.y, first = split * nk;   // (nk % 4 == 0 where K is split)
   const char* xb = reinterpret_cast<const char*>(P.x + m0 * P.ldx + (int64_t)first * GROUP);
   const char* wb = reinterpret_cast<const char*>(P.w + n0 * P.ldw + (int64_t)first * GROUP);
   auto copy_x = [&](int q, int kt, int buf) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      dma16_at(xb + (int64_t)kt * GROUP, xo[q][h], lds0 + (uint32_t)(buf * BUF + (xrow + 64 * q + 128 * h) * GROUP));
+    for (int i = q; i < 4; i += 2)
+      dma16_at(xb + (int64_t)kt * GROUP, xo[i], lds0 + (uint32_t)(buf * BUF + (64 * i + crow) * GROUP));
   };
-  auto copy_w = [&](int q, int kt, int buf) {
+  auto copy_w = [&](int kt, int buf) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      dma16_at(wb + (int64_t)kt * GROUP, wo[q][h], lds0 + (uint32_t)((2 + buf) * BUF + (wrow + 32 * q + 128 * h) * GROUP));
+    for (int i = 0; i < 4; ++i)
+      dma16_at(wb + (int64_t)kt * GROUP, wo[i], lds0 + (uint32_t)((2 + buf) * BUF + (64 * i + crow) * GROUP));
   };
   // 64 rows' words of the four stages from kt (a multiple of 4) on: waves 0..3 X's, 4..7 W's
   const int64_t srows = wm ? P.N : P.M;
@@ -532,24 +530,26 @@ __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-  i32x8 xf[2][2], w0[2], w1[2];   // [tile][k-step], [k-step]
+  i32x8 xf[2][2], wf[2][2];   // [tile][k-step]
   uint32_t xs[4], ws[2];
 
   auto read_x = [&](int q, int buf) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int i = 0; i < 2; ++i) {
         const uint32_t at = (uint32_t)(buf * BUF + q * 64 * GROUP + i * 32 * GROUP);
         xf[i][ks] = both_chunks(*(LdsFrag*)(uintptr_t)(xl[2 * ks] + at), *(LdsFrag*)(uintptr_t)(xl[2 * ks + 1] + at));
       }
   };
-  auto read_w = [&](i32x8 (&wf)[2], int q, int buf) {
+  auto read_w = [&](int buf) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const uint32_t at = (uint32_t)(buf * BUF + q * 32 * GROUP);
-      wf[ks] = both_chunks(*(LdsFrag*)(uintptr_t)(wl[2 * ks] + at), *(LdsFrag*)(uintptr_t)(wl[2 * ks + 1] + at));
-    }
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t at = (uint32_t)(buf * BUF + j * 32 * GROUP);
+        wf[j][ks] = both_chunks(*(LdsFrag*)(uintptr_t)(wl[2 * ks] + at), *(LdsFrag*)(uintptr_t)(wl[2 * ks + 1] + at));
+      }
   };
   auto read_s = [&](int kt) {
     const uint32_t* p = words[kt >> 2 & 1];
@@ -563,83 +563,64 @@ __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  // one phase's second half: 4 products, each as its operands arrive
-  auto mul = [&](auto byte, int qm, int qn, const i32x8 (&wf)[2]) {
+  // one phase's second half: 8 products, each as its operands arrive
+  auto mul = [&](auto byte, int q) {
     barrier();
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        acc[2 * qm + i][qn] = mfma_codes32<decltype(byte)::value>(wf[ks], xf[i][ks], acc[2 * qm + i][qn], ws[qn], xs[2 * qm + i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[2 * q + i][j] = mfma_codes32<decltype(byte)::value>(wf[j][ks], xf[i][ks], acc[2 * q + i][j], ws[j], xs[2 * q + i]);
     __builtin_amdgcn_s_setprio(0);
     barrier();
   };
-  // stage kt, whose groups are byte kt % 4 of the words; buf = kt & 1: it starts with W's quarter buf, and ends reading
-  // the next one's. inner: two more stages follow it, and four behind its group's first (no branches: the compiler moves
-  // these products past them, barriers or not, to the stage's end)
+  // stage kt, whose groups are byte kt % 4 of the words. inner: two more stages follow it, and four behind its group's
+  // first (no branches: the compiler moves these products past them, barriers or not, to the stage's end)
   auto stage = [&](int kt, auto byte, auto inner) {
-    constexpr int buf = decltype(byte)::value & 1;
+    constexpr int buf = decltype(byte)::value & 1;   // kt & 1
     constexpr bool IN = decltype(inner)::value != 0;
-    i32x8 (&wfirst)[2] = buf ? w1 : w0;
-    i32x8 (&wsecond)[2] = buf ? w0 : w1;
     const bool next = IN || kt + 1 < nk, next2 = IN || kt + 2 < nk;
     const bool scales = decltype(byte)::value == 0 && (IN || kt + 4 < nk);   // this stage's waits count one copy more
-    auto wait = [&]() {
-      if (scales) wait_vm<9>();
-      else wait_vm<8>();
-    };
     if (decltype(byte)::value == 0) read_s(kt);
+    read_w(buf);
     read_x(0, buf);
     if (scales) copy_s(kt + 4);
     if (next) {
-      copy_w(buf, kt + 1, buf ^ 1);   // the next stage's second quarter is this stage's first
-      wait();
-    } else {
-      wait_vm<2>();
-    }
-    mul(byte, 0, buf, wfirst);
-    read_w(wsecond, buf ^ 1, buf);
-    if (next) {
       copy_x(1, kt + 1, buf ^ 1);
-      wait();
+      if (scales) wait_vm<9>();
+      else wait_vm<8>();
     } else {
       wait_vm<0>();
     }
-    mul(byte, 0, buf ^ 1, wsecond);
+    mul(byte, 0);
     read_x(1, buf);
     if (next2) {
-      copy_w(buf, kt + 2, buf);
-      wait();
-    } else if (next) {
-      wait_vm<6>();
-    }
-    mul(byte, 1, buf ^ 1, wsecond);
-    if (next) read_w(wsecond, buf ^ 1, buf ^ 1);
-    if (next2) {
+      copy_w(kt + 2, buf);
       copy_x(0, kt + 2, buf);
-      wait();
+      if (scales) wait_vm<9>();
+      else wait_vm<8>();
     } else if (next) {
-      wait_vm<4>();
+      wait_vm<2>();
     }
-    mul(byte, 1, buf, wfirst);
+    mul(byte, 1);
   };
 
   copy_s(0);
-  copy_w(0, 0, 0);
+  copy_w(0, 0);
   copy_x(0, 0, 0);
-  copy_w(1, 0, 0);
   copy_x(1, 0, 0);
   if (nk > 1) {
-    copy_w(1, 1, 1);
+    copy_w(1, 1);
     copy_x(0, 1, 1);
     wait_vm<8>();
   } else {
-    wait_vm<4>();
+    wait_vm<2>();
   }
   barrier();
   if (wm) barrier();   // the second group runs one barrier behind
-  read_w(w0, 0, 0);
   int kt = 0;
   for (; kt + 5 < nk; kt += 4) {
     stage(kt, Int<0>{}, Int<1>{});
