@@ -27,6 +27,7 @@ typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
 
 constexpr int GROUP = 128;        // K per scale, and per matrix instruction
 constexpr int SHORT_ROWS = 16;    // rows that one launch takes
+constexpr int SHORT_BYTES = 64 * 1024;   // and their codes
 template <int I> struct Int { static constexpr int value = I; };
 
 // D = A . B^T of 16 x 128 codes each: a lane holds 32 of its row's (two 16-byte chunks: any two, the same for A and B).
@@ -45,6 +46,11 @@ FS_DEVICE f32x16 mfma_codes32(i32x8 a, i32x8 b, f32x16 c, uint32_t sa, uint32_t 
 FS_DEVICE i32x8 both_chunks(u32x4 a, u32x4 b) {
   return __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
+
+// A stage's rows in LDS are 128 bytes, eight 16-byte chunks, chunk c at place c ^ swap_of(row): an operand read's 16
+// lanes take one chunk of 16 consecutive rows, which must differ in their place within 256 bytes, two rows' worth.
+// (Swapped by row & 7, as 128-byte banks would have it, half of the LDS port's time went to conflicts.)
+FS_DEVICE int swap_of(int row) { return (row >> 1) & 7; }
 
 // ------------------------------------------------------------------------------------------------
 // encoding rows of 16-bit values
@@ -104,6 +110,30 @@ FS_DEVICE float finite_max(const uint32_t (&w)[N]) {
   return m;
 }
 
+// The largest over a lane's LANES neighbours, 8 or 16, in each of them (within a row of lanes: no trip through LDS):
+// lanes 1 and 2 apart, then mirrored within 8, then within 16.
+template <int LANES>
+FS_DEVICE uint32_t group_max(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));
+  return LANES == 8 ? m : max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, false));
+}
+// (magnitudes order as their bits do)
+template <int LANES>
+FS_DEVICE float group_max(float m) { return __uint_as_float(group_max<LANES>(__float_as_uint(m))); }
+
+// A group of 128 values, 2 NW in each of 64 / NW lanes: the exponent byte of its scale, and the lane's codes.
+template <int DT, int NW>
+FS_DEVICE void encode_group(const uint32_t (&w)[NW], int& e, uint32_t (&c)[NW / 2]) {
+  constexpr int LANES = 64 / NW;
+  const uint32_t m = group_max<LANES>(magnitude_bits(w));
+  const bool far = __any(m > LARGEST<DT>);
+  e = far ? scale_exponent<FS_F32>(group_max<LANES>(finite_max<DT>(w))) : exponent_of_bits<DT>(m);
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) c[i] = encode_words<DT>(w[2 * i], w[2 * i + 1], e, far);
+}
+
 // A wave per 512 columns of a row: 16 lanes of 8 values share a group. VEC: rows of aligned 16-byte pieces.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) quantize_e4m3_kernel(const typename Elem<DT>::T* __restrict__ X, int64_t ldx,
@@ -125,9 +155,7 @@ __global__ void __launch_bounds__(256) quantize_e4m3_kernel(const typename Elem<
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_magnitude(v[j]));
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    e = scale_exponent<FS_F32>(m);
+    e = scale_exponent<FS_F32>(group_max<16>(m));
     const float inv = scale_inverse(e);
     out = u32x2_t{encode4(v[0], v[1], v[2], v[3], inv), encode4(v[4], v[5], v[6], v[7], inv)};
   } else {
@@ -142,19 +170,9 @@ __global__ void __launch_bounds__(256) quantize_e4m3_kernel(const typename Elem<
           w[j] = (uint32_t)X[row * ldx + k + 2 * j] | ((uint32_t)X[row * ldx + k + 2 * j + 1] << 16);
       }
     }
-    uint32_t m = magnitude_bits(w);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    const bool far = __any(m > LARGEST<DT>);
-    if (far) {
-      float f = finite_max<DT>(w);
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) f = fmaxf(f, __shfl_xor(f, o, 64));
-      e = scale_exponent<FS_F32>(f);
-    } else {
-      e = exponent_of_bits<DT>(m);
-    }
-    out = u32x2_t{encode_words<DT>(w[0], w[1], e, far), encode_words<DT>(w[2], w[3], e, far)};
+    uint32_t c[2];
+    encode_group<DT>(w, e, c);
+    out = u32x2_t{c[0], c[1]};
   }
   if (in) *reinterpret_cast<u32x2_t*>(codes + row * ldc + k) = out;
   // the row's word: lane 16 g holds byte g (zeros past K)
@@ -196,19 +214,42 @@ inline bool rows_by_8(const void* C, int64_t ldc, const void* R, int64_t ldr) {
 // ------------------------------------------------------------------------------------------------
 // A workgroup takes 16 TN columns of C; its eight waves split K and are joined in order through LDS. Weights go straight
 // from HBM to registers in the instruction's own shape (a lane's two 16-byte chunks of a row's 128; a wave's load covers
-// whole lines), DEPTH stages ahead. Each wave encodes its part of the rows itself while its weights are on their way:
-// 32 values a lane and stage, 16 words of magnitudes and 16 conversions.
-template <int DT, int TN, int DEPTH>
+// whole lines), DEPTH stages ahead. While the first of them are on their way the workgroup encodes the rows into LDS,
+// eight lanes to a group: M K bytes of codes (XB at most, which bounds the rows) and a byte per
+// row and group.
+template <int DT, int TN, int DEPTH, int XB>
 __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __restrict__ X, int64_t ldx,
                                                               const uint8_t* __restrict__ W, int64_t ldw,
                                                               const uint8_t* __restrict__ wsc, uint16_t* __restrict__ C,
                                                               int64_t ldc, const uint16_t* __restrict__ R, int64_t ldr,
                                                               int M, int64_t N, int nk, bool vec) {
-  __shared__ float4_t red[8][TN][64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(XB >= 8 * TN * 1024, "the sums take the codes' place");
+  __shared__ __attribute__((aligned(1024))) char xcodes[XB];   // [stage][row][128], chunk c of a row at c ^ swap_of(row)
+  __shared__ uint8_t xexp[XB / GROUP];                          // [stage][row]
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * TN);
   const int k0 = (int)((int64_t)w * nk / 8), k1 = (int)((int64_t)(w + 1) * nk / 8);
+
+  // The rows in pieces of 16 values (a chunk of codes), thread t's being t, t + 512, ...: one batch of them ahead of the
+  // weights' loads, and always one on its way while another is encoded.
+  constexpr int BATCH = 2;
+  const int per_row = 8 * nk, pieces = M * per_row, row_step = 512 / per_row, piece_step = 512 - row_step * per_row;
+  int lrow = tid / per_row, lpiece = tid - lrow * per_row;   // the next piece to load
+  auto load_pieces = [&](u32x4 (&xp)[BATCH][2]) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const u32x4* p = reinterpret_cast<const u32x4*>(X + min(lrow, M - 1) * ldx + 16 * lpiece);
+      xp[i][0] = p[0];
+      xp[i][1] = p[1];
+      lrow += row_step;
+      lpiece += piece_step;
+      if (lpiece >= per_row) lpiece -= per_row, ++lrow;
+    }
+  };
+  u32x4 xa[BATCH][2], xb[BATCH][2];
+  load_pieces(xa);
+
   struct Stage {
     u32x4 c[TN][2];
     uint32_t s[TN];
@@ -221,8 +262,7 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
     wrow[j] = W + n * ldw + 16 * g;
     srow[j] = 4 * n;
   }
-  auto load = [&](int kt, Stage& x) {
-    const int k = min(kt, nk - 1);
+  auto load = [&](int k, Stage& x) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       x.c[j][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP));
@@ -230,22 +270,41 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
       x.s[j] = wsc[(int64_t)(k >> 2) * 4 * N + srow[j] + (k & 3)];
     }
   };
-  // the row's values of stage kt: chunks g and 4 + g of 16
-  const bool row_in = l16 < M;
-  const uint16_t* xrow = X + (row_in ? l16 : 0) * ldx + 16 * g;
-  auto load_x = [&](int kt, uint32_t (&x)[16]) {
-    const int k = min(kt, nk - 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(xrow + (int64_t)k * GROUP + 64 * (i >> 1) + 8 * (i & 1));
+  for (int d = 0; d < DEPTH; ++d)
+    if (k0 + d < k1) load(k0 + d, ring[d]);
+
+  int row = tid / per_row, piece = tid - row * per_row;   // the next piece to encode
+  auto encode_pieces = [&](const u32x4 (&xp)[BATCH][2], int first) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = row_in ? v[e] : 0u;
+    for (int i = 0; i < BATCH; ++i) {
+      if (first + i * 512 + 64 * w >= pieces) return;   // (wave-uniform; a group's 8 lanes are in or out together)
+      uint32_t x[8], c[4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = xp[i][j >> 2][j & 3];
+      int e;
+      encode_group<DT>(x, e, c);
+      if (row < M) {
+        const int at = (piece >> 3) * M + row;
+        *reinterpret_cast<u32x4*>(xcodes + at * GROUP + 16 * ((piece & 7) ^ swap_of(row))) = u32x4{c[0], c[1], c[2], c[3]};
+        if ((piece & 7) == 0) xexp[at] = (uint8_t)e;
+      }
+      row += row_step;
+      piece += piece_step;
+      if (piece >= per_row) piece -= per_row, ++row;
     }
   };
-  uint32_t xn[16];
-  load_x(k0, xn);
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) load(k0 + d, ring[d]);
+  for (int first = 0; first < pieces; first += 2 * BATCH * 512) {
+    if (first + BATCH * 512 < pieces) load_pieces(xb);
+    encode_pieces(xa, first);
+    if (first + BATCH * 512 >= pieces) break;
+    if (first + 2 * BATCH * 512 < pieces) load_pieces(xa);
+    encode_pieces(xb, first + BATCH * 512);
+  }
+  __syncthreads();
+
+  const int xrow = l16 < M ? l16 : 0;   // (lanes past the last row: results nobody stores)
+  const int c0 = 16 * (g ^ swap_of(xrow)), c1 = 16 * ((4 + g) ^ swap_of(xrow));
   float4_t acc[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -253,28 +312,17 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (kt + d >= k1) break;   // (wave-uniform)
-      uint32_t m = magnitude_bits(xn);
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-      int e = exponent_of_bits<DT>(m);
-      const bool far = __any(m > LARGEST<DT>);
-      if (far) {
-        float f = finite_max<DT>(xn);
-        f = fmaxf(f, __shfl_xor(f, 16, 64));
-        f = fmaxf(f, __shfl_xor(f, 32, 64));
-        e = scale_exponent<FS_F32>(f);
-      }
-      u32x4 xc[2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) xc[i >> 2][i & 3] = encode_words<DT>(xn[2 * i], xn[2 * i + 1], e, far);
-      load_x(kt + d + 1, xn);
+      const char* row = xcodes + ((kt + d) * M + xrow) * GROUP;
+      const i32x8 xf = both_chunks(*reinterpret_cast<const u32x4*>(row + c0), *reinterpret_cast<const u32x4*>(row + c1));
+      const uint32_t xe = xexp[(kt + d) * M + xrow];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        acc[j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), both_chunks(xc[0], xc[1]), acc[j], ring[d].s[j],
-                               (uint32_t)e);
-      load(kt + d + DEPTH, ring[d]);
+        acc[j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), xf, acc[j], ring[d].s[j], xe);
+      if (kt + d + DEPTH < k1) load(kt + d + DEPTH, ring[d]);
     }
   }
+  __syncthreads();   // every wave has read its codes
+  float4_t(*red)[TN][64] = reinterpret_cast<float4_t(*)[TN][64]>(xcodes);
 #pragma unroll
   for (int j = 0; j < TN; ++j) red[w][j][lane] = acc[j];
   __syncthreads();
@@ -287,7 +335,7 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
 #pragma unroll
     for (int r = 0; r < 4; ++r) a[r] += b[r];
   }
-  if (row_in) store_row4<DT>(a, l16, n0 + 16 * w + 4 * g, C, ldc, R, ldr, N, vec);
+  if (l16 < M) store_row4<DT>(a, l16, n0 + 16 * w + 4 * g, C, ldc, R, ldr, N, vec);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -322,11 +370,6 @@ FS_DEVICE bool tile_of(int tiles_m, int ntiles, int bm, int bn, int64_t& m0, int
   n0 = (int64_t)(in_grp / gm) * bn;
   return true;
 }
-
-// A stage's rows in LDS are 128 bytes, eight 16-byte chunks, chunk c at place c ^ swap_of(row): an operand read's 16
-// lanes take one chunk of 16 consecutive rows, which must differ in their place within 256 bytes, two rows' worth.
-// (Swapped by row & 7, as 128-byte banks would have it, half of the LDS port's time went to conflicts.)
-FS_DEVICE int swap_of(int row) { return (row >> 1) & 7; }
 
 struct Operands {
   const uint8_t *x, *w;          // codes
@@ -734,7 +777,13 @@ int64_t scale_bytes(int64_t rows, int64_t K) { return (K + 511) / 512 * rows * 4
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool short_call(int64_t M, const void* X, int64_t ldx) { return M <= SHORT_ROWS && al16(X) && ldx % 8 == 0; }
+// Whether one launch takes a call: few rows, in aligned pieces. Every workgroup encodes them for itself, 0.06 us per KB of
+// codes and round of workgroups, where the other way's two more launches cost 4.5 us: 16 x 4096 x 4096 12.0 us against
+// 14.3, 8 x 2048 x 8192 13.5 against 14.9, 8 x 4096 x 14336 22.8 against 18.8; in two rounds 4 x 28672 x 4096 32.7 against
+// 31.2, 1 x 31.1.
+bool short_call(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx) {
+  return M <= SHORT_ROWS && M * K <= (N <= 16384 ? SHORT_BYTES : 8 * 1024) && al16(X) && ldx % 8 == 0;
+}
 
 void quantize(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, uint8_t* codes, int64_t ldc, uint32_t* scales,
               hipStream_t s) {
@@ -758,13 +807,22 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
          const uint16_t* R, int64_t ldr, int64_t M, int64_t N, int64_t K, char* work, hipStream_t s) {
   const bool vec = rows_by_8(C, ldc, R, ldr);
   const int nk = (int)(K / GROUP);
-  if (short_call(M, X, ldx)) {
-    if (N <= 8192)
-      gemm_e4m3_short_kernel<DT, 1, 4><<<dim3((unsigned)((N + 15) / 16)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, R, ldr, (int)M,
-                                                                                     N, nk, vec);
-    else
-      gemm_e4m3_short_kernel<DT, 4, 2><<<dim3((unsigned)((N + 63) / 64)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, R, ldr, (int)M,
-                                                                                     N, nk, vec);
+  if (short_call(M, N, K, X, ldx)) {
+    // so many columns a workgroup that the grid is one round of the CUs where it can be
+    const int64_t tiles = (N + 15) / 16;
+#define FS_SHORT_XB(TN, DEPTH, XB)                                                                                     \
+  gemm_e4m3_short_kernel<DT, TN, DEPTH, XB><<<dim3((unsigned)((tiles + TN - 1) / TN)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, \
+                                                                                                    R, ldr, (int)M, N, nk, vec)
+#define FS_SHORT(TN, DEPTH)                                          \
+  do {                                                               \
+    if (M * K <= 32 * 1024) FS_SHORT_XB(TN, DEPTH, 32 * 1024);        \
+    else FS_SHORT_XB(TN, DEPTH, SHORT_BYTES);                        \
+  } while (0)
+    if (tiles <= 256) FS_SHORT(1, 7);
+    else if (tiles <= 512) FS_SHORT(2, 4);
+    else FS_SHORT(4, 2);
+#undef FS_SHORT_XB
+#undef FS_SHORT
     return fs::launch_status("gemm_e4m3");
   }
   uint8_t* codes = reinterpret_cast<uint8_t*>(work);
