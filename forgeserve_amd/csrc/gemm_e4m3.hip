@@ -500,15 +500,25 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
 // ------------------------------------------------------------------------------------------------
 // long batches: 256 x 256 tiles, 8 waves of 128 x 64 in two alternating groups
 // ------------------------------------------------------------------------------------------------
-// Bound by the matrix cores with the LDS port close behind: a stage of 128 is 32 instructions of 32 cycles a wave, 2048
-// cycles a SIMD, against 192 KB of operand reads (1536 cycles) and 64 KB of copies (512), the same bytes and cycles as a
-// 16-bit product's stage of 64, for twice the depth. So the loop is that product's (gemm.hip, gemm_bf16_long_kernel): four
-// phases a stage, one 64 x 32 quadrant of the wave's tile each, ordered so that each needs one new operand; the reads and
-// copies of a phase in its first half, the products in its second; waves 4..7 half a phase behind waves 0..3, so that
-// on each SIMD one wave multiplies while the other reads and copies; copies issued five phases before they are read,
-// eight per wave on their way.
+// A stage of 128 is 2048 cycles of products a SIMD (16 instructions of 64 cycles in each of its two waves), 192 KB of
+// operand reads and 64 KB of copies, and all three have to overlap. Waves w and w + 4 share a SIMD; waves 4..7 run half a
+// phase behind waves 0..3, so that one multiplies while the other reads and copies. A phase is one 64 x 64 half of the
+// wave's tile: its first half reads the operands (in a stage's first phase the W's for both) and issues copies, its
+// second, behind a barrier, multiplies. Two stages live in LDS. In halves from a stage's start (the second group one
+// later): W and X0 (rows 0-63 of each group of 128) are read in half 0, X1 in half 2; the copies that take their places,
+// two stages on, are issued in halves 2 and 4 and are read six halves later; a wave waits at the end of each first half
+// until only its eight youngest copies are on their way, one barrier at least before anyone reads the others.
+//   phase of stage kt     reads        copies                     waits for its copies of
+//   0                     W, X0        X1 of kt + 1               X1 of kt
+//   1                     X1           W and X0 of kt + 2         W and X0 of kt + 1
 // The scale words of four stages (2 KB) are one more copy per wave, issued four stages before they are read and counted
-// in that stage's waits; a lane keeps its 12 words in registers and each stage's instructions pick their byte.
+// in that stage's waits; a lane keeps its six words in registers and each stage's instructions pick their byte.
+//
+// Measured, 8005 x 28672 x 4096 with the rows' encoding (21 us): 1,230 us in 128 x 128 tiles, 999 in four phases of 64 x 32
+// quadrants a stage (the order of the 16-bit kernel, on 32 x 32 products: on 16 x 16 ones the compiler moves the sums from
+// register to register and spills), 762-822 in two (2.3-2.5 PFLOP/s, one box and another). Without the copies the loop
+// would take 675, without the operand reads 640, with neither 597, all tiles the same one (copies from L2 alone) 700: the
+// copies' way from L2 is what is left, some 10 TB/s over the chip.
 template <int DT, bool PARTIAL>
 __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint16_t* __restrict__ C, int64_t ldc,
                                                                 const uint16_t* __restrict__ R, int64_t ldr, bool vec,
@@ -762,15 +772,32 @@ __global__ void __launch_bounds__(256) gemm_e4m3_join_kernel(const float* __rest
 }
 
 struct Plan {
-  int bm, bn, splits;
+  int tile, splits;   // tile x tile
 };
-// The tile and the K splits of a shape.
+// The tile and the K splits of a shape: the cheapest of what a sweep over the 8B and 1B projections and 17 to 8000 rows
+// fits (us): each round of 256 workgroups takes its stages at `stage` and `fixed` on top (of 64 x 64 tiles two share a
+// CU, at half the rate each), and a split writes and reads its partials at 4.5 TB/s and joins them in a launch of 3.
+// What the sweep's best would have saved over these choices is 1-2 us of 15-50, 5% beyond.
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
-  const int bm = M <= 64 ? 64 : M > 1024 ? 256 : 128, bn = bm;
-  const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn), nk = K / GROUP;
-  int s = 1;
-  while (s < 8 && N % 4 == 0 && tiles * s * 2 <= 512 && nk % (8 * s) == 0 && nk / (2 * s) >= 4) s *= 2;
-  return Plan{bm, bn, s};
+  struct Cand {
+    int tile;
+    double stage, fixed;
+  };
+  static const Cand cands[] = {{64, 0.43, 3.0}, {128, 0.66, 5.0}, {256, 1.5, 10.0}};
+  const int64_t nk = K / GROUP;
+  Plan best{64, 1};
+  double least = 1e30;
+  for (const Cand& c : cands) {
+    const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + c.tile - 1) / c.tile);
+    for (int s = 1; s <= 8; s *= 2) {
+      // (a split starts at a whole word of scales; partials are stored four columns at a time)
+      if (s > 1 && (nk % (4 * s) != 0 || N % 4 != 0)) break;
+      const double us = (double)((tiles * s + 255) / 256) * ((double)(nk / s) * c.stage + c.fixed) +
+                        (s > 1 ? 3.0 + (double)s * (double)M * (double)N * 8.0 / 4.5e6 : 0.0);
+      if (us < least) least = us, best = Plan{c.tile, s};
+    }
+  }
+  return best;
 }
 
 int64_t scale_bytes(int64_t rows, int64_t K) { return (K + 511) / 512 * rows * 4; }
@@ -830,15 +857,15 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
   float* part = reinterpret_cast<float*>(xs + align256(scale_bytes(M, K)));
   quantize(X, ldx, M, K, DT, codes, K, reinterpret_cast<uint32_t*>(xs), s);
   const Plan p = plan_for(M, N, K);
-  Operands P{codes, W, xs, ws, K, ldw, M, N, nk, (int)((M + p.bm - 1) / p.bm), 0};
-  P.ntiles = P.tiles_m * (int)((N + p.bn - 1) / p.bn);
+  Operands P{codes, W, xs, ws, K, ldw, M, N, nk, (int)((M + p.tile - 1) / p.tile), 0};
+  P.ntiles = P.tiles_m * (int)((N + p.tile - 1) / p.tile);
   const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
   float* out = p.splits > 1 ? part : nullptr;
-  if (p.bm == 64)
+  if (p.tile == 64)
     gemm_e4m3_tile_kernel<DT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, C, ldc, R, ldr, vec, out);
-  else if (p.bm == 256 && out)
+  else if (p.tile == 256 && out)
     gemm_e4m3_long_kernel<DT, true><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
-  else if (p.bm == 256)
+  else if (p.tile == 256)
     gemm_e4m3_long_kernel<DT, false><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, nullptr);
   else
     gemm_e4m3_tile_kernel<DT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
