@@ -502,8 +502,12 @@ FS_DEVICE float fold_value(float x, float cM, float y, float cm) { return fmaf(x
 // Two waves on a CU (four parts) want two (3 rows of 8000-30000 keys: 68 -> 64 us); four want one (16 rows of
 // 128-1280 keys, 64 dims: 12.3 against 13.4). The last pair is consumed with nothing left to load: prefetching
 // past the end cost 64 rows of 1000-2000 keys 7 us.
-constexpr int unit_pairs(int store) { return store == FS_BF16 ? 1 : 2; }
-constexpr int part_pairs(int store, int parts) { return store == FS_BF16 ? (parts == 4 ? 2 : 1) : (parts == 4 ? 4 : 2); }
+// Of codes a pair is half the registers: two, unless 128 dims and a second half of rows leave no room (with the two
+// spilled, 64 rows of 2048-8192 keys and windows of 7 took 272 us).
+constexpr int unit_pairs(int store, int D, bool two) { return store == FS_BF16 || (D == 128 && two) ? 1 : 2; }
+constexpr int part_pairs(int store, int parts, int D, bool two) {
+  return store == FS_BF16 ? (parts == 4 ? 2 : 1) : unit_pairs(store, D, two);
+}
 
 // TWO: the tile has a second 16-row half. NP: pair buffers in registers.
 template <int D, int BSZ, bool TWO, int NP>
@@ -788,10 +792,24 @@ attn_unit_kernel(AttnParams P) {
   const int nkv = P.kv.n_kv_heads;
   const int64_t e_idx = blockIdx.x / nkv;
   const int hkv = (int)(blockIdx.x - e_idx * nkv);
-  if (e_idx >= P.n_items[0]) return;   // uniform over the workgroup
-  typedef __attribute__((address_space(4))) const AttnItem ConstItem;   // read-only: scalar loads
-  ConstItem* ep = (ConstItem*)(uintptr_t)(P.items + e_idx);
-  const int b = ep->b, z = ep->z, s = ep->s, qmax = ep->qmax;
+  int b, z, s, qmax;
+  if (ST != FS_BF16 && P.items == nullptr) {   // (a small call: no plan)
+    const int qtiles = (P.T * P.G + QTILE - 1) / QTILE;
+    const int u = (int)(e_idx / P.nsplit);
+    s = (int)(e_idx - (int64_t)u * P.nsplit);
+    b = u / qtiles;
+    z = u - b * qtiles;
+    qmax = tile_qmax(P, b, z);
+    if (s >= tile_chunks(P, qmax)) return;   // uniform over the workgroup
+  } else {
+    if (e_idx >= P.n_items[0]) return;   // uniform over the workgroup
+    typedef __attribute__((address_space(4))) const AttnItem ConstItem;   // read-only: scalar loads
+    ConstItem* ep = (ConstItem*)(uintptr_t)(P.items + e_idx);
+    b = ep->b;
+    z = ep->z;
+    s = ep->s;
+    qmax = ep->qmax;
+  }
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // wave-uniform, in a scalar register
   const int row0 = z * QTILE;
@@ -806,7 +824,7 @@ attn_unit_kernel(AttnParams P) {
   const int kbeg = s * P.split;
   const int kend = min(kbeg + P.split, qmax + 1);
 
-  wave_tiles<ST, D, BSZ, TWO, unit_pairs(ST)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc[w], red_m[w], red_l[w]);
+  wave_tiles<ST, D, BSZ, TWO, unit_pairs(ST, D, TWO)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, w, red_acc[w], red_m[w], red_l[w]);
   __syncthreads();
 
   // fold the waves' partials in wave order; wave w takes the (query half, 16-dim tile) pairs w,
@@ -860,7 +878,7 @@ FS_DEVICE float ld1_dev(__amdgpu_buffer_rsrc_t r, int off) {
 // last folds them in order and emits the rows. The arrival is counted (an agent-scope atomic), never awaited;
 // the published values cross XCDs through device-coherent accesses.
 template <int ST, int D, int BSZ, bool TWO, int PARTS>
-__global__ void __launch_bounds__(64 * UNIT_WAVES / PARTS) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ void __launch_bounds__(64 * UNIT_WAVES / PARTS) __attribute__((amdgpu_waves_per_eu(ST == FS_BF16 ? 1 : 2)))
 attn_unit_part_kernel(AttnParams P) {
   constexpr int WPP = UNIT_WAVES / PARTS;
   constexpr int MT = D / 16, GI = (TWO ? 2 : 1) * MT;
@@ -893,7 +911,7 @@ attn_unit_part_kernel(AttnParams P) {
   const int kbeg = s * P.split;
   const int kend = min(kbeg + P.split, qmax + 1);
 
-  wave_tiles<ST, D, BSZ, TWO, part_pairs(ST, PARTS)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, WPP * part + w,
+  wave_tiles<ST, D, BSZ, TWO, part_pairs(ST, PARTS, D, TWO)>(P, b, kbeg, kend, qmax, row0, nrows, rpos, hkv, WPP * part + w,
                                                      red_acc[w], red_m[w], red_l[w]);
   __syncthreads();
 
@@ -1750,6 +1768,15 @@ int attn_split() {
   return split;
 }
 
+// Over codes a wave takes a pair in about the time of a 16-bit pair, for half the bytes, so few rows of long contexts are
+// bound by their waves, not by HBM: smaller chunks make more of them. Measured (us with chunks of 4096, 8192 and 16384
+// keys; 32/8 heads, 128 dims): 3 rows of 8000-30000 keys, T = 1: 36 / 44 / 60; 64 rows of 1000-8000 keys, T = 1:
+// 118 / 110 / 106, of 2000-8000 keys, T = 5: 152 / 122 / 125.
+constexpr int E4M3_SPLIT = 8192;
+int e4m3_split() { return attn_split() < E4M3_SPLIT ? attn_split() : E4M3_SPLIT; }
+
+constexpr int PLANLESS_KEYS = 2048;   // table lengths up to which a call over codes may go without a plan
+
 int64_t nsplit_for(int32_t max_blocks, int32_t block_size, int split) {
   const int64_t S = (int64_t)max_blocks * block_size;
   return (S + split - 1) / split;
@@ -1857,7 +1884,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
   P.G = n_heads / kv->n_kv_heads;
   P.scale_log2 = scale * LOG2E;
   const bool mfma = mfma_eligible(*kv, q, q_sb, q_st, q_sh);
-  P.split = mfma ? attn_split() : GENERIC_SPLIT;
+  P.split = !mfma ? GENERIC_SPLIT : e4m3 ? e4m3_split() : attn_split();
   P.nsplit = (int32_t)nsplit_for(max_blocks, kv->block_size, P.split);
   const int64_t rows = (int64_t)B * T * n_heads;
   char* ws = reinterpret_cast<char*>(workspace);
@@ -1901,11 +1928,22 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
     key.nsplit = P.nsplit;
     key.direct = P.direct;
     key.zgroup = P.zgroup;
-    if (!(reuse_plan && last_plan == key)) {
+    const bool two = (int64_t)T * P.G > 16;   // else no tile has a second half of query rows
+    const int64_t keys = (int64_t)max_blocks * kv->block_size;
+    // few, possibly long units: several workgroups each, to keep more CUs reading
+    int parts = prefill ? 1 : split_parts(units, keys, two);
+    // Over codes, a call of short rows that all run at once does without the plan (its order matters to none of them)
+    // and without its launch, 3.5 us of 16.
+    const bool planless = e4m3 && !prefill && units <= 256 && keys <= PLANLESS_KEYS;
+    if (planless) {
+      parts = 1;
+      P.items = nullptr;
+      last_plan = PlanKey{};
+    } else if (!(reuse_plan && last_plan == key)) {
       if (prefill) attn_plan_kernel<PLAN_THREADS_PREFILL><<<1, PLAN_THREADS_PREFILL, 0, st>>>(P);
       else attn_plan_kernel<PLAN_THREADS><<<1, PLAN_THREADS, 0, st>>>(P);
     }
-    last_plan = key;
+    if (!planless) last_plan = key;
     const unsigned grid = (unsigned)units;
     if (prefill) {
       const unsigned threads = 64 * PF_WAVES;
@@ -1926,9 +1964,6 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
 #undef FS_COMMA
 #undef FS_PREFILL
     } else {
-      // few, possibly long units: several workgroups each, to keep more CUs reading
-      const bool two = (int64_t)T * P.G > 16;   // else no tile has a second half of query rows
-      const int parts = split_parts(units, (int64_t)max_blocks * kv->block_size, two);
       const unsigned pgrid = grid * (unsigned)parts, pthreads = 64 * UNIT_WAVES / (unsigned)parts;
 #define FS_ATTN_LAUNCH(ST_, D_, BS_, TWO_)                                                     \
   do {                                                                                         \

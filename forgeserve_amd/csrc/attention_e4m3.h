@@ -94,9 +94,9 @@ FS_DEVICE void tile_scores_e4m3(const u32x4 (&kf)[D / 32], const u32x4 (&qf)[2][
 
 // pair_probs with a value's scale in its probability (bf16). A score that is NaN moves no reference; its p, l and
 // sums are NaN (and partial_reference keeps such a partial from counting as empty).
-template <int DT, bool TWO>
-FS_DEVICE bool pair_probs_e4m3(const float (&sc)[2][2][4], const float (&vs)[2][4], float scale, float (&m_run)[2],
-                               float (&l_run)[2], float (&alpha)[2], u32x4 (&pf)[2]) {
+template <int DT, bool TWO, class Scales>
+FS_DEVICE bool pair_probs_e4m3(const float (&sc)[2][2][4], Scales scales, float scale, float (&m_run)[2], float (&l_run)[2],
+                               float (&alpha)[2], u32x4 (&pf)[2]) {
   constexpr int NT = TWO ? 2 : 1;
   typedef Operand<DT> O;
   float x[2];
@@ -121,35 +121,42 @@ FS_DEVICE bool pair_probs_e4m3(const float (&sc)[2][2][4], const float (&vs)[2][
       m_run[nt] = m_new;
     }
   }
+  float ref[2], sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float ref = m_run[nt] == -INFINITY ? 0.f : m_run[nt];   // (a row that has seen nothing yet: every p is 0)
-    float pv[2][4];
+  for (int nt = 0; nt < NT; ++nt) ref[nt] = m_run[nt] == -INFINITY ? 0.f : m_run[nt];   // (a row that has seen nothing yet: every p is 0)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < 2; ++u) {
+    float vs[4];
+    if (DT == FS_BF16) scales(u, vs);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pv[u][e] = fast_exp2(fmaf(sc[u][nt][e], scale, -ref));
-    l_run[nt] += ((pv[0][0] + pv[0][1]) + (pv[0][2] + pv[0][3])) + ((pv[1][0] + pv[1][1]) + (pv[1][2] + pv[1][3]));
+    for (int nt = 0; nt < NT; ++nt) {
+      float pv[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int e = 0; e < 4; ++e) pv[e] = fast_exp2(fmaf(sc[u][nt][e], scale, -ref[nt]));
+      sum[nt] += (pv[0] + pv[1]) + (pv[2] + pv[3]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float a = pv[u][2 * c], b = pv[u][2 * c + 1];
-        pf[nt][2 * u + c] = DT == FS_BF16 ? O::round2(a * vs[u][2 * c], b * vs[u][2 * c + 1]) : O::round2(a, b);
+        const float x = pv[2 * c], y = pv[2 * c + 1];
+        pf[nt][2 * u + c] = DT == FS_BF16 ? O::round2(x * vs[2 * c], y * vs[2 * c + 1]) : O::round2(x, y);
       }
+    }
   }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) l_run[nt] += sum[nt];
   return moved;
 }
 
 // The reference of a finished partial: one that saw NaN alone has none yet, and would pass for an empty one.
 FS_DEVICE float partial_reference(float m, float l) { return __builtin_isnan(l) ? 0.f : m; }
 
-// pair_step over codes: value(mt) is the pair's values of dims 16 mt .. as an operand, vs the scales of the lane's keys
-// (bf16; f16's value has them). In a pair that some row sees only in part, a value that is NaN is zeroed in the operand,
+// pair_step over codes: value(mt) is the pair's values of dims 16 mt .. as an operand, scales(u, s) the scales of the
+// lane's four keys of tile u (bf16; f16's value has them). In a pair that some row sees only in part, a value that is NaN is zeroed in the operand,
 // and a product of two indicators (which values are NaN, which keys a row sees) says which sums it belongs to: 0 * NaN
 // would reach the rows that may not see it.
-template <int DT, int D, bool TWO, bool SEEN = false, class Value>
-FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, const float (&vs)[2][4], int j0, const bool (&ok)[2],
+// again() makes the compiler take the values for new ones: else it would keep all of a pair's operands in registers from
+// the search for NaN to the products, and from there to the indicators.
+template <int DT, int D, bool TWO, bool SEEN = false, class Value, class Again, class Scales>
+FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Again again, Scales scales, int j0, const bool (&ok)[2],
                               bool fresh, int qmax, const int (&rpos)[2], int rmin, float scale, float4_t (&acc)[D / 16][2],
                               float (&m_run)[2], float (&l_run)[2]) {
   constexpr int MT = D / 16;
@@ -178,7 +185,7 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, const flo
   }
   u32x4 pf[2];
   float alpha[2];
-  const bool moved = pair_probs_e4m3<DT, TWO>(s, vs, scale, m_run, l_run, alpha, pf);
+  const bool moved = pair_probs_e4m3<DT, TWO>(s, scales, scale, m_run, l_run, alpha, pf);
   if (moved && !fresh) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -187,37 +194,37 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, const flo
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[mt][nt][e] *= alpha[nt];
   }
-  // operand bits of one where a row at `pos` sees the key
-  auto seen_bits = [&](int pos, uint32_t ones) {
+  // all bits of an operand's keys that a row at `pos` sees
+  auto seen_bits = [&](int pos) {
     u32x4 k;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int last = last_key(c >> 1, pos), e = 2 * (c & 1);   // keys e, e + 1
-      k[c] = ((e <= last ? 0xffffu : 0u) | (e < last ? 0xffff0000u : 0u)) & ones;
+      k[c] = (e <= last ? 0xffffu : 0u) | (e < last ? 0xffff0000u : 0u);
     }
     return k;
   };
+  // all bits of an operand's values that are NaN (codes have no infinities)
+  auto nan_bits = [](u32x4 v) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t x = ~v[c] & O::EXPONENTS;
+      v[c] = ((x & 0xffffu) == 0 ? 0xffffu : 0u) | ((x >> 16) == 0 ? 0xffff0000u : 0u);
+    }
+    return v;
+  };
   bool any_nan = false;
-  u32x4 keep = {~0u, ~0u, ~0u, ~0u}, seen[2];
+  u32x4 keep = {~0u, ~0u, ~0u, ~0u};
   if (!full) {
-    keep = seen_bits(qmax, ~0u);
+    keep = seen_bits(qmax);
     // a probability is 0 where its key is hidden, whatever the scale there
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      seen[nt] = seen_bits(rpos[nt], O::ONES);
-      pf[nt] &= seen_bits(rpos[nt], ~0u);
-    }
-    uint32_t bad = 0;
+    for (int nt = 0; nt < NT; ++nt) pf[nt] &= seen_bits(rpos[nt]);
+    u32x4 bad = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const u32x4 v = value(mt) & keep;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t x = ~v[c] & O::EXPONENTS;   // a half of it is 0 where that value is not finite
-        bad |= (x & 0xffffu) == 0 || (x >> 16) == 0;
-      }
-    }
-    any_nan = __any(bad != 0);
+    for (int mt = 0; mt < MT; ++mt) bad |= nan_bits(value(mt) & keep);
+    any_nan = __any((bad[0] | bad[1] | bad[2] | bad[3]) != 0);
+    again();
   }
   __builtin_amdgcn_sched_barrier(0);
   u32x4 v[2][2];
@@ -233,26 +240,7 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, const flo
     __builtin_amdgcn_sched_barrier(0);
     if (!full) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) now[i] &= keep;
-      if (any_nan) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          u32x4 nan;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t x = ~now[i][c] & O::EXPONENTS;
-            nan[c] = ((x & 0xffffu) == 0 ? 0xffffu : 0u) | ((x >> 16) == 0 ? 0xffff0000u : 0u);
-          }
-          now[i] &= ~nan;
-          nan &= O::ONES;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float4_t n = O::mfma(nan, seen[nt], float4_t{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[mt + i][nt][e] = n[e] > 0.f ? __uint_as_float(0x7fc00000u) : acc[mt + i][nt][e];
-          }
-        }
-      }
+      for (int i = 0; i < 2; ++i) now[i] &= any_nan ? keep & ~nan_bits(now[i]) : keep;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -260,6 +248,20 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, const flo
       if (TWO) acc[mt + i][1] = O::mfma(now[i], pf[1], acc[mt + i][1]);
     }
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if (!full && any_nan) {
+    again();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const u32x4 seen = seen_bits(rpos[nt]) & O::ONES;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float4_t n = O::mfma(nan_bits(value(mt)) & keep & O::ONES, seen, float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = n[e] > 0.f ? __uint_as_float(0x7fc00000u) : acc[mt][nt][e];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
 }
 
@@ -425,19 +427,28 @@ __device__ __attribute__((always_inline)) inline void attn_wave_tiles_e4m3(const
       __builtin_amdgcn_sched_barrier(0);
       load_keys(p + NP, kb[j]);
     }
-    float vs[2][4];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) four_scales(vb[j].s[u], vs[u]);
+    auto scales = [&](int u, float (&vs)[4]) { four_scales(vb[j].s[u], vs); };
     u32x4 vso = {};
-    if (DT == FS_F16) vso = scale_operand(vs[0], vs[1]);
+    if (DT == FS_F16) {
+      float a[4], c[4];
+      scales(0, a);
+      scales(1, c);
+      vso = scale_operand(a, c);
+    }
     auto value = [&](int mt) {
       const u32x4 o = operand8<DT>(vb[j].v[0][mt >> 2][mt & 3], vb[j].v[1][mt >> 2][mt & 3], 1.f);
       return DT == FS_F16 ? times8(o, vso) : o;
     };
+    auto again = [&]() {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) asm volatile("" : "+v"(vb[j].v[u][c]));
+    };
     if constexpr (decltype(seen)::value)
-      pair_step_e4m3<DT, D, TWO, true>(sc, value, vs, 0, {true, true}, p == 0, 0, rpos, rmin, scale, acc, m_run, l_run);
+      pair_step_e4m3<DT, D, TWO, true>(sc, value, again, scales, 0, {true, true}, p == 0, 0, rpos, rmin, scale, acc, m_run, l_run);
     else
-      pair_step_e4m3<DT, D, TWO>(sc, value, vs, pair_key(p), {there(p, 0), there(p, 1)}, p == 0, qmax, rpos, rmin, scale, acc,
+      pair_step_e4m3<DT, D, TWO>(sc, value, again, scales, pair_key(p), {there(p, 0), there(p, 1)}, p == 0, qmax, rpos, rmin, scale, acc,
                                  m_run, l_run);
     if (refill) {
       __builtin_amdgcn_sched_barrier(0);

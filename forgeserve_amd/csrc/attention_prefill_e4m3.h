@@ -132,8 +132,11 @@ attn_prefill_e4m3_kernel(AttnParams P) {
   };
   static_assert(PF_TILES == 8, "a stage's scales are one word a lane");
 
-  // one stage's codes into operands
+  // one stage's codes into operands (its addresses from a thread index that the compiler takes for new each time: kept
+  // over the stages they would need registers, and spilled ones are waited for with the copies)
   auto convert = [&](int k) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
     const char* raw = ring + (k % NS) * STAGE;
     const uint32_t* sc = sring[k % NS];
     const uint8_t* sb = reinterpret_cast<const uint8_t*>(sc);
@@ -240,16 +243,14 @@ attn_prefill_e4m3_kernel(AttnParams P) {
         tile_scores_e4m3<DT, D, true>(kf, qf, sc[h]);
         __builtin_amdgcn_sched_barrier(0);   // (one tile's keys in registers)
       }
-      float vs[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      auto scales = [&](int h, float (&vs)[4]) {
         const float4_t x = *reinterpret_cast<const float4_t*>(&vscale[u + h][4 * g]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vs[h][e] = x[e];
-      }
+        for (int e = 0; e < 4; ++e) vs[e] = x[e];
+      };
       const int key0 = kbeg + 32 * pair;
       const bool ok[2] = {mapped(key0), 2 * pair + 1 < ntiles && mapped(key0 + 16)};
-      pair_step_e4m3<DT, D, true>(sc, value, vs, key0, ok, fresh, qmax, rpos, rmin, scale, acc, m_run, l_run);
+      pair_step_e4m3<DT, D, true>(sc, value, [] { asm volatile("" ::: "memory"); }, scales, key0, ok, fresh, qmax, rpos, rmin, scale, acc, m_run, l_run);
       fresh = false;
     }
   }

@@ -450,6 +450,29 @@ def test_long_context(dtype):
     check_attention(out[0].cpu(), want, mag, dtype)
 
 
+@pytest.mark.parametrize("dtype,hd,heads,T", [(BF16, 128, 4, 1), (F16, 64, 8, 1), (BF16, 128, 8, 4)])
+def test_lengths_about_a_chunk(dtype, hd, heads, T):
+    """Rows that end just before, at and behind the borders of the chunks of keys, alone and in a batch."""
+    g = torch.Generator().manual_seed(15)
+    bs, kv = 16, 1
+    ends = [2047, 2048, 2049, 4096, 4097, 8191, 8192, 8193, 8256, 16384, 16385]
+    nb = -(-max(ends) // bs)
+    pool = make_pool(hd, kv, bs, nb, dtype, heads=heads)
+    k, v = fill(pool, g)
+    table = torch.randperm(nb, generator=g).view(1, nb).int()
+    pos = torch.stack([torch.arange(n - T, n) for n in ends]).int()
+    q = torch.randn(len(ends), T, heads, hd, generator=g).to(dtype)
+    scale = 1 / math.sqrt(hd)
+    out = ops.paged_attention(q.to(DEV), pool.layout(0), table.expand(len(ends), -1).contiguous().to(DEV), pos.to(DEV), scale)
+    kr, vr = row_keys(k, table[0], bs), row_keys(v, table[0], bs)
+    for i, n in enumerate(ends):
+        want, mag = ref.attention(q[i], kr, vr, pos[i], scale)
+        check_attention(out[i].cpu(), want, mag, dtype)
+        short = table[:, : -(-n // bs)].contiguous().to(DEV)       # a table no longer than the row
+        one = ops.paged_attention(q[i: i + 1].to(DEV), pool.layout(0), short, pos[i: i + 1].to(DEV), scale)
+        assert torch.equal(one[0], out[i]), n
+
+
 def test_packed_rows_behind_the_last_sequence_are_left_alone():
     g = torch.Generator().manual_seed(15)
     pool = make_pool(128, 2, 16, 40, BF16, heads=8)
