@@ -3,6 +3,106 @@
 
 namespace {
 
+// The bytes of four codes that are NaN: 0x80 there, 0 elsewhere.
+FS_DEVICE uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// The four bytes of nan_codes as four bits.
+FS_DEVICE uint32_t code_bits(uint32_t n) { return (n >> 7 & 1u) | (n >> 14 & 2u) | (n >> 21 & 4u) | (n >> 28 & 8u); }
+
+// pair_step over operands without NaN (the workgroup's conversion zeroes such values and says which they were): the
+// products run without a branch. nan: some value of the stage was NaN; then nans(mt) has a bit for each of the lane's
+// eight values of dims 16 mt .., and a product of two indicators (which values are NaN, which keys a row sees) says
+// which sums it belongs to.
+template <int DT, int D, class Value, class Nans, class Scales>
+FS_DEVICE void pair_step_clean(const float4_t (&sc)[2][2], Value value, bool nan, Nans nans, Scales scales, int j0,
+                               const bool (&ok)[2], bool fresh, const int (&rpos)[2], int rmin, float scale,
+                               float4_t (&acc)[D / 16][2], float (&m_run)[2], float (&l_run)[2]) {
+  constexpr int MT = D / 16;
+  typedef Operand<DT> O;
+  const int g = (threadIdx.x & 63) >> 4;
+  const bool full = ok[0] && ok[1] && j0 + 31 <= rmin;   // wave-uniform
+  // the row sees the lane's keys e <= last_key(u, row's position)
+  auto last_key = [&](int u, int pos) { return (ok[u] ? pos : -1) - j0 - 16 * u - 4 * g; };
+  float s[2][2][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][nt][e] = sc[u][nt][e];
+  if (!full) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int last = last_key(u, rpos[nt]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][nt][e] = e <= last ? s[u][nt][e] : -INFINITY;
+      }
+  }
+  u32x4 pf[2];
+  float alpha[2];
+  const bool moved = pair_probs_e4m3<DT, true>(s, scales, scale, m_run, l_run, alpha, pf);
+  if (moved && !fresh) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] *= alpha[nt];
+  }
+  // all bits of an operand's keys that a row at `pos` sees
+  auto seen_bits = [&](int pos) {
+    u32x4 k;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int last = last_key(c >> 1, pos), e = 2 * (c & 1);   // keys e, e + 1
+      k[c] = (e <= last ? 0xffffu : 0u) | (e < last ? 0xffff0000u : 0u);
+    }
+    return k;
+  };
+  if (!full) {   // a probability is 0 where its key is hidden, whatever the scale there
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) pf[nt] &= seen_bits(rpos[nt]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  u32x4 v[2][2];
+  v[0][0] = value(0);
+  v[0][1] = value(1);
+#pragma unroll
+  for (int mt = 0; mt < MT; mt += 2) {
+    u32x4(&now)[2] = v[mt / 2 & 1], (&next)[2] = v[(mt / 2 & 1) ^ 1];
+    if (mt + 2 < MT) {
+      next[0] = value(mt + 2);
+      next[1] = value(mt + 3);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      acc[mt + i][0] = O::mfma(now[i], pf[0], acc[mt + i][0]);
+      acc[mt + i][1] = O::mfma(now[i], pf[1], acc[mt + i][1]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (nan) {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const u32x4 seen = seen_bits(rpos[nt]) & O::ONES;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t bits = nans(mt);
+        u32x4 bad;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          bad[c] = ((bits >> (2 * c) & 1u ? 0xffffu : 0u) | (bits >> (2 * c + 1) & 1u ? 0xffff0000u : 0u)) & O::ONES;
+        const float4_t n = O::mfma(bad, seen, float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = n[e] > 0.f ? __uint_as_float(0x7fc00000u) : acc[mt][nt][e];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // prefill kernel: attn_prefill_kernel's split, order and folds over codes
 // ------------------------------------------------------------------------------------------------
@@ -29,6 +129,8 @@ attn_prefill_e4m3_kernel(AttnParams P) {
   __shared__ __attribute__((aligned(1024))) char vop[PF_TILES * 2 * TK];   // values by pair
   __shared__ __attribute__((aligned(256))) uint32_t sring[NS][64];         // a stage's scale bytes: 32 per tile
   __shared__ __attribute__((aligned(16))) float vscale[PF_TILES][16];      // the values' scales of the operands' stage
+  __shared__ uint32_t vnan[PF_TILES / 2][MT / 4][64];   // a bit for each value of the operands' stage that was NaN
+  __shared__ int nan_stage;                         // the last stage that had one (+ 1)
   __shared__ int tbl[MAX_SPLIT / 16 + 1];           // the chunk's physical blocks (-1: unmapped)
 
   const int nkv = P.kv.n_kv_heads;
@@ -69,6 +171,7 @@ attn_prefill_e4m3_kernel(AttnParams P) {
   const int blk0 = kbeg / BS;
   const int nblk = ntiles > 0 ? (kbeg + 16 * ntiles - 1) / BS - blk0 + 1 : 0;
   int unmapped = 0;
+  if (tid == 0) nan_stage = 0;
   for (int i = tid; i < nblk; i += THREADS) {
     const int blk = blk0 + i;
     int v = blk < P.max_blocks ? P.table[(int64_t)b * P.table_stride + blk] : -1;
@@ -84,58 +187,56 @@ attn_prefill_e4m3_kernel(AttnParams P) {
   // pool's order: of the keys chunk c * 16 + slot (16 dims of a slot), of the values whole 4-key groups.
   const int p = w % CPT;
   const bool kpart = p < CPT / 2;
-  uint32_t coff;
-  {
-    const int ch = (kpart ? p : p - CPT / 2) * 64 + lane;
-    coff = kpart ? (uint32_t)((ch >> 4) * 16 * BS + (ch & 15) * 16) : (uint32_t)(16 * ch);
-  }
   const char* pool_h = reinterpret_cast<const char*>(kpart ? key_tile(P.kv, 0, hkv) : value_tile(P.kv, 0, hkv));
   const char* pool_s = reinterpret_cast<const char*>(tile_scales(P.kv, 0, hkv));
   const int64_t blk_stride = kpart ? P.kv.k_block : P.kv.v_block;
   const int slot_mul = kpart ? 16 : D;
   const uint32_t ring0 = (uint32_t)(uintptr_t)ring, sring0 = (uint32_t)(uintptr_t)sring;
 
-  // Lane j holds the byte offsets of the tile at ring position 64 * win + j (codes relative to pool_h, scales to
-  // pool_s), refreshed when a stage enters the next 64 positions; a position without a tile copies the last tile again.
-  static_assert(64 % PF_TILES == 0, "a stage's positions lie in one 64-position window");
-  uint32_t woff_lo = 0, woff_hi = 0, soff_lo = 0, soff_hi = 0;
-  auto refresh = [&](int win) {
-    const int j = min(64 * win + lane, 2 * npairs - 1);
-    const int t = min(2 * pf_pair(j >> 1, npairs) + (j & 1), ntiles - 1);
+  // The copies of the next stage, k: lane j finds the byte offsets of the stage's tile j / 8 (codes relative to pool_h,
+  // scales to pool_s); a position behind the last pair copies some tile again. All of it comes from a thread index that
+  // the compiler takes for new each time, here and in convert(): kept over the stages the addresses would need registers,
+  // and spilled ones are waited for together with the copies.
+  int copied = 0;   // the pair copied next
+  auto issue = [&](int k) {
+    int lane = threadIdx.x;
+    asm volatile("" : "+v"(lane));
+    lane &= 63;
+    int pair = copied;
+#pragma unroll
+    for (int i = 1; i < PF_TILES / 2; ++i) {
+      copied = pf_next_pair(copied, npairs);
+      pair = lane >> 4 >= i ? copied : pair;
+    }
+    copied = pf_next_pair(copied, npairs);
+    const int t = min(2 * pair + (lane >> 3 & 1), ntiles - 1);
     const int key0 = kbeg + 16 * t;
     const int bi = key0 / BS;
     const int ph = tbl[bi - blk0];
     const int64_t pb = ph >= 0 ? ph : 0;         // unmapped: block 0, masked in the step
     const int slot0 = key0 - bi * BS;
-    const uint64_t o = (uint64_t)(pb * blk_stride + slot0 * slot_mul), os = (uint64_t)(pb * P.kv.k_slot + slot0);
-    woff_lo = (uint32_t)o;
-    woff_hi = (uint32_t)(o >> 32);
-    soff_lo = (uint32_t)os;
-    soff_hi = (uint32_t)(os >> 32);
-  };
-  auto issue = [&](int k) {
-    if ((k & (64 / PF_TILES - 1)) == 0) refresh(k / (64 / PF_TILES));
+    const uint64_t o = (uint64_t)(pb * blk_stride + slot0 * slot_mul);
+    const int ch = (kpart ? p : p - CPT / 2) * 64 + lane;
+    const uint32_t coff = kpart ? (uint32_t)((ch >> 4) * 16 * BS + (ch & 15) * 16) : (uint32_t)(16 * ch);
     const uint32_t base = ring0 + (uint32_t)((k % NS) * STAGE) + (uint32_t)(p * 1024);
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
       const int u = (w + PF_WAVES * i) / CPT;   // the stage's tile this copy fills
-      const int j = (PF_TILES * k + u) & 63;
-      const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)woff_hi, j) << 32) |
-                         (uint32_t)__builtin_amdgcn_readlane((int)woff_lo, j);
-      pf_dma16(pool_h + o, coff, base + (uint32_t)(u * TB));
+      const uint64_t ou = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(o >> 32), 8 * u) << 32) |
+                          (uint32_t)__builtin_amdgcn_readlane((int)o, 8 * u);
+      pf_dma16(pool_h + ou, coff, base + (uint32_t)(u * TB));
     }
     // the stage's scales, 8 words a tile (four of the keys, four of the values): every wave copies them, to the same
     // place, so that all of them count the same copies
-    const int j = (PF_TILES * k + (lane >> 3)) & 63, word = lane & 7;
-    const uint64_t o = ((uint64_t)(uint32_t)__shfl((int)soff_hi, j, 64) << 32) | (uint32_t)__shfl((int)soff_lo, j, 64);
-    pf_dma4(pool_s + o + (word < 4 ? 4 * word : BS + 4 * (word - 4)), sring0 + (uint32_t)((k % NS) * 256));
+    const int word = lane & 7;
+    pf_dma4(pool_s + pb * P.kv.k_slot + slot0 + (word < 4 ? 4 * word : BS + 4 * (word - 4)), sring0 + (uint32_t)((k % NS) * 256));
   };
+  static_assert(THREADS % D == 0, "");
   static_assert(PF_TILES == 8, "a stage's scales are one word a lane");
 
-  // one stage's codes into operands (its addresses from a thread index that the compiler takes for new each time: kept
-  // over the stages they would need registers, and spilled ones are waited for with the copies)
+  // one stage's codes into operands
   auto convert = [&](int k) {
-    int tid = threadIdx.x;
+    uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const char* raw = ring + (k % NS) * STAGE;
     const uint32_t* sc = sring[k % NS];
@@ -143,7 +244,7 @@ attn_prefill_e4m3_kernel(AttnParams P) {
     if (tid < PF_TILES * 16) vscale[tid >> 4][tid & 15] = scale_value(sb[32 * (tid >> 4) + 16 + (tid & 15)]);
 #pragma unroll
     for (int i = 0; i < PF_TILES * D / THREADS; ++i) {   // keys: chunk x = c * 16 + slot of tile u
-      const int n = i * THREADS + tid, u = n / D, x = n % D, c = x >> 4, slot = x & 15;
+      const uint32_t u = i * (THREADS / D) + tid / D, x = tid % D, c = x >> 4, slot = x & 15;
       const u32x4 q = *reinterpret_cast<const u32x4*>(raw + u * TB + 16 * x);
       const float sk = scale_value(sb[32 * u + slot]);
       char* to = kop + u * 2 * TK + (2 * (c >> 2) * 64 + (c & 3) * 16 + slot) * 16;   // k-step 2 (c / 4), then the next
@@ -152,16 +253,35 @@ attn_prefill_e4m3_kernel(AttnParams P) {
     }
 #pragma unroll
     for (int i = 0; i < (PF_TILES / 2 * D + THREADS - 1) / THREADS; ++i) {   // values: place x of both tiles of a pair
-      const int n = i * THREADS + tid, pr = n / D, x = n % D;
-      if (PF_TILES / 2 * D % THREADS && n >= PF_TILES / 2 * D) break;
-      const int gk = x / (D / 4), y = x % (D / 4), q = y >> 4, r = y & 15;   // 4-key group, 64 dims, dim % 16
-      const u32x4 a = *reinterpret_cast<const u32x4*>(raw + (2 * pr) * TB + TK + 16 * x);
-      const u32x4 c = *reinterpret_cast<const u32x4*>(raw + (2 * pr + 1) * TB + TK + 16 * x);
+      const uint32_t pr = i * (THREADS / D) + tid / D, x = tid % D;
+      if (PF_TILES / 2 * D % THREADS && pr >= PF_TILES / 2) break;
+      const uint32_t gk = x / (D / 4), y = x % (D / 4), q = y >> 4, r = y & 15;   // 4-key group, 64 dims, dim % 16
+      u32x4 a = *reinterpret_cast<const u32x4*>(raw + (2 * pr) * TB + TK + 16 * x);
+      u32x4 c = *reinterpret_cast<const u32x4*>(raw + (2 * pr + 1) * TB + TK + 16 * x);
+      uint32_t bits = 0, found = 0;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) found |= nan_codes(a[m]) | nan_codes(c[m]);
+      if (found) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t na = nan_codes(a[m]), nc = nan_codes(c[m]);
+          bits |= (code_bits(na) | code_bits(nc) << 4) << (8 * m);
+          a[m] &= ~((na >> 7) * 255u);
+          c[m] &= ~((nc >> 7) * 255u);
+        }
+        nan_stage = k + 1;   // (by any number of threads)
+      }
+      vnan[pr][q][gk * 16 + r] = bits;
       u32x4 vso = {};
-      if (DT == FS_F16) {
+      if (DT == FS_F16) {   // (a slot that was never written may hold any byte: what stands there must stay finite)
         float sa[4], sd[4];
         four_scales(sc[8 * (2 * pr) + 4 + gk], sa);
         four_scales(sc[8 * (2 * pr + 1) + 4 + gk], sd);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sa[e] = fminf(sa[e], scale_value(ScaleRange<FS_F16>::HI));
+          sd[e] = fminf(sd[e], scale_value(ScaleRange<FS_F16>::HI));
+        }
         vso = scale_operand(sa, sd);
       }
       char* to = vop + pr * 4 * TK + (4 * q * 64 + gk * 16 + r) * 16;
@@ -220,6 +340,7 @@ attn_prefill_e4m3_kernel(AttnParams P) {
     __syncthreads();   // stage k has landed for every wave, and the operands of stage k-1 are no longer being read
     convert(k);
     __syncthreads();
+    const bool nan = __builtin_amdgcn_readfirstlane(nan_stage) == k + 1;
     if (k + NS < nst) issue(k + NS);
 #pragma unroll 1
     for (int u = 0; u < PF_TILES; u += 2) {
@@ -250,7 +371,8 @@ attn_prefill_e4m3_kernel(AttnParams P) {
       };
       const int key0 = kbeg + 32 * pair;
       const bool ok[2] = {mapped(key0), 2 * pair + 1 < ntiles && mapped(key0 + 16)};
-      pair_step_e4m3<DT, D, true>(sc, value, [] { asm volatile("" ::: "memory"); }, scales, key0, ok, fresh, qmax, rpos, rmin, scale, acc, m_run, l_run);
+      auto nans = [&](int mt) { return vnan[u >> 1][mt >> 2][lane] >> (8 * (mt & 3)); };
+      pair_step_clean<DT, D>(sc, value, nan, nans, scales, key0, ok, fresh, rpos, rmin, scale, acc, m_run, l_run);
       fresh = false;
     }
   }
