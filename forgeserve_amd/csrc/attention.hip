@@ -1809,6 +1809,13 @@ int split_parts(int64_t units, int64_t keys, bool two) {
   return units <= SPLIT_UNITS_MAX / 2 && keys >= (two ? 4096 : 2048) ? 4 : 2;
 }
 
+// The same over codes, whose waves are bound by their instructions: two workgroups a unit, each wave with a SIMD of its
+// own, and no more. Measured (us: one, two and four; 32/8 heads, 128 dims): one row of 4000 keys, T = 1: 28.7 / 24.9 /
+// 26.2, of 8000: 46.0 / 36.9 / 36.8; 8 of 512-4096: 31.9 / 27.5 / 28.8; 3 of 8000-30000: 57.6 / 48.1 / 47.1; T = 5, 8 of
+// 512-4096: 36.3 / 36.6 / 42.2, 2 of 2000-6000: 45.0 / 42.8 / 46.1. Shorter rows need no plan when they are not split (one
+// of 2000: 15.2 / 18.3 / 20.0).
+int split_parts_e4m3(int64_t units, int64_t keys) { return units <= SPLIT_UNITS_MAX && keys > PLANLESS_KEYS ? 2 : 1; }
+
 }  // namespace
 
 extern "C" int32_t fs_paged_attention_split(void) { return attn_split(); }
@@ -1931,12 +1938,11 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
     const bool two = (int64_t)T * P.G > 16;   // else no tile has a second half of query rows
     const int64_t keys = (int64_t)max_blocks * kv->block_size;
     // few, possibly long units: several workgroups each, to keep more CUs reading
-    int parts = prefill ? 1 : split_parts(units, keys, two);
+    int parts = prefill ? 1 : e4m3 ? split_parts_e4m3(units, keys) : split_parts(units, keys, two);
     // Over codes, a call of short rows that all run at once does without the plan (its order matters to none of them)
     // and without its launch, 3.5 us of 16.
     const bool planless = e4m3 && !prefill && units <= 256 && keys <= PLANLESS_KEYS;
     if (planless) {
-      parts = 1;
       P.items = nullptr;
       last_plan = PlanKey{};
     } else if (!(reuse_plan && last_plan == key)) {
@@ -1967,7 +1973,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
       const unsigned pgrid = grid * (unsigned)parts, pthreads = 64 * UNIT_WAVES / (unsigned)parts;
 #define FS_ATTN_LAUNCH(ST_, D_, BS_, TWO_)                                                     \
   do {                                                                                         \
-    if (parts == 4) attn_unit_part_kernel<ST_, D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
+    if (ST_ == FS_BF16 && parts == 4) attn_unit_part_kernel<FS_BF16, D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
     else if (parts == 2) attn_unit_part_kernel<ST_, D_, BS_, TWO_, 2><<<pgrid, pthreads, 0, st>>>(P); \
     else attn_unit_kernel<ST_, D_, BS_, TWO_><<<grid, 64 * UNIT_WAVES, 0, st>>>(P);              \
   } while (0)
