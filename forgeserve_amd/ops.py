@@ -82,8 +82,9 @@ def kv_layout_e4m3(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, dtype
     (num_blocks, n_kv_heads, 2, block_size), the exponent bytes e of the keys', then of the values' scales
     2^(e - 127). The blocks and heads may have any strides; a tile, and a pair of scale rows, is contiguous.
     head_dim is a multiple of 16 and at most 256, block_size a multiple of 4. The scale is the smallest power of
-    two that brings a group's largest magnitude to 448 or less (fs_kv_layout says what lies beyond the limits);
-    attention is fast for bfloat16 and float16 with head_dim 64 or 128 and block_size % 16 == 0."""
+    two that brings a group's largest magnitude to 448 or less (fs_kv_layout says what lies beyond the limits).
+    Attention is fast for bfloat16 and float16 with head_dim 64 or 128 and block_size % 16 == 0. A write call
+    names a slot once: of two tokens for the same one a mixture may remain."""
     if any(t.dtype not in (torch.uint8, torch.float8_e4m3fn) for t in (k, v)) or scales.dtype != torch.uint8:
         raise ValueError(f"8-bit pool: codes must be float8_e4m3fn or uint8, scales uint8: {k.dtype}, {v.dtype}, "
                          f"{scales.dtype}")
@@ -93,7 +94,8 @@ def kv_layout_e4m3(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, dtype
         raise ValueError(f"8-bit pool: shapes {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)}")
     nb, h, c, bs, w = k.shape
     d = 16 * c
-    if w != 16 or v.shape != (nb, h, bs // 4, d, 4) or scales.shape != (nb, h, 2, bs) or bs % 4 or d > 256:
+    if (min(nb, h, c, bs) < 1 or w != 16 or v.shape != (nb, h, bs // 4, d, 4) or scales.shape != (nb, h, 2, bs) or bs % 4
+            or d > 256):
         raise ValueError(f"8-bit pool: shapes {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)} (head_dim a "
                          "multiple of 16 up to 256, block_size a multiple of 4)")
     if not (k[0, 0].is_contiguous() and v[0, 0].is_contiguous() and scales[0, 0].is_contiguous()):
@@ -160,9 +162,13 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out = a @ w.T (+ residual) with the weight in 8-bit floating point, as quantize_e4m3 leaves it (w (n, k) codes with
     16-byte aligned rows, w_scales (ceil(k / 512), n, 4)), and a (bfloat16 or float16) brought to the same form within
-    the call: nn.Linear with half the weight bytes and twice the matrix rate of gemm's. Sums are float32; product and
-    residual are rounded once, to a's dtype. A row's last bit may depend on how many rows the call has."""
+    the call: nn.Linear with half the weight bytes and twice the matrix rate of gemm's. Sums are float32 (of each eight
+    products the matrix instruction drops what lies more than 13 binary places below the largest); product and residual
+    are rounded once, to a's dtype. A row's last bit may depend on how many rows the call has. out may be the
+    residual itself, but shares no memory with a or w."""
     require_device(a, w, w_scales)
+    if not a.device == w.device == w_scales.device or any(t is not None and t.device != a.device for t in (out, residual)):
+        raise ValueError("gemm_e4m3: tensors on different devices")
     m, lda = _rows(a)
     n, ldb = _rows(w)
     k = a.shape[1]
@@ -179,14 +185,13 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
         raise ValueError("gemm_e4m3: out shape/dtype")
     ldr = 0
     if residual is not None:
-        require_device(residual)
         _, ldr = _rows(residual)
         if residual.shape != out.shape or residual.dtype != a.dtype:
             raise ValueError("gemm_e4m3: residual shape/dtype")
     if m == 0 or n == 0:
         return out
     lib = _lib.load()
-    ws = _persistent_ws("gemm_e4m3", lib.fs_gemm_e4m3_workspace_size(m, n, k), a.device)
+    ws = _ws(lib.fs_gemm_e4m3_workspace_size(m, n, k), a.device)   # (of the current stream: calls on two do not share it)
     check(lib.fs_gemm_e4m3(ptr(a), lda, ptr(w), ldb, ptr(w_scales), ptr(out), ldc, ptr(residual), ldr, m, n, k, _dt(a), ptr(ws),
                            ws.numel(), stream_ptr()), "gemm_e4m3")
     return out

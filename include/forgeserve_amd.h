@@ -56,7 +56,9 @@ extern "C" {
  *   scales             k + k_group + block*k_slot + head*k_dim: block_size bytes of the keys', then of the values'
  * v_slot and v_dim are 0. head_dim % 16 == 0 and at most 256, block_size % 4 == 0; k, v and the tiles' strides are
  * multiples of 16, those of the scales of 4. The fast attention path takes bf16 and f16 with head_dim 64 or 128 and
- * block_size % 16 == 0. The rotary write rotates in f32 and rounds once (queries to the dtype, keys to the codes). */
+ * block_size % 16 == 0. The rotary write rotates in f32 and rounds once (queries to the dtype, keys to the codes).
+ * A token's codes and scale are several stores: of two tokens of one call that name the same slot (of a block that two
+ * table rows share, say) a mixture of both may remain, so a call names a slot once. */
 typedef struct fs_kv_layout {
   void* k;
   void* v;
@@ -285,8 +287,9 @@ int fs_quantize_e4m3(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_
 
 /* C[M,N] = X[M,K] . W[N,K]^T (+ R[M,N]) (nn.Linear: model.py:57-60, 88-90, with the residual add of model.py:105-106)
  * with W as fs_quantize_e4m3 leaves it (ldw bytes from row to row, a multiple of 16) and X encoded in the same way
- * within the call, f32 accumulation, and one rounding of product and residual to the dtype (bf16 or f16). Rows of X, C
- * and R may be strided and of any alignment; columns are contiguous. K % 128 == 0. The order of a sum over K goes by M
+ * within the call, f32 accumulation (of eights of products, of each of which the matrix instruction drops what lies more
+ * than 13 binary places below the largest), and one rounding of product and residual to the dtype (bf16 or f16). C may be
+ * R itself, but shares no memory with X or W. Rows of X, C and R may be strided and of any alignment; columns are contiguous. K % 128 == 0. The order of a sum over K goes by M
  * (as do the tiles), so a row's last bit may differ between a short and a long batch. workspace: at least
  * fs_gemm_e4m3_workspace_size bytes for this M, 256-byte aligned. */
 int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* w_scales, void* C, int64_t ldc,

@@ -182,3 +182,19 @@ def test_projection_wrappers_refuse(monkeypatch):
         ops.gemm_e4m3(x, w, s, residual=torch.zeros(2, 8))
     with pytest.raises(ValueError, match="128"):
         ops.quantize_e4m3(torch.zeros(3, 200))
+
+
+def test_empty_layouts_are_refused():
+    for kw in (dict(nb=0), dict(h=0), dict(hd=0), dict(bs=0)):
+        with pytest.raises(ValueError, match="8-bit pool"):
+            ops.kv_layout_e4m3(*tensors(**kw), torch.bfloat16)
+
+
+def test_projection_refuses_tensors_of_two_devices(monkeypatch):
+    monkeypatch.setattr(ops, "require_device", lambda *t: None)
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    w, s = torch.zeros(32, 128, dtype=torch.uint8), torch.zeros(1, 32, 4, dtype=torch.uint8)
+    y = torch.zeros(2, 32, dtype=torch.bfloat16)
+    for kw in (dict(w=w.to("meta")), dict(w_scales=s.to("meta")), dict(out=y.to("meta")), dict(residual=y.to("meta"))):
+        with pytest.raises(ValueError, match="devices"):
+            ops.gemm_e4m3(x, **(dict(w=w, w_scales=s) | kw))

@@ -1,5 +1,7 @@
 """Projections in 8-bit floating point against their definition in 64 bits."""
 
+import math
+
 import pytest
 import torch
 
@@ -181,3 +183,70 @@ def test_an_mlp_of_8_bit_projections():
         h = ops.silu_mul(gu)
         y = ops.gemm_e4m3(h, cd, sd, residual=x)
         check(y, encoded(h.cpu()), values(cd, sd, f), x.cpu())
+
+
+# tiles of 256 whole and cut off, with and without a split of K, and what the smaller tiles take of large calls
+@pytest.mark.parametrize("m,n,k", [(700, 4096, 14336), (2050, 2048, 8192), (4097, 1100, 640), (1100, 9000, 256), (2300, 3001, 384),
+                                   (512, 6144, 4096)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_calls(dtype, m, n, k):
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x = (torch.randn(m, k, generator=g, device=DEV) * torch.exp(0.7 * torch.randn(k, generator=g, device=DEV))).to(dtype)
+    w = torch.randn(n, k, generator=g, device=DEV).mul_(0.02)
+    codes, scales = ops.quantize_e4m3(w)
+    xv, wv = (t.to(DEV) for t in (encoded(x.cpu()), values(codes, scales, k)))
+    want, mag = xv @ wv.t().contiguous(), xv.abs() @ wv.abs().t().contiguous()
+
+    # What the matrix instruction drops: it adds eight products at a time (of eight neighbours in K), aligned to the
+    # largest, and of each of the other seven loses less than 2^-13 of the largest's power of two (found with a pair
+    # that cancels beside products of every smaller size: those 13 places below count in full, those 14 below not at all
+    # where they share its eight, in full elsewhere). So an element is off by less than 7 * 2^-13 max |x| max |w| of each
+    # eight, plus 2^-23 of mag for each float32 sum on its way (an instruction takes 64 of K or more and adds 8 to 16
+    # eights), plus its rounding. That bound grows as K where the errors grow as its root, so the whole result's norm is
+    # held to more: rounding is off by at most eps / sqrt(12) of it, and the dropped parts were measured at 2.5e-5 of it, a
+    # fifth of the 2^-13 allowed here.
+    eights = [t.abs().unflatten(1, (k // 8, 8)).amax(2) for t in (xv, wv)]
+    dropped = 7 * 2.0 ** -13 * (eights[0] @ eights[1].t().contiguous()) + (k // 64 + 16) * 2.0 ** -23 * mag
+    eps = torch.finfo(dtype).eps
+
+    def close(got, plus):
+        y = want + plus
+        err = (got.double() - y).abs()
+        assert (err <= (1 + eps) * dropped + eps / 2 * y.abs() + (2.0 ** -25 if dtype == F16 else 0)).all()
+        assert err.norm() <= (1.02 * eps / math.sqrt(12)) * y.norm() + 2.0 ** -13 * want.norm()
+
+    close(ops.gemm_e4m3(x, codes, scales), 0)
+    r = torch.randn(m, n, generator=g, device=DEV).to(dtype)
+    back = torch.full((m, n + 12), 3.0, dtype=dtype, device=DEV)
+    close(ops.gemm_e4m3(x, codes, scales, out=back[:, 5: 5 + n], residual=r), r.double())
+    assert (back[:, :5] == 3).all() and (back[:, 5 + n:] == 3).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 640, 512), (50, 512, 2048), (448, 520, 3584), (2050, 2048, 1024)])
+def test_result_over_its_residual(m, n, k):
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x = torch.randn(m, k, generator=g, device=DEV).bfloat16()
+    codes, scales = ops.quantize_e4m3(torch.randn(n, k, generator=g, device=DEV))
+    r = torch.randn(m, n, generator=g, device=DEV).bfloat16()
+    want = ops.gemm_e4m3(x, codes, scales, residual=r)
+    got = ops.gemm_e4m3(x, codes, scales, out=r, residual=r)
+    assert got is r and torch.equal(got, want)
+
+
+def test_calls_on_two_streams():
+    """Calls that split K and hold encoded rows, in flight together."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    k, n, m = 8192, 1024, 200
+    codes, scales = ops.quantize_e4m3(torch.randn(n, k, generator=g, device=DEV))
+    xs = [torch.randn(m, k, generator=g, device=DEV).bfloat16() for _ in range(2)]
+    want = [ops.gemm_e4m3(x, codes, scales) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.gemm_e4m3(xs[i], codes, scales))
+    torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(w, y) for y in ys)
