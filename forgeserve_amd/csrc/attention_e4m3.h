@@ -149,14 +149,18 @@ FS_DEVICE bool pair_probs_e4m3(const float (&sc)[2][2][4], Scales scales, float 
 // The reference of a finished partial: one that saw NaN alone has none yet, and would pass for an empty one.
 FS_DEVICE float partial_reference(float m, float l) { return __builtin_isnan(l) ? 0.f : m; }
 
+// The bytes of four codes that are NaN: 0x80 there, 0 elsewhere.
+FS_DEVICE uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // pair_step over codes: value(mt) is the pair's values of dims 16 mt .. as an operand, scales(u, s) the scales of the
-// lane's four keys of tile u (bf16; f16's value has them). In a pair that some row sees only in part, a value that is NaN is zeroed in the operand,
-// and a product of two indicators (which values are NaN, which keys a row sees) says which sums it belongs to: 0 * NaN
-// would reach the rows that may not see it.
+// lane's four keys of tile u (bf16; f16's value has them), nans() not 0 if one of the lane's codes of values is NaN. In a
+// pair that some row sees only in part, a value that is NaN is zeroed in the operand, and a product of two indicators
+// (which values are NaN, which keys a row sees) says which sums it belongs to: 0 * NaN would reach the rows that may not
+// see it. (The search runs over the codes, four at a time: over the operands it took longer than the rest of the pair.)
 // again() makes the compiler take the values for new ones: else it would keep all of a pair's operands in registers from
 // the search for NaN to the products, and from there to the indicators.
-template <int DT, int D, bool TWO, bool SEEN = false, class Value, class Again, class Scales>
-FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Again again, Scales scales, int j0, const bool (&ok)[2],
+template <int DT, int D, bool TWO, bool SEEN = false, class Value, class Nans, class Again, class Scales>
+FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Nans nans, Again again, Scales scales, int j0, const bool (&ok)[2],
                               bool fresh, int qmax, const int (&rpos)[2], int rmin, float scale, float4_t (&acc)[D / 16][2],
                               float (&m_run)[2], float (&l_run)[2]) {
   constexpr int MT = D / 16;
@@ -220,10 +224,7 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Again aga
     // a probability is 0 where its key is hidden, whatever the scale there
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) pf[nt] &= seen_bits(rpos[nt]);
-    u32x4 bad = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) bad |= nan_bits(value(mt) & keep);
-    any_nan = __any((bad[0] | bad[1] | bad[2] | bad[3]) != 0);
+    any_nan = __any(nans() != 0);
     again();
   }
   __builtin_amdgcn_sched_barrier(0);
@@ -238,9 +239,9 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Again aga
       next[1] = value(mt + 3);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (!full) {
+    if (!full && any_nan) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) now[i] &= any_nan ? keep & ~nan_bits(now[i]) : keep;
+      for (int i = 0; i < 2; ++i) now[i] &= keep & ~nan_bits(now[i]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -433,11 +434,28 @@ __device__ __attribute__((always_inline)) inline void attn_wave_tiles_e4m3(const
       float a[4], c[4];
       scales(0, a);
       scales(1, c);
+      if constexpr (!decltype(seen)::value) {   // (a slot that was never written may hold any byte: it must stay finite)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = fminf(a[e], scale_value(ScaleRange<FS_F16>::HI));
+          c[e] = fminf(c[e], scale_value(ScaleRange<FS_F16>::HI));
+        }
+      }
       vso = scale_operand(a, c);
     }
     auto value = [&](int mt) {
       const u32x4 o = operand8<DT>(vb[j].v[0][mt >> 2][mt & 3], vb[j].v[1][mt >> 2][mt & 3], 1.f);
       return DT == FS_F16 ? times8(o, vso) : o;
+    };
+    auto nans = [&]() {
+      uint32_t n = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n |= nan_codes(vb[j].v[u][c][e]);
+      return n;
     };
     auto again = [&]() {
 #pragma unroll
@@ -446,9 +464,9 @@ __device__ __attribute__((always_inline)) inline void attn_wave_tiles_e4m3(const
         for (int c = 0; c < C; ++c) asm volatile("" : "+v"(vb[j].v[u][c]));
     };
     if constexpr (decltype(seen)::value)
-      pair_step_e4m3<DT, D, TWO, true>(sc, value, again, scales, 0, {true, true}, p == 0, 0, rpos, rmin, scale, acc, m_run, l_run);
+      pair_step_e4m3<DT, D, TWO, true>(sc, value, nans, again, scales, 0, {true, true}, p == 0, 0, rpos, rmin, scale, acc, m_run, l_run);
     else
-      pair_step_e4m3<DT, D, TWO>(sc, value, again, scales, pair_key(p), {there(p, 0), there(p, 1)}, p == 0, qmax, rpos, rmin, scale, acc,
+      pair_step_e4m3<DT, D, TWO>(sc, value, nans, again, scales, pair_key(p), {there(p, 0), there(p, 1)}, p == 0, qmax, rpos, rmin, scale, acc,
                                  m_run, l_run);
     if (refill) {
       __builtin_amdgcn_sched_barrier(0);

@@ -3,8 +3,6 @@
 
 namespace {
 
-// The bytes of four codes that are NaN: 0x80 there, 0 elsewhere.
-FS_DEVICE uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // The four bytes of nan_codes as four bits.
 FS_DEVICE uint32_t code_bits(uint32_t n) { return (n >> 7 & 1u) | (n >> 14 & 2u) | (n >> 21 & 4u) | (n >> 28 & 8u); }
 
