@@ -723,6 +723,7 @@ FS_DEVICE void attn_emit(const AttnParams& P, int b, int s, int kbeg, int hkv, i
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const bool direct = P.direct && (rp < P.split || P.nsplit == 1);
   if (direct ? s != 0 : rp < kbeg) return;
+  if ((ST & FS_STORE_E4M3) && rp < 0) L = 0.f;   // (over codes such a row may have summed what the others see)
   const int t = rr / P.G, h = hkv * P.G + (rr - t * P.G);
   if (direct) {
     if (!token_exists(P, b, t)) return;

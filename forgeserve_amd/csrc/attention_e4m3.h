@@ -266,6 +266,19 @@ FS_DEVICE void pair_step_e4m3(const float4_t (&sc)[2][2], Value value, Nans nans
   }
 }
 
+// The smallest position of a tile's queries, padding apart (rows_min_pos's -1 would send every pair of a padded window
+// through the masks: 32 padded windows of 5 over 128-2048 keys, 64 dims, took 24 us for 16). What a padding row sums over
+// pairs that all others see is never looked at: attn_emit gives it zeros.
+FS_DEVICE int rows_min_seen(const int (&rpos)[2], int nrows) {
+  const int l16 = threadIdx.x & 15;
+  int v = 0x7ffffffe;
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt) v = 16 * nt + l16 < nrows && rpos[nt] >= 0 ? min(v, rpos[nt]) : v;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) v = min(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
 // The queries of a wave's 32-row tile as operands: Q[row][16 (g + 4j) + 8h .. +8] in k-step 2j + h.
 template <int DT, int D, int NT>
 FS_DEVICE void load_queries_e4m3(const AttnParams& P, int b, int hkv, int row0, int nrows, u32x4 (&qf)[2][D / 32]) {
@@ -403,7 +416,7 @@ __device__ __attribute__((always_inline)) inline void attn_wave_tiles_e4m3(const
   float m_run[2] = {-INFINITY, -INFINITY};
   float l_run[2] = {0.f, 0.f};
 
-  const int rmin = rows_min_pos(rpos, nrows);
+  const int rmin = rows_min_seen(rpos, nrows);
   const int n_seen = rmin + 1 > kbeg ? min((rmin + 1 - kbeg) >> 5, ntiles >> 1) : 0;   // pairs all rows see
   const int n_full = all_mapped && n_seen > w ? (n_seen - w + UNIT_WAVES - 1) / UNIT_WAVES : 0;
   const float scale = positive_scale(P.scale_log2);

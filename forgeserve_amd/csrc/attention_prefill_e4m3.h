@@ -159,7 +159,7 @@ attn_prefill_e4m3_kernel(AttnParams P) {
     rpos[nt] = (r < nrows) ? posb[(row0 + r) / P.G] : -1;
   }
   const int qmax = nrows > 0 ? tile_qmax(P, b, z) : -1;
-  const int rmin = rows_min_pos(rpos, nrows);
+  const int rmin = rows_min_seen(rpos, nrows);
   const int ntiles_w = nrows > 0 ? min(max((min(kbeg + P.split, qmax + 1) - kbeg + 15) >> 4, 0), ntiles) : 0;
 
   u32x4 qf[2][KS];

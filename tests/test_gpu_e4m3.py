@@ -473,6 +473,42 @@ def test_lengths_about_a_chunk(dtype, hd, heads, T):
         assert torch.equal(one[0], out[i]), n
 
 
+@pytest.mark.parametrize("dtype,hd,heads,kv,T", [(BF16, 128, 8, 2, 6), (F16, 64, 8, 2, 6), (BF16, 64, 8, 1, 40), (F16, 128, 4, 1, 70)])
+@pytest.mark.parametrize("n", [40, 700, 9000])
+def test_padding_between_the_tokens_of_a_window(dtype, hd, heads, kv, T, n):
+    """Padding rows anywhere in a window give zeros, whatever their neighbours see (NaN among it), and change nothing of
+    theirs; a window of padding alone gives zeros."""
+    g = torch.Generator().manual_seed(n + T)
+    bs = 16
+    nb = -(-(n + T) // bs)
+    pool = make_pool(hd, kv, bs, 3 * nb, dtype, heads=heads)
+    k, v = fill(pool, g)
+    pool.v[0].view(torch.uint8)[0, 0, 0, 5, 1] = 0x7f    # NaN: slot 1 of block 0
+    d = int((ref.value_order(hd) == 5).nonzero())
+    v[0, 0, 1, d] = float("nan")
+    tables = torch.arange(3 * nb).view(3, nb).int()      # row 0 sees the NaN
+    pos = torch.stack([torch.arange(n, n + T)] * 3).int()
+    pad = torch.rand(3, T, generator=g) < 0.4
+    pad[1, 0] = pad[0, -1] = True
+    pad[2] = True
+    pos[pad] = -1
+    q = torch.randn(3, T, heads, hd, generator=g).to(dtype)
+    scale = 1 / math.sqrt(hd)
+    out = ops.paged_attention(q.to(DEV), pool.layout(0), tables.to(DEV), pos.to(DEV), scale)
+    assert not out[pad.to(DEV)].any()
+    for i in range(2):
+        want, mag = ref.attention(q[i], row_keys(k, tables[i], bs), row_keys(v, tables[i], bs), pos[i], scale)
+        there = ~pad[i]
+        got = out[i].cpu()
+        nan = want.isnan()
+        assert torch.equal(got.isnan()[there], nan[there])
+        check_attention(torch.where(nan, 0.0, got.float())[there].to(dtype), torch.where(nan, 0.0, want)[there],
+                        torch.where(nan, 0.0, mag)[there], dtype)
+    # a row alone has the same bits
+    one = ops.paged_attention(q[1:2].to(DEV), pool.layout(0), tables[1:2].to(DEV), pos[1:2].to(DEV), scale)
+    assert torch.equal(one[0], out[1])
+
+
 def test_packed_rows_behind_the_last_sequence_are_left_alone():
     g = torch.Generator().manual_seed(15)
     pool = make_pool(128, 2, 16, 40, BF16, heads=8)
