@@ -5,8 +5,8 @@
 // key_pos <= query_pos mask, scaled_dot_product_attention with scale 1/sqrt(D)).
 //
 // Work split (all kernels): the keys of a row are cut into fixed chunks of `split` absolute positions
-// (512 for the float32 and generic kernels, FS_ATTN_SPLIT (default 16384) for the MFMA kernels; fixed for the life
-// of the process); chunk s covers keys
+// (512 for the float32 and generic kernels, FS_ATTN_SPLIT (default 16384) for the MFMA kernels, at most 8192 of them
+// over e4m3 codes; fixed for the life of the process); chunk s covers keys
 // [s*split, (s+1)*split). Each workgroup produces the softmax partial
 // (running max m, sum l, unnormalised output acc) of its chunk, and attn_combine merges the chunks of
 // a query in increasing chunk order. A query at position p only ever reads the chunks that hold
@@ -21,8 +21,9 @@
 //   O^T[dim, row] += V^T . P^T v_mfma_f32_16x16x32_bf16, A = 16 dims x 4 keys of each tile of a pair
 // With the transposed products every lane owns whole query rows (row = lane % 16), so the softmax
 // statistics, the P operand and the O rescale stay in the lane's own registers.
-// float32 in such a layout takes the same products on v_mfma_f32_16x16x4_f32; any other type or layout the
-// scalar kernel.
+// float32 in such a layout takes the same products on v_mfma_f32_16x16x4_f32; a pool of e4m3 codes with bf16 or f16
+// rows takes this path with the codes made operands in registers (unit kernels) or once per workgroup (prompts); any
+// other type or layout the scalar kernels.
 #include <math.h>
 #include <stdlib.h>
 

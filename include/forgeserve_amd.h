@@ -154,7 +154,7 @@ int fs_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
  * several prompts at once. workspace: fs_paged_attention_workspace_size(S, T, ...). */
 /* Keys per chunk of the MFMA attention path (FS_ATTN_SPLIT, default 16384), fixed for the life of the
  * process: a query at position p reads chunks 0 .. p / split and, past the first, its output is merged
- * from per-chunk partials. No counterpart in the reference (it gathers every key); for callers and
+ * from per-chunk partials. Over e4m3 codes a chunk is 8192 keys, or this if it is smaller. No counterpart in the reference (it gathers every key); for callers and
  * benchmarks that report how a workload is split. */
 int32_t fs_paged_attention_split(void);
 
