@@ -1636,9 +1636,7 @@ __global__ void __launch_bounds__(64) attn_generic_e4m3_kernel(AttnParams P) {
         decode4(*reinterpret_cast<const uint32_t*>(value_tile(P.kv, blk, hkv) + value_code(P.kv, (j0 + jj) % BS, d)), f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pj = ps[jj + e];
-          if (pj == 0.f) continue;   // a masked key, or one past kend: whatever lies there adds nothing
-          a = fmaf(pj, f[e], a);
+          if (j0 + jj + e < kend) a = fmaf(ps[jj + e], f[e], a);   // (past kend lies whatever was there)
         }
       }
       acc[c] = a;

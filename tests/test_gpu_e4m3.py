@@ -473,6 +473,29 @@ def test_lengths_about_a_chunk(dtype, hd, heads, T):
         assert torch.equal(one[0], out[i]), n
 
 
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (BF16, 128), (F16, 64), (BF16, 96), (F32, 16)])
+@pytest.mark.parametrize("n", [6, 32, 700])
+def test_a_nan_value_without_weight_is_still_seen(dtype, hd, n):
+    """0 * NaN: a visible key's NaN reaches the output however small the key's probability, in its dim alone."""
+    g = torch.Generator().manual_seed(hd + n)
+    bs = 16
+    nb = -(-n // bs)
+    pool = make_pool(hd, 1, bs, nb, dtype, heads=2)
+    k, v = fill(pool, g)
+    pool.v[0].view(torch.uint8)[0, 0, 0, 5, 3] = 0xff    # slot 3 of block 0
+    d = int((ref.value_order(hd) == 5).nonzero())
+    tables = torch.arange(nb, dtype=torch.int32, device=DEV)[None]
+    q = (row_keys(k, tables[0].cpu(), bs)[0, 5] * 60).to(dtype).expand(1, 1, 2, hd).contiguous()
+    pos = torch.tensor([[n - 1]], dtype=torch.int32)
+    out = ops.paged_attention(q.to(DEV), pool.layout(0), tables, pos.to(DEV), 1.0).cpu()
+    assert out[..., d].isnan().all()
+    out[..., d] = 0
+    v[0, 0, 3, d] = 0
+    want, mag = ref.attention(q[0], row_keys(k, tables[0].cpu(), bs), row_keys(v, tables[0].cpu(), bs), pos[0], 1.0)
+    want[..., d] = 0
+    check_attention(out[0], want, mag, dtype)
+
+
 @pytest.mark.parametrize("dtype,hd,heads,kv,T", [(BF16, 128, 8, 2, 6), (F16, 64, 8, 2, 6), (BF16, 64, 8, 1, 40), (F16, 128, 4, 1, 70)])
 @pytest.mark.parametrize("n", [40, 700, 9000])
 def test_padding_between_the_tokens_of_a_window(dtype, hd, heads, kv, T, n):
