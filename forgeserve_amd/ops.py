@@ -105,6 +105,12 @@ def kv_layout_e4m3(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, dtype
                     scales.data_ptr() - k.data_ptr())
 
 
+def _check_current(what: str, t: torch.Tensor) -> None:
+    """A launch goes to the current device's stream."""
+    if t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 def _check_rows(what: str, t_dtype: torch.dtype, layout: KVLayout) -> None:
     """A pool of codes takes and gives rows of its own dtype only."""
     if layout.dtype & STORE_E4M3 and DTYPE_CODE.get(t_dtype) != layout.dtype & ~STORE_E4M3:
@@ -146,6 +152,7 @@ def quantize_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     448 or less, so a value is kept within 2^-4 of it (2^-19 of the group's largest, if it is below 2^-15 of that).
     What is not finite becomes NaN."""
     require_device(x)
+    _check_current("quantize_e4m3", x)
     m, ldx = _rows(x)
     k = x.shape[1]
     if k % 128 or k == 0:
@@ -169,6 +176,7 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
     require_device(a, w, w_scales)
     if not a.device == w.device == w_scales.device or any(t is not None and t.device != a.device for t in (out, residual)):
         raise ValueError("gemm_e4m3: tensors on different devices")
+    _check_current("gemm_e4m3", a)
     m, lda = _rows(a)
     n, ldb = _rows(w)
     k = a.shape[1]

@@ -198,3 +198,14 @@ def test_projection_refuses_tensors_of_two_devices(monkeypatch):
     for kw in (dict(w=w.to("meta")), dict(w_scales=s.to("meta")), dict(out=y.to("meta")), dict(residual=y.to("meta"))):
         with pytest.raises(ValueError, match="devices"):
             ops.gemm_e4m3(x, **(dict(w=w, w_scales=s) | kw))
+
+
+def test_tensors_of_another_device_than_the_current_are_refused(monkeypatch):
+    class Elsewhere:
+        device = torch.device("cuda", 1)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="current device"):
+        ops._check_current("gemm_e4m3", Elsewhere())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    ops._check_current("gemm_e4m3", Elsewhere())
