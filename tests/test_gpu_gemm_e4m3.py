@@ -250,3 +250,58 @@ def test_calls_on_two_streams():
     torch.cuda.synchronize()
     for w, ys in zip(want, got):
         assert all(torch.equal(w, y) for y in ys)
+
+
+@pytest.mark.parametrize("dtype,T", [(BF16, 1), (BF16, 5), (F16, 3), (BF16, 40)])
+def test_a_block_in_8_bits(dtype, T):
+    """The attention half of a decoder block, all of it over codes: the fused projection, its rotation and write into the
+    pool, the attention over it and the output projection with its residual; each step against 64 bits from its own
+    inputs, eagerly and replayed from a graph."""
+    from forgeserve_amd import ModelConfig, PagedKVPool
+
+    g = torch.Generator().manual_seed(T)
+    heads, kv, hd, b, bs, ctx = 8, 2, 64, 3, 16, 90
+    d = heads * hd
+    pool = PagedKVPool(ModelConfig(vocab_size=32, d_model=d, n_layers=1, n_heads=heads, n_kv_heads=kv, ffn_dim=64,
+                                   max_seq_len=1024), b * 9, bs, dtype=dtype, device=DEV, cache_dtype=torch.float8_e4m3fn)
+    tables = torch.randperm(b * 9, generator=g).view(b, 9).int().to(DEV)
+    angle = torch.rand(256, hd // 2, generator=g) * 6.28
+    cos, sin = angle.cos().to(DEV), angle.sin().to(DEV)
+    (cq, sq), (co, so) = (ops.quantize_e4m3(torch.randn(n, d, generator=g).mul_(0.05).to(DEV)) for n in ((heads + 2 * kv) * hd, d))
+    old = torch.randn(b * ctx, (heads + 2 * kv) * hd, generator=g).to(dtype).to(DEV)     # what the pool holds already
+    ops.qkv_rope_write(old, torch.arange(ctx, dtype=torch.int32).repeat(b).to(DEV), ctx, heads, cos, sin, tables, pool.layout(0))
+    x = torch.randn(b * T, d, generator=g).to(dtype).to(DEV)
+    pos = (ctx + torch.arange(T, dtype=torch.int32)).repeat(b, 1).to(DEV)
+
+    def step():
+        qkv = ops.gemm_e4m3(x, cq, sq)
+        q = ops.qkv_rope_write(qkv, pos.view(-1), T, heads, cos, sin, tables, pool.layout(0))
+        a = ops.paged_attention(q.view(b, T, heads, hd), pool.layout(0), tables, pos, hd ** -0.5)
+        return qkv, q, a, ops.gemm_e4m3(a.view(b * T, d), co, so, residual=x)
+
+    qkv, q, a, y = step()
+    check(qkv, encoded(x.cpu()), values(cq, sq, d))
+    k_all, v_all = (t.cpu().double() for t in ops.paged_gather(pool.layout(0), tables, dtype, DEV))
+    for i in range(b):
+        want, mag = ref.attention(q.view(b, T, heads, hd)[i].cpu(), k_all[i], v_all[i], pos[i].cpu(), hd ** -0.5)
+        eps = torch.finfo(dtype).eps / 2       # p and the result rounded to the type, scores and sums in float32
+        assert ((a[i].cpu().double() - want).abs() <= (1.02 * eps + 1e-4) * mag + eps * want.abs() + 2.0 ** -24).all()
+    check(y, encoded(a.view(b * T, d).cpu()), values(co, so, d), x.cpu())
+    # the keys as written: rotated in float32, then within half a step of a code (2^-4 of it, or 2^-10 of the scale,
+    # which is less than 2^-17 of the largest)
+    k1, k2 = (t.double().cpu() for t in qkv.view(b, T, -1, hd)[:, :, heads: heads + kv].chunk(2, -1))
+    c, s = (t[ctx: ctx + T, None].double().cpu() for t in (cos, sin))
+    rot = torch.cat([k1 * c - k2 * s, k2 * c + k1 * s], -1).transpose(1, 2)
+    near = 2.0 ** -4 * rot.abs() + 2.0 ** -17 * rot.abs().amax(-1, keepdim=True)
+    assert ((k_all[:, :, ctx: ctx + T] - rot).abs() <= near * 1.001).all()
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        x.copy_(torch.randn(b * T, d, generator=g))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, w) for u, w in zip(captured, eager))
