@@ -292,21 +292,23 @@ FS_DEVICE void store8(typename Elem<DT>::T* p, const float (&v)[8]) {   // 16-by
   }
 }
 
-// One wave per tile: (row b, table entry j, head h) in the outputs' order of heads. Keys: 8 consecutive dims of a
-// slot per lane; values: four keys of 8 consecutive dims per lane, so that both sides' stores are 8 consecutive
-// elements and a row's lanes lie side by side. A block id outside the pool reads as zeros. Bound by HBM: 16 rows of 256
-// blocks, 8 heads of 128, 16-bit outputs: 404 MB in 77-87 us, 4.6-5.2 TB/s.
+// Two waves per tile, one for its keys and one for its values: (row b, table entry j, head h) in the outputs' order of
+// heads. Keys: 8 consecutive dims of a slot per lane; values: four keys of 8 consecutive dims per lane, so that both sides'
+// stores are 8 consecutive elements and a row's lanes lie side by side. A block id outside the pool reads as zeros. Bound
+// by HBM: 16 rows of 256 blocks, 8 heads of 128, 16-bit outputs: 404 MB in 77-86 us, 4.7-5.2 TB/s; small calls by one load
+// after another (64 blocks: 5.7 us; with one wave a tile 7.7).
 template <int DT>
 __global__ void __launch_bounds__(256) gather_e4m3_kernel(fs_kv_layout kv, const int32_t* __restrict__ table,
                                                           int64_t table_stride, int32_t max_blocks,
                                                           typename Elem<DT>::T* __restrict__ k_out,
-                                                          typename Elem<DT>::T* __restrict__ v_out, int64_t tiles) {
-  const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                          typename Elem<DT>::T* __restrict__ v_out, uint32_t tiles) {
+  const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const uint32_t tile = unit >> 1;
   if (tile >= tiles) return;
   const int lane = threadIdx.x & 63, D = kv.head_dim, BS = kv.block_size, Hkv = kv.n_kv_heads;
-  const int h = (int)(tile % Hkv);
-  const int64_t bj = tile / Hkv;
-  const int64_t b = bj / max_blocks, j = bj - b * max_blocks;
+  const uint32_t bj = tile / (uint32_t)Hkv, row = bj / (uint32_t)max_blocks;
+  const int h = (int)(tile - bj * (uint32_t)Hkv);
+  const int64_t b = row, j = bj - row * (uint32_t)max_blocks;
   const int64_t blk = table[b * table_stride + j];
   const bool ok = blk >= 0 && blk < kv.num_blocks;
   const int64_t out0 = ((b * Hkv + h) * max_blocks + j) * BS * (int64_t)D;
@@ -314,21 +316,31 @@ __global__ void __launch_bounds__(256) gather_e4m3_kernel(fs_kv_layout kv, const
   const uint8_t* vt = value_tile(kv, ok ? blk : 0, h);
   const uint8_t* sc = tile_scales(kv, ok ? blk : 0, h);
   const int c8 = D / 8;
-  for (int i = lane; i < BS * c8; i += 64) {
-    const int slot = i / c8, d = 8 * (i - slot * c8);
-    float v[8];
-    const u32x2_t w = *reinterpret_cast<const u32x2_t*>(kt + key_code(kv, slot, d));
-    const float s = ok ? scale_value(sc[slot]) : 0.f;
+  for (int i0 = unit & 1 ? BS * c8 : lane; i0 < BS * c8; i0 += 256) {   // four at a time, their loads together
+    u32x2_t w[4];
+    float s[4];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      float f[4];
-      decode4(w[q], f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * q + e] = ok ? f[e] * s : 0.f;
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(i0 + 64 * u, BS * c8 - 1), slot = i / c8, d = 8 * (i - slot * c8);
+      w[u] = *reinterpret_cast<const u32x2_t*>(kt + key_code(kv, slot, d));
+      s[u] = ok ? scale_value(sc[slot]) : 0.f;
     }
-    store8<DT>(k_out + out0 + (int64_t)slot * D + d, v);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 64 * u, slot = i / c8, d = 8 * (i - slot * c8);
+      if (i >= BS * c8) break;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float f[4];
+        decode4(w[u][q], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = ok ? f[e] * s[u] : 0.f;
+      }
+      store8<DT>(k_out + out0 + (int64_t)slot * D + d, v);
+    }
   }
-  for (int i = lane; i < BS / 4 * c8; i += 64) {
+  for (int i = unit & 1 ? lane : BS / 4 * c8; i < BS / 4 * c8; i += 64) {
     const int g = i / c8, d = 8 * (i - g * c8);
     float v[4][8];
     float s[4];
@@ -420,11 +432,11 @@ int paged_gather_e4m3(const fs_kv_layout& kv, const int32_t* tables, int64_t tab
   FS_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0,
                "paged_gather: outputs of an 8-bit pool must be 16-byte aligned");
   const int64_t tiles = (int64_t)B * max_blocks * kv.n_kv_heads;
-  FS_CHECK_ARG(tiles / 4 < 0x7fffffff, "paged_gather: %lld tiles", (long long)tiles);
-  const dim3 grid((unsigned)((tiles + 3) / 4));
+  FS_CHECK_ARG(tiles < 0x3fffffff, "paged_gather: %lld tiles", (long long)tiles);
+  const dim3 grid((unsigned)((tiles + 1) / 2));
 #define FS_LAUNCH(DT)                                                                                       \
   gather_e4m3_kernel<DT><<<grid, 256, 0, s>>>(kv, tables, table_stride, max_blocks, (typename Elem<DT>::T*)k_out, \
-                                              (typename Elem<DT>::T*)v_out, tiles)
+                                              (typename Elem<DT>::T*)v_out, (uint32_t)tiles)
   switch (row_dtype(kv)) {
     case FS_F32: FS_LAUNCH(FS_F32); break;
     case FS_BF16: FS_LAUNCH(FS_BF16); break;
