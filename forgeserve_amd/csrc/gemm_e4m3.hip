@@ -774,29 +774,31 @@ __global__ void __launch_bounds__(256) gemm_e4m3_join_kernel(const float* __rest
 }
 
 struct Plan {
-  int tile, splits;   // tile x tile
+  int bm, bn, splits;
 };
 // The tile and the K splits of a shape: the cheapest of what a sweep over the 8B and 1B projections and 17 to 8000 rows
 // fits (us): each round of 256 workgroups takes its stages at `stage` and `fixed` on top (of 64 x 64 tiles two share a
 // CU, at half the rate each), and a split writes and reads its partials at 4.5 TB/s and joins them in a launch of 3.
-// What the sweep's best would have saved over these choices is 1-2 us of 15-50, 5% beyond.
+// What the sweep's best would have saved over these choices is 1-2 us of 15-50, 5% beyond. Without the 256 x 128 tiles,
+// which copy three quarters of 128 x 128's bytes for a product, 256 x 28672 x 4096 took 53.8 us for 45.1, 1000 x 6144 x 4096
+// 52.1 for 42.3, 448 x 16384 x 2048 33.0 for 28.1, 2000 x 4096 x 4096 55.6 for 46.0.
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
   struct Cand {
-    int tile;
+    int bm, bn;
     double stage, fixed;
   };
-  static const Cand cands[] = {{64, 0.43, 3.0}, {128, 0.66, 5.0}, {256, 1.5, 10.0}};
+  static const Cand cands[] = {{64, 64, 0.43, 3.0}, {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0}, {256, 256, 1.5, 10.0}};
   const int64_t nk = K / GROUP;
-  Plan best{64, 1};
+  Plan best{64, 64, 1};
   double least = 1e30;
   for (const Cand& c : cands) {
-    const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + c.tile - 1) / c.tile);
+    const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
     for (int s = 1; s <= 8; s *= 2) {
       // (a split starts at a whole word of scales; partials are stored four columns at a time)
       if (s > 1 && (nk % (4 * s) != 0 || N % 4 != 0)) break;
       const double us = (double)((tiles * s + 255) / 256) * ((double)(nk / s) * c.stage + c.fixed) +
                         (s > 1 ? 3.0 + (double)s * (double)M * (double)N * 8.0 / 4.5e6 : 0.0);
-      if (us < least) least = us, best = Plan{c.tile, s};
+      if (us < least) least = us, best = Plan{c.bm, c.bn, s};
     }
   }
   return best;
@@ -859,16 +861,18 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
   float* part = reinterpret_cast<float*>(xs + align256(scale_bytes(M, K)));
   quantize(X, ldx, M, K, DT, codes, K, reinterpret_cast<uint32_t*>(xs), s);
   const Plan p = plan_for(M, N, K);
-  Operands P{codes, W, xs, ws, K, ldw, M, N, nk, (int)((M + p.tile - 1) / p.tile), 0};
-  P.ntiles = P.tiles_m * (int)((N + p.tile - 1) / p.tile);
+  Operands P{codes, W, xs, ws, K, ldw, M, N, nk, (int)((M + p.bm - 1) / p.bm), 0};
+  P.ntiles = P.tiles_m * (int)((N + p.bn - 1) / p.bn);
   const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
   float* out = p.splits > 1 ? part : nullptr;
-  if (p.tile == 64)
+  if (p.bm == 64)
     gemm_e4m3_tile_kernel<DT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, C, ldc, R, ldr, vec, out);
-  else if (p.tile == 256 && out)
+  else if (p.bn == 256 && out)
     gemm_e4m3_long_kernel<DT, true><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
-  else if (p.tile == 256)
+  else if (p.bn == 256)
     gemm_e4m3_long_kernel<DT, false><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, nullptr);
+  else if (p.bm == 256)
+    gemm_e4m3_tile_kernel<DT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
   else
     gemm_e4m3_tile_kernel<DT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, C, ldc, R, ldr, vec, out);
   if (p.splits > 1) {

@@ -187,7 +187,7 @@ def test_an_mlp_of_8_bit_projections():
 
 # tiles of 256 whole and cut off, with and without a split of K, and what the smaller tiles take of large calls
 @pytest.mark.parametrize("m,n,k", [(700, 4096, 14336), (2050, 2048, 8192), (4097, 1100, 640), (1100, 9000, 256), (2300, 3001, 384),
-                                   (512, 6144, 4096)])
+                                   (512, 6144, 4096), (448, 16384, 1024), (300, 16301, 640)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_large_calls(dtype, m, n, k):
     g = torch.Generator(device=DEV).manual_seed(m)
