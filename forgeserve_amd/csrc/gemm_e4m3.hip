@@ -506,21 +506,26 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
 // operand reads and 64 KB of copies, and all three have to overlap. Waves w and w + 4 share a SIMD; waves 4..7 run half a
 // phase behind waves 0..3, so that one multiplies while the other reads and copies. A phase is one 64 x 64 half of the
 // wave's tile: its first half reads the operands (in a stage's first phase the W's for both) and issues copies, its
-// second, behind a barrier, multiplies. Two stages live in LDS. In halves from a stage's start (the second group one
-// later): W and X0 (rows 0-63 of each group of 128) are read in half 0, X1 in half 2; the copies that take their places,
-// two stages on, are issued in halves 2 and 4 and are read six halves later; a wave waits at the end of each first half
-// until only its eight youngest copies are on their way, one barrier at least before anyone reads the others.
-//   phase of stage kt     reads        copies                     waits for its copies of
-//   0                     W, X0        X1 of kt + 1               X1 of kt
-//   1                     X1           W and X0 of kt + 2         W and X0 of kt + 1
-// The scale words of four stages (2 KB) are one more copy per wave, issued four stages before they are read and counted
-// in that stage's waits; a lane keeps its six words in registers and each stage's instructions pick their byte.
+// second, behind a barrier, multiplies. Two stages live in LDS. In halves from a stage's start (in brackets the second
+// group, one later):
+//   phase of stage kt     reads        they are back   copies                     waits for its copies of
+//   0: halves 0, 1 (1, 2) W, X0        in half 0 (1)   X1 of kt + 1               X1 of kt
+//   1: halves 2, 3 (3, 4) X1           in half 2 (3)   W and X0 of kt + 2         W and X0 of kt + 1
+// (X0: rows 0-63 of each group of 128.) Both orders of a place in LDS hold by the barriers that end the first halves:
+//  - what a copy overwrites has been read. A wave waits for its own reads before that barrier, so W and X0 of kt are in
+//    every wave's registers behind the one that ends half 1, and X1 behind the one that ends half 3; the copies into
+//    their places are issued in halves 2 (3) and, by the next stage's first phase, 4 (5).
+//  - what is read has landed. A wave waits there too, until only its eight youngest copies are on their way: for W and
+//    X0 of kt + 1 in half 2 (3), read in half 4 (5); for X1 of kt in half 0 (1), read in half 2 (3).
+// The scale words of four stages (2 KB) are one more copy per wave, issued four stages before they are read, into the
+// place of words that were read four stages earlier, and counted in that stage's waits; a lane keeps its six words in
+// registers and each stage's instructions pick their byte.
 //
 // Measured, 8005 x 28672 x 4096 with the rows' encoding (21 us): 1,230 us in 128 x 128 tiles, 999 in four phases of 64 x 32
 // quadrants a stage (the order of the 16-bit kernel, on 32 x 32 products: on 16 x 16 ones the compiler moves the sums from
-// register to register and spills), 762-822 in two (2.3-2.5 PFLOP/s, one box and another). Without the copies the loop
-// would take 675, without the operand reads 640, with neither 597, all tiles the same one (copies from L2 alone) 700: the
-// copies' way from L2 is what is left, some 10 TB/s over the chip.
+// register to register and spills), 803 in two (2.40 PFLOP/s). With the copies issued one half later in place of the wait
+// for the reads 830. What bounds it: with the reads not yet waited for (795-825), the loop without its copies took 675,
+// without the operand reads 640, with neither 597, all tiles the same one (copies from L2 alone) 700.
 template <int DT, bool PARTIAL>
 __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint16_t* __restrict__ C, int64_t ldc,
                                                                 const uint16_t* __restrict__ R, int64_t ldr, bool vec,
@@ -618,8 +623,10 @@ __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, uint
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  // one phase's second half: 8 products, each as its operands arrive
+  // the end of a phase's first half, its reads back, and the second half: 8 products
   auto mul = [&](auto byte, int q) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     barrier();
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
