@@ -78,6 +78,7 @@ SIGNATURES = {
     "fs_gemm_e4m3": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_i64, c_i32, c_p, c_i64,
                              c_p]),
     "fs_gemm_e4m3_workspace_size": (c_i64, [c_i64, c_i64, c_i64]),
+    "fs_gemm_e4m3_plan": (c_i32, [c_i64, c_i64, c_i64, c_p]),
     "fs_gemm_serial": (c_i32, [c_i64, c_i64, c_i64, c_i32]),
     "fs_gemm_partials": (c_i32, [c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_i64, c_i32, c_p, c_i64, c_p]),
     "fs_splitk_add_rmsnorm": (c_i32, [c_p, c_i32, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_i64, c_i64, c_f32, c_i32,

@@ -819,8 +819,14 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // codes and round of workgroups, where the other way's two more launches cost 4.5 us: 16 x 4096 x 4096 12.0 us against
 // 14.3, 8 x 2048 x 8192 13.5 against 14.9, 8 x 4096 x 14336 22.8 against 18.8; in two rounds 4 x 28672 x 4096 32.7 against
 // 31.2, 1 x 31.1.
+bool short_size(int64_t M, int64_t N, int64_t K) { return M <= SHORT_ROWS && M * K <= (N <= 16384 ? SHORT_BYTES : 8 * 1024); }
 bool short_call(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx) {
-  return M <= SHORT_ROWS && M * K <= (N <= 16384 ? SHORT_BYTES : 8 * 1024) && al16(X) && ldx % 8 == 0;
+  return short_size(M, N, K) && al16(X) && ldx % 8 == 0;
+}
+// So many 16-column tiles a workgroup of it that the grid is one round of the CUs where it can be.
+int short_tiles(int64_t N) {
+  const int64_t tiles = (N + 15) / 16;
+  return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4;
 }
 
 void quantize(const void* X, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, uint8_t* codes, int64_t ldc, uint32_t* scales,
@@ -846,8 +852,8 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
   const bool vec = rows_by_8(C, ldc, R, ldr);
   const int nk = (int)(K / GROUP);
   if (short_call(M, N, K, X, ldx)) {
-    // so many columns a workgroup that the grid is one round of the CUs where it can be
     const int64_t tiles = (N + 15) / 16;
+    const int tn = short_tiles(N);
 #define FS_SHORT_XB(TN, DEPTH, XB)                                                                                     \
   gemm_e4m3_short_kernel<DT, TN, DEPTH, XB><<<dim3((unsigned)((tiles + TN - 1) / TN)), 512, 0, s>>>(X, ldx, W, ldw, ws, C, ldc, \
                                                                                                     R, ldr, (int)M, N, nk, vec)
@@ -856,8 +862,8 @@ int gemm(const uint16_t* X, int64_t ldx, const uint8_t* W, int64_t ldw, const ui
     if (M * K <= 32 * 1024) FS_SHORT_XB(TN, DEPTH, 32 * 1024);        \
     else FS_SHORT_XB(TN, DEPTH, SHORT_BYTES);                        \
   } while (0)
-    if (tiles <= 256) FS_SHORT(1, 7);
-    else if (tiles <= 512) FS_SHORT(2, 4);
+    if (tn == 1) FS_SHORT(1, 7);
+    else if (tn == 2) FS_SHORT(2, 4);
     else FS_SHORT(4, 2);
 #undef FS_SHORT_XB
 #undef FS_SHORT
@@ -909,6 +915,17 @@ extern "C" int64_t fs_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K) 
   if (M <= 0 || N <= 0 || K <= 0 || K % GROUP) return 0;
   const Plan p = plan_for(M, N, K);
   return align256(M * K) + align256(scale_bytes(M, K)) + (p.splits > 1 ? (int64_t)p.splits * M * N * (int64_t)sizeof(float) : 0);
+}
+
+extern "C" int fs_gemm_e4m3_plan(int64_t M, int64_t N, int64_t K, int32_t* plan) {
+  FS_CHECK_ARG(plan && M > 0 && N > 0 && K > 0 && K % GROUP == 0, "gemm_e4m3_plan: M %lld N %lld K %lld (K a multiple of %d)",
+               (long long)M, (long long)N, (long long)K, GROUP);
+  Plan p = plan_for(M, N, K);
+  if (short_size(M, N, K)) p = Plan{SHORT_ROWS, 16 * short_tiles(N), 1};
+  plan[0] = p.bm;
+  plan[1] = p.bn;
+  plan[2] = p.splits;
+  return 0;
 }
 
 extern "C" int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* w_scales, void* C, int64_t ldc,

@@ -297,6 +297,11 @@ int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t ldw, const v
                  int64_t workspace_bytes, void* stream);
 int64_t fs_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
 
+/* How fs_gemm_e4m3 computes a product of this shape: the rows and columns of a workgroup's tile and the K splits, into
+ * plan[0..2]. {16, 16 .. 64, 1} is the one launch of short calls, for rows in aligned 16-byte pieces; others take tiles
+ * there too. Internal tuning, no counterpart in the reference. */
+int fs_gemm_e4m3_plan(int64_t M, int64_t N, int64_t K, int32_t* plan);
+
 /* One decoder block of fs_run_blocks: its weights (contiguous rows, the dtype of the run; w_qkv holds wq, wk and
  * wv one below the other, w_gate_up the gate then the up projection), the norm after the attention, the
  * norm that the block's output goes through next (NULL: none; the last block only), its cache layer with
