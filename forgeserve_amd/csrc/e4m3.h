@@ -1,9 +1,10 @@
 // 8-bit floating point (e4m3: 4 exponent and 3 mantissa bits, OCP, largest value 448) with a power of two as the
 // scale of a group of values, kept as its biased exponent byte e: a code c stands for value(c) * 2^(e - 127).
 //
-// A power of two loses nothing against any other scale: it moves no mantissa bit, so a value's rounding is within
-// half a step, 2^-4 of it, wherever the code is normal (down to 2^-15 of the group's largest), and both the encoding
-// x * 2^(127 - e) and the decoding are exact but for that one rounding. It is also what the hardware takes: the
+// A power of two moves no mantissa bit: both the encoding x * 2^(127 - e) and the decoding are exact but for one rounding,
+// which is within half a step: 2^-4 of the value where the code is normal, from 2^-6 of the scale s on, and 2^-10 s below
+// that. The group's largest is above 224 s (unless s is the smallest there is), so these are at most 2^-13.8 and 2^-17.8
+// of it; another scale would put it at 448 s and gain a factor of two there. It is also what the hardware takes: the
 // conversions to bf16 and f16 and the matrix instructions apply such a scale by themselves.
 #pragma once
 

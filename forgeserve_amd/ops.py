@@ -149,7 +149,9 @@ def quantize_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x (rows, K) (float32, bfloat16, float16; K a multiple of 128) in 8-bit floating point: (codes, torch.float8_e4m3fn
     (rows, K); scales, uint8 (ceil(K / 512), rows, 4)). Columns 128g .. of row r stand for
     codes * 2^(scales[g // 4, r, g % 4] - 127): the smallest power of two that brings the group's largest magnitude to
-    448 or less, so a value is kept within 2^-4 of it (2^-19 of the group's largest, if it is below 2^-15 of that).
+    448 or less. A value is kept within 2^-4 of it down to 2^-6 of the scale (at most 2^-13.8 of the group's largest), and
+    within 2^-10 of the scale (2^-17.8 of the largest) below that; where the scale is the smallest there is, 2^-117, a
+    share of the scale only.
     What is not finite becomes NaN."""
     require_device(x)
     _check_current("quantize_e4m3", x)

@@ -20,8 +20,9 @@ every result are the same.
 pool: e4m3 codes with a power of two per token, KV head and side as their scale. Rows are encoded as they are
 written and decoded by whatever reads them, so everything that takes a pool's views takes these. `pool.k[layer]`,
 `pool.v[layer]` and `pool.scales[layer]` are then the codes and exponent bytes as `ops.kv_layout_e4m3` describes
-them; `ops.paged_gather` gives their values. A value is stored within half a step of e4m3, 2^-4 of it (of values
-below 2^-15 of their group's largest, 2^-19 of that).
+them; `ops.paged_gather` gives their values. A value is stored within half a step of e4m3: 2^-4 of it, down to 2^-6
+of its group's scale (at most 2^-13.8 of the group's largest value), and 2^-10 of the scale (2^-17.8 of the largest)
+below that. Scales are at least 2^-117 (float16 rows: 2^-15, under which float16's own smallest steps are kept exactly).
 
 The block allocator and the block tables stay on the host, as in the reference; tables are copied
 to the GPU (int32) once per step and shared by every layer's view.

@@ -209,3 +209,29 @@ def test_tensors_of_another_device_than_the_current_are_refused(monkeypatch):
         ops._check_current("gemm_e4m3", Elsewhere())
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
     ops._check_current("gemm_e4m3", Elsewhere())
+
+
+@pytest.mark.parametrize("limits", [(10, 246), (112, 134)])
+def test_how_far_a_code_is_from_its_value(limits):
+    """Half a step: 2^-4 of the value from 2^-6 of the scale on, 2^-10 of the scale below. A group's largest may be as low
+    as 224 scales, which puts these at 2^-13.8 and 2^-17.8 of it, and not lower."""
+    g = torch.Generator().manual_seed(22)
+    tops = torch.tensor([224.0000001, 225.0, 300.0, 448.0], dtype=torch.float64)
+    x = torch.exp2(-22 * torch.rand(4, 200000, generator=g, dtype=torch.float64)) * tops[:, None]
+    x[:, 0] = tops
+    c, e = ref.encode(x, limits)
+    assert (e == 127).all()   # the scale is 1
+    err, top = (ref.decode(c, e) - x).abs(), tops[:, None]
+    normal = x >= 2.0 ** -6
+    assert (err <= 2.0 ** -4 * x)[normal].all() and (err <= 2.0 ** -10)[~normal].all()
+    assert (err <= 2.0 ** -4 * x)[x >= 2.0 ** -13.8 * top].all() and (err <= 2.0 ** -17.8 * top)[x < 2.0 ** -13.8 * top].all()
+    # a bound that took the largest for 448 scales would be too small for the first two groups
+    low = x < 2.0 ** -14.5 * top
+    assert (err > 2.0 ** -18.5 * top)[:2][low[:2]].any() and (err > 2.0 ** -4 * x)[:2][(x >= 2.0 ** -14.5 * top)[:2]].any()
+
+
+def test_the_smallest_float16_values_are_kept_exactly():
+    """float16's scale is at least 2^-15: below 2^-21 the codes are its own smallest steps of 2^-24."""
+    x = torch.arange(8, dtype=torch.float64) * 2.0 ** -24
+    c, e = ref.encode(x, ref.LIMITS[torch.float16])
+    assert int(e) == 112 and torch.equal(ref.decode(c, e), x)
