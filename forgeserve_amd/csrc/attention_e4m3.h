@@ -98,6 +98,12 @@ FS_DEVICE void tile_scores_e4m3(const u32x4 (&kf)[D / 32], const u32x4 (&qf)[2][
   }
 }
 
+// f16 holds p times 2^7 (as do l and the sums, of every partial, so that it leaves the quotient): the largest, 2^REF_SLACK
+// of it, still fits, and eleven bits are kept down to 2^-21 of the reference, within 2^-32 of it below, where p as it is
+// would have lost them below 2^-14 and been nothing below 2^-25. (bf16: p times the value's scale, at least 2^-117, is
+// below a normal number only for values of 1e-30 and less.)
+template <int DT> constexpr float P_LOG2 = DT == FS_F16 ? 7.f : 0.f;
+
 // pair_probs with a value's scale in its probability (bf16). A score that is NaN moves no reference; its p, l and
 // sums are NaN (and partial_reference keeps such a partial from counting as empty).
 template <int DT, bool TWO, class Scales>
@@ -129,7 +135,7 @@ FS_DEVICE bool pair_probs_e4m3(const float (&sc)[2][2][4], Scales scales, float 
   }
   float ref[2], sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) ref[nt] = m_run[nt] == -INFINITY ? 0.f : m_run[nt];   // (a row that has seen nothing yet: every p is 0)
+  for (int nt = 0; nt < NT; ++nt) ref[nt] = (m_run[nt] == -INFINITY ? 0.f : m_run[nt]) - P_LOG2<DT>;   // (a row that has seen nothing yet: every p is 0)
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     float vs[4];

@@ -674,3 +674,27 @@ def test_engine_and_speculation_over_the_pool(graphs):
     assert plain == engine(draft=draft, k=3, graphs=graphs) == engine(draft=draft, k=3, graphs=graphs, share_kv=False)
     sb = fa.SpeculativeBatch(model, draft, 60, k=3, graphs=graphs, cache_dtype=E4M3)
     assert sb.pool_t.cache_dtype == E4M3
+
+
+@pytest.mark.parametrize("dtype,hd,T", [(F16, 64, 1), (F16, 128, 7), (F16, 64, 60), (BF16, 64, 1), (BF16, 128, 60)])
+@pytest.mark.parametrize("n", [100, 700, 9000])
+def test_keys_far_below_the_largest(dtype, hd, T, n):
+    """Many keys whose probabilities are 2^-25.3 of one key's: their share counts in full where that key's value is 0."""
+    pool = make_pool(hd, 1, 16, -(-n // 16), dtype, heads=2)
+    rows = torch.zeros(2, pool.num_blocks * 16, hd, dtype=torch.float64)
+    rows[0, 0, 0], rows[1, 1:] = 8.0, 1.0
+    rows[1, 1:, 5] = 3.0
+    coded = [ref.encode(x, ref.LIMITS[dtype]) for x in rows]
+    kc, vc = (c.view(pool.num_blocks, 1, 16, hd) for c, _ in coded)
+    k, v = ref.tiles_of(kc, vc)
+    pool.k[0].view(torch.uint8).copy_(k)
+    pool.v[0].view(torch.uint8).copy_(v)
+    pool.scales[0].copy_(torch.stack([e.view(-1, 1, 16) for _, e in coded], 2))
+    q = torch.zeros(1, T, 2, hd, dtype=dtype)
+    q[..., 0] = 2.0
+    scale = 25.3 * math.log(2) / 16
+    pos = torch.arange(n - T, n).int()[None]
+    table = torch.arange(pool.num_blocks, dtype=torch.int32)[None]
+    out = ops.paged_attention(q.to(DEV), pool.layout(0), table.to(DEV), pos.to(DEV), scale)
+    want, mag = ref.attention(q[0], rows[0, None], rows[1, None], pos[0], scale)
+    check_attention(out[0].cpu(), want, mag, dtype)
