@@ -1973,7 +1973,7 @@ int paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, con
       const unsigned pgrid = grid * (unsigned)parts, pthreads = 64 * UNIT_WAVES / (unsigned)parts;
 #define FS_ATTN_LAUNCH(ST_, D_, BS_, TWO_)                                                     \
   do {                                                                                         \
-    if (ST_ == FS_BF16 && parts == 4) attn_unit_part_kernel<FS_BF16, D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
+    if ((ST_) == FS_BF16 && parts == 4) attn_unit_part_kernel<FS_BF16, D_, BS_, TWO_, 4><<<pgrid, pthreads, 0, st>>>(P); \
     else if (parts == 2) attn_unit_part_kernel<ST_, D_, BS_, TWO_, 2><<<pgrid, pthreads, 0, st>>>(P); \
     else attn_unit_kernel<ST_, D_, BS_, TWO_><<<grid, 64 * UNIT_WAVES, 0, st>>>(P);              \
   } while (0)
