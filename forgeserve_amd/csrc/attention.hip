@@ -1775,7 +1775,8 @@ int attn_split() {
 constexpr int E4M3_SPLIT = 8192;
 int e4m3_split() { return attn_split() < E4M3_SPLIT ? attn_split() : E4M3_SPLIT; }
 
-constexpr int PLANLESS_KEYS = 2048;   // table lengths up to which a call over codes may go without a plan
+// Table lengths (not rows': a wider table costs the same rows a plan) up to which a call over codes may go without one.
+constexpr int PLANLESS_KEYS = 2048;
 
 int64_t nsplit_for(int32_t max_blocks, int32_t block_size, int split) {
   const int64_t S = (int64_t)max_blocks * block_size;

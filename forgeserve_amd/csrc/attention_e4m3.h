@@ -5,7 +5,9 @@
 // operands in registers. Both conversions are exact: a key's scale is applied by the conversion itself; a value's, which
 // differs from key to key within an operand, goes into the probabilities (bf16: p is rounded once, after the exact
 // product with the power of two) or multiplies the operand (f16, whose range p times a scale would leave). So the only
-// roundings are those of a 16-bit pool's attention (p and the output) and the sums', in f32; l sums p unrounded.
+// roundings are p's to 16 bits, which the product of 16-bit operands needs and the bf16 pool's attention has too (the f16
+// pool's scalar kernel keeps p in f32: f16 rows give up that much for the matrix cores, 2.1e-4 -> 2.3e-4 of the output's
+// norm), the output's, and the sums', in f32; l sums p unrounded.
 //
 // The tiles are stored so that a wave's loads are whole: 16 bytes a lane are dims 16c .. 16c+15 of a key (lane l16 = key,
 // c = g, g + 4), which makes k-step 2j + h of the product dims 16 (g + 4j) + 8h .. +7 of lane group g, for the keys as

@@ -111,12 +111,12 @@ FS_DEVICE void pair_step_clean(const float4_t (&sc)[2][2], Value value, bool nan
 // pair's values of dims 16 mt .. are 1 KB each, lane after lane. Two stages of codes are on their way while one is
 // multiplied; the one buffer of operands costs a second barrier a stage.
 //
-// Bound by vector instructions and by what they and the products wait for: 59% of the SIMDs' time and 25% of the matrix
-// cores', at two waves per SIMD (238 registers at 128 dims). Measured (us): prompts of 4096, 2811, 2196 and 1829 tokens,
-// 32/8 heads of 128: 450, 600 TFLOP/s; of 4096, 3771, 2631 and 850: 538, where the 16-bit pool's kernel takes 515; of 64
-// dims and 4096, 3586, 3428 and 558: 377 and 337. Raising the waves' priority in their products, keys read a tile ahead,
-// values read before the softmax: each within 1%. Stages of 4 tiles with two buffers of operands, so that one stage is
-// converted beside the products of another behind one barrier: 575 and 425.
+// No unit is full: vector instructions take 58% of the SIMDs' time, products 26% of the matrix cores', and a wave waits for
+// 36% of its own, at two waves per SIMD (238 registers at 128 dims). Measured (us): prompts of 4096, 2811, 2196 and 1829
+// tokens, 32/8 heads of 128: 442 (610 TFLOP/s), f16 447, where the 16-bit pool's kernel, which converts nothing, takes
+// 410; of 64 dims: 322, 317 and 283. Raising the waves' priority in their products, keys read a tile ahead, values read
+// before the softmax: each within 1%. Stages of 4 tiles with two buffers of operands, so that one stage is converted
+// beside the products of another behind one barrier: 7% more at 128 dims, 13% at 64.
 template <int DT, int D, int BSZ>
 __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 attn_prefill_e4m3_kernel(AttnParams P) {

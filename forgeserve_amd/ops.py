@@ -3,6 +3,9 @@
 Each function checks shapes on the host, allocates outputs and workspace with torch's caching
 allocator, and launches on torch's current stream. Inputs must already be on the GPU; nothing here
 computes on the CPU.
+
+gemm, paged_attention and the acceptance keep one scratch buffer per device from call to call: their calls on several
+streams at once are for the caller to order. gemm_e4m3 and the sampling calls take scratch of their own each time.
 """
 
 import math
@@ -31,8 +34,8 @@ _RETIRED = []   # outgrown scratch buffers: a captured HIP graph may still hold 
 
 
 def _persistent_ws(name: str, nbytes: int, device) -> torch.Tensor:
-    """A per-device scratch buffer reused across calls (calls are ordered on torch's current stream,
-    so consecutive users never overlap); grown when a call needs more. An outgrown buffer is kept
+    """A per-device scratch buffer reused across calls (calls on one stream are ordered, so consecutive
+    users never overlap); grown when a call needs more. An outgrown buffer is kept
     alive for the life of the process, since graphs captured earlier launch kernels on it."""
     key = (name, torch.device(device))
     ws = _PERSISTENT.get(key)
@@ -171,7 +174,8 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out = a @ w.T (+ residual) with the weight in 8-bit floating point, as quantize_e4m3 leaves it (w (n, k) codes with
     16-byte aligned rows, w_scales (ceil(k / 512), n, 4)), and a (bfloat16 or float16) brought to the same form within
-    the call: nn.Linear with half the weight bytes and twice the matrix rate of gemm's. Sums are float32 (of each eight
+    the call: nn.Linear with half the weight bytes and twice the matrix rate of gemm's (17 to 64 rows of a small weight gain
+    little: three launches). Sums are float32 (of each eight
     products the matrix instruction drops what lies more than 13 binary places below the largest); product and residual
     are rounded once, to a's dtype. A row's last bit may depend on how many rows the call has. out may be the
     residual itself, but shares no memory with a or w."""

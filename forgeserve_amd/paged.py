@@ -23,6 +23,9 @@ written and decoded by whatever reads them, so everything that takes a pool's vi
 them; `ops.paged_gather` gives their values. A value is stored within half a step of e4m3: 2^-4 of it, down to 2^-6
 of its group's scale (at most 2^-13.8 of the group's largest value), and 2^-10 of the scale (2^-17.8 of the largest)
 below that. Scales are at least 2^-117 (float16 rows: 2^-15, under which float16's own smallest steps are kept exactly).
+It is for decoding: one token's or a window's attention reads half the bytes (64 rows of long contexts, 0.6 of the time),
+while a prompt's, bound by arithmetic, takes 8-14% longer than over a bfloat16 pool. Attention rounds probabilities to 16
+bits, as over a bfloat16 pool; over a float16 pool they stay in float32.
 
 The block allocator and the block tables stay on the host, as in the reference; tables are copied
 to the GPU (int32) once per step and shared by every layer's view.
