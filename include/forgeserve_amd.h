@@ -154,8 +154,8 @@ int fs_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
  * several prompts at once. workspace: fs_paged_attention_workspace_size(S, T, ...). */
 /* Keys per chunk of the MFMA attention path (FS_ATTN_SPLIT, default 16384), fixed for the life of the
  * process: a query at position p reads chunks 0 .. p / split and, past the first, its output is merged
- * from per-chunk partials. Over e4m3 codes a chunk is 8192 keys, or this if it is smaller. No counterpart in the reference (it gathers every key); for callers and
- * benchmarks that report how a workload is split. */
+ * from per-chunk partials. Over e4m3 codes a chunk is 8192 keys, or this if it is smaller. No counterpart in the
+ * reference (it gathers every key); for callers and benchmarks that report how a workload is split. */
 int32_t fs_paged_attention_split(void);
 
 int fs_paged_attention_varlen(const void* q, int64_t q_st, int64_t q_sh, const fs_kv_layout* kv,
@@ -327,7 +327,8 @@ typedef struct fs_block {
  * x_out the stream behind the last block, y_out its next_norm (unused when that is NULL). Every step is the
  * entry point that computes it alone, chosen as a caller would (partials into the norm and rotary
  * kernels where the projection splits K), with the same results (model.py:99-106, 136). All blocks have
- * blocks[0]'s n_kv_heads and head_dim. The three buffers (256-byte aligned) hold the bytes that
+ * blocks[0]'s n_kv_heads and head_dim; dtype is their caches' kv.dtype, FS_STORE_E4M3 included, in both calls (rows and
+ * weights have it without the flag). The three buffers (256-byte aligned) hold the bytes that
  * fs_run_blocks_workspace gives for the largest max_blocks: bytes[0] gemm_ws, bytes[1] attn_ws,
  * bytes[2] scratch. */
 int fs_run_blocks_workspace(int32_t B, int32_t T, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
