@@ -31,6 +31,16 @@ class KVLayout(ctypes.Structure):
     ]
 
 
+class Linear(ctypes.Structure):
+    """fs_linear: a projection over codes."""
+
+    _fields_ = [
+        *[(name, c_p) for name in ("x", "x_scales", "w", "w_scales", "bias", "residual", "out", "out_scales")],
+        *[(name, c_i64) for name in ("ldx", "ldw", "ldr", "ldo", "m", "n", "k")],
+        *[(name, c_i32) for name in ("x_dtype", "dtype", "bias_dtype", "activation", "gated", "reserved")],
+    ]
+
+
 class Block(ctypes.Structure):
     """fs_block: one decoder block of fs_run_blocks."""
 
@@ -78,6 +88,12 @@ SIGNATURES = {
     "fs_gemm_e4m3": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_i64, c_i32, c_p, c_i64,
                              c_p]),
     "fs_gemm_e4m3_workspace_size": (c_i64, [c_i64, c_i64, c_i64]),
+    "fs_dequantize_e4m3": (c_i32, [c_p, c_i64, c_p, c_i64, c_i64, c_i32, c_p, c_i64, c_p]),
+    "fs_add_rmsnorm_e4m3": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_f32, c_i32,
+                                    c_p]),
+    "fs_linear_e4m3": (c_i32, [ctypes.POINTER(Linear), c_p, c_i64, c_p]),
+    "fs_linear_e4m3_workspace_size": (c_i64, [ctypes.POINTER(Linear)]),
+    "fs_linear_e4m3_plan": (c_i32, [ctypes.POINTER(Linear), c_p]),
     "fs_gemm_e4m3_plan": (c_i32, [c_i64, c_i64, c_i64, c_p]),
     "fs_gemm_serial": (c_i32, [c_i64, c_i64, c_i64, c_i32]),
     "fs_gemm_partials": (c_i32, [c_p, c_i64, c_p, c_i64, c_i64, c_i64, c_i64, c_i32, c_p, c_i64, c_p]),

@@ -28,8 +28,8 @@ FLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
 
-SOURCES = ["abi.hip", "kv.hip", "kv_e4m3.hip", "attention.hip", "norm.hip", "gemm.hip", "gemm_f32.hip", "gemm_e4m3.hip", "sample.hip", "rng.hip",
-           "blocks.hip"]
+SOURCES = ["abi.hip", "kv.hip", "kv_e4m3.hip", "attention.hip", "norm.hip", "gemm.hip", "gemm_f32.hip", "gemm_e4m3.hip", "linear_e4m3.hip",
+           "norm_e4m3.hip", "sample.hip", "rng.hip", "blocks.hip"]
 
 
 def _run(cmd):

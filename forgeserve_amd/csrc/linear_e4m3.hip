@@ -1,0 +1,452 @@
+// Projections over codes with what follows them in one call: with z = x w^T + b,
+//
+//   y = act(z) + R, or with a gate (W and b hold the gate's F rows, then the others')  y = act(z_gate) * z_up + R
+//
+// x and w in e4m3 codes (rows_e4m3.h; 16-bit or 32-bit rows of x are encoded first), the sums as gemm_e4m3.hip's, everything
+// behind them in f32 and rounded once: to 16-bit rows, or to codes with a scale for each 128 columns, which is what the next
+// product reads. The products are gemm_e4m3.h's kernels; where a tile holds what its results need (a gate's column beside its
+// other's: the tile's columns are drawn from both halves of W; for codes whole groups of 128 columns), the workgroup finishes
+// them from LDS, else the sums go through memory and a second kernel finishes them.
+#include "gemm_e4m3.h"
+
+namespace {
+
+constexpr int SHORT_ROWS = 16;   // rows that the kernel without tiles takes
+
+// ------------------------------------------------------------------------------------------------
+// what is done with the sums
+// ------------------------------------------------------------------------------------------------
+// z / (1 + e^-y). The factor 2^-6 keeps the reciprocal a normal number up to e^-y = 2^128, where z's share of the result is
+// less than 2^-120; the hardware's exponential and reciprocal are within two f32 steps, and y's rounding times log2(e)
+// adds |y| 2^-24: nothing against 16 bits.
+FS_DEVICE float over_one_plus_exp(float z, float y) {
+  const float e = __builtin_amdgcn_exp2f(y * -1.4426950408889634f);
+  return (z * 0x1p-6f) * __builtin_amdgcn_rcpf(fmaf(e, 0x1p-6f, 0x1p-6f));
+}
+// z Phi(z) with Phi(-a) = erfc(a / sqrt 2) / 2 = e^(-a^2 / 2) t Q(t) / 2, t = 1 / (1 + 0.4 a / sqrt 2): Q, of degree 6, is
+// the polynomial whose largest relative error over 0 <= a <= 19.8 is least (3.5e-6, fitted to scipy's erfcx). The result is
+// within 8e-6 of itself in both tails, a thirtieth of f16's rounding.
+FS_DEVICE float gelu_erf(float z) {
+  const float a = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(a, 0.282842712f, 1.f));
+  float q = -0.0880692603f;
+  q = fmaf(q, t, 0.161608521f);
+  q = fmaf(q, t, 0.102756314f);
+  q = fmaf(q, t, 0.158245978f);
+  q = fmaf(q, t, 0.215523985f);
+  q = fmaf(q, t, 0.224155506f);
+  q = fmaf(q, t, 0.225775499f);
+  const float phi = 0.5f * t * q * __builtin_amdgcn_exp2f(a * a * -0.72134752f);   // Phi(-a)
+  return z * (z < 0.f ? phi : 1.f - phi);
+}
+
+template <int DT_, bool GATED_, bool CODES_>
+struct LinearOut {
+  static constexpr int DT = DT_;
+  static constexpr bool GATED = GATED_, CODES = CODES_, STAGED = true;
+  uint16_t* C;            // rows, or codes
+  int64_t ldc;            // in elements
+  const uint16_t* R;
+  int64_t ldr;
+  const void* bias;
+  int64_t up;             // where the others' bias begins
+  int32_t bias_dtype, act;
+  bool vec, bias_vec;     // eight columns of C and R at a time; of the bias
+  uint8_t* scales;        // of codes
+  int64_t rows;
+  float* part;
+
+  template <int NC>
+  FS_DEVICE void add_bias(float (&v)[NC], int64_t at, int64_t left) const {
+    if (bias_vec && left >= NC) {
+      if (bias_dtype == FS_F32) {
+#pragma unroll
+        for (int h = 0; h < NC / 4; ++h) {
+          const float4_t b = *reinterpret_cast<const float4_t*>(static_cast<const float*>(bias) + at + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] += b[e];
+        }
+        return;
+      }
+#pragma unroll
+      for (int h = 0; h < NC / 4; ++h) {
+        const u32x2_t b = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(bias) + at + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[4 * h + e] += bias_dtype == FS_BF16 ? half_of<FS_BF16>(b[e >> 1], e & 1) : half_of<FS_F16>(b[e >> 1], e & 1);
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < NC; ++e) {
+      if (e >= left) break;
+      if (bias_dtype == FS_F32) v[e] += static_cast<const float*>(bias)[at + e];
+      else if (bias_dtype == FS_BF16) v[e] += bf16_to_f32(static_cast<const uint16_t*>(bias)[at + e]);
+      else v[e] += f16_to_f32(static_cast<const uint16_t*>(bias)[at + e]);
+    }
+  }
+  // NC columns' sums from col on, of `cols`, to what is rounded
+  template <int NC>
+  FS_DEVICE void compute(float (&v)[NC], float (&u)[NC], int64_t row, int64_t col, int64_t cols) const {
+    if (bias) {
+      add_bias(v, col, cols - col);
+      if (GATED) add_bias(u, up + col, cols - col);
+    }
+    switch (act) {
+      case FS_ACT_RELU:
+#pragma unroll
+        for (int e = 0; e < NC; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+        break;
+      case FS_ACT_SILU:
+#pragma unroll
+        for (int e = 0; e < NC; ++e) v[e] = over_one_plus_exp(v[e], v[e]);
+        break;
+      case FS_ACT_GELU:
+#pragma unroll
+        for (int e = 0; e < NC; ++e) v[e] = gelu_erf(v[e]);
+        break;
+      case FS_ACT_GELU_TANH:   // (1 + tanh y) / 2 = 1 / (1 + e^-2y), y = sqrt(2 / pi) (z + 0.044715 z^3)
+#pragma unroll
+        for (int e = 0; e < NC; ++e)
+          v[e] = over_one_plus_exp(v[e], v[e] * fmaf(v[e] * v[e], 0.0713548163f, 1.59576912f));
+        break;
+      default: break;
+    }
+    if (GATED) {
+#pragma unroll
+      for (int e = 0; e < NC; ++e) v[e] *= u[e];
+    }
+    if (!CODES && R) {
+      const uint16_t* r = R + row * ldr + col;
+      if (vec && col + NC <= cols) {
+#pragma unroll
+        for (int h = 0; h < NC / 4; ++h) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(r + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] += half_of<DT>(w[e >> 1], e & 1);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < NC; ++e)
+          if (col + e < cols) v[e] += Elem<DT>::to_f32(r[e]);
+      }
+    }
+  }
+  FS_DEVICE void finish(float4_t& a, int64_t row, int64_t col0, int64_t cols) const {
+    float4_t b = a;
+    finish(a, b, row, col0, cols);
+  }
+  FS_DEVICE void finish(float4_t& a, float4_t b, int64_t row, int64_t col0, int64_t cols) const {
+    float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
+    compute(v, u, row, col0, cols);
+    a = float4_t{v[0], v[1], v[2], v[3]};
+  }
+  // Eight columns' sums finished and stored. For codes 16 lanes side by side hold a row's group (all in range, or none).
+  FS_DEVICE void piece(float (&v)[8], float (&u)[8], int64_t row, int64_t col, int64_t cols) const {
+    compute(v, u, row, col, cols);
+    if constexpr (CODES) {
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_magnitude(v[e]));
+      const int e = scale_exponent<FS_F32>(group_max<16>(m));
+      const float inv = scale_inverse(e);
+      *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(C) + row * ldc + col) =
+          u32x2_t{encode4(v[0], v[1], v[2], v[3], inv), encode4(v[4], v[5], v[6], v[7], inv)};
+      if ((col & (GROUP - 1)) == 0) {
+        const int g = (int)(col / GROUP);
+        uint8_t* word = scales + ((int64_t)(g >> 2) * rows + row) * 4;
+        word[g & 3] = (uint8_t)e;
+        if (col + GROUP >= cols)
+          for (int b = (g & 3) + 1; b < 4; ++b) word[b] = 0;
+      }
+    } else {
+      uint16_t* c = C + row * ldc + col;
+      uint16_t o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = Elem<DT>::store_bits(v[e]);
+      if (vec && col + 8 <= cols) {
+        *reinterpret_cast<u32x4*>(c) = u32x4{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16,
+                                             o[4] | (uint32_t)o[5] << 16, o[6] | (uint32_t)o[7] << 16};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < cols) c[e] = o[e];
+      }
+    }
+  }
+};
+
+// The splits' sums added in order and finished, eight columns of the results a thread (N % 4 == 0: rows of W).
+template <class OUT>
+__global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __restrict__ part, int splits, int64_t M, int64_t N,
+                                                               uint32_t pieces, OUT out) {
+  const int64_t cols = OUT::GATED ? N / 2 : N;
+  const uint32_t unit = blockIdx.x * 256u + threadIdx.x;   // (M * pieces < 2^31)
+  const int64_t row = unit / pieces, col = 8 * (int64_t)(unit % pieces);
+  if (row >= M) return;   // (by groups of 16 lanes where codes are written: pieces % 16 == 0)
+  float v[8], u[8];
+  auto add = [&](float (&to)[8], const float* p, bool set) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (col + 4 * h >= cols) continue;
+      const float4_t a = *reinterpret_cast<const float4_t*>(p + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[4 * h + e] = set ? a[e] : to[4 * h + e] + a[e];
+    }
+  };
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float* p = part + ((int64_t)s * M + row) * N + col;
+    add(v, p, s == 0);
+    if (OUT::GATED) add(u, p + cols, s == 0);
+  }
+  out.piece(v, u, row, col, cols);
+}
+
+// ------------------------------------------------------------------------------------------------
+// up to 16 rows: bound by the weight's bytes
+// ------------------------------------------------------------------------------------------------
+// A workgroup takes 16 TN rows of W; its eight waves split K and are joined in order through LDS. Codes of both operands go
+// straight to registers in the instruction's own shape, DEPTH stages ahead: W's from HBM, x's (16 rows of them at most, the
+// same for every workgroup) from L2.
+template <class OUT, int TN, int DEPTH>
+__global__ void __launch_bounds__(512) linear_e4m3_short_kernel(Operands P, OUT out) {
+  __shared__ float4_t red[8][TN][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * TN);
+  const int k0 = (int)((int64_t)w * P.nk / 8), k1 = (int)((int64_t)(w + 1) * P.nk / 8);
+  const int M = (int)P.M;
+  struct Stage {
+    u32x4 c[TN][2], x[2];
+    uint32_t s[TN], xs;
+  } ring[DEPTH];
+  const int xrow = min(l16, M - 1);   // (lanes past the last row: results nobody stores)
+  const uint8_t* xp = P.x + xrow * P.ldx + 16 * g;
+  const uint8_t* wrow[TN];
+  int64_t srow[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t n = short_row<OUT::GATED>(n0, j, l16, P.N);
+    wrow[j] = P.w + n * P.ldw + 16 * g;
+    srow[j] = 4 * n;
+  }
+  auto load = [&](int k, Stage& x) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      x.c[j][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP));
+      x.c[j][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP + 64));
+      x.s[j] = P.ws[(int64_t)(k >> 2) * 4 * P.N + srow[j] + (k & 3)];
+    }
+    x.x[0] = *reinterpret_cast<const u32x4*>(xp + (int64_t)k * GROUP);
+    x.x[1] = *reinterpret_cast<const u32x4*>(xp + (int64_t)k * GROUP + 64);
+    x.xs = P.xs[((int64_t)(k >> 2) * M + xrow) * 4 + (k & 3)];
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (k0 + d < k1) load(k0 + d, ring[d]);
+  float4_t acc[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int kt = k0; kt < k1; kt += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (kt + d >= k1) break;   // (wave-uniform)
+      const i32x8 xf = both_chunks(ring[d].x[0], ring[d].x[1]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), xf, acc[j], ring[d].s[j], ring[d].xs);
+      if (kt + d + DEPTH < k1) load(kt + d + DEPTH, ring[d]);
+    }
+  }
+  short_results(out, red, acc, w, lane, n0, M, P.N);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+struct Plan {
+  int bm, bn, splits;
+  bool join;   // through memory
+};
+int64_t weight_rows(const fs_linear& c) { return c.gated ? 2 * c.N : c.N; }
+
+// Tiles as gemm_e4m3.hip's rule has them. Codes leave a tile of 256 x 256, or of 128 columns without a gate, by themselves;
+// sums that go through memory are written and read at 4.5 TB/s and cost a launch of 3 us.
+Plan plan_for(const fs_linear& c) {
+  const int64_t M = c.M, N = weight_rows(c), nk = c.K / GROUP;
+  if (M <= SHORT_ROWS) {
+    const int64_t tiles = c.gated ? 2 * ((c.N + 15) / 16) : (N + 15) / 16;
+    const int tn = tiles <= 256 && !c.gated ? 1 : tiles <= 512 ? 2 : 4;
+    return Plan{SHORT_ROWS, 16 * tn, 1, c.out_scales != nullptr};
+  }
+  struct Cand {
+    int bm, bn;
+    double stage, fixed;
+  };
+  static const Cand cands[] = {{64, 64, 0.43, 3.0}, {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0}, {256, 256, 1.5, 10.0}};
+  Plan best{64, 64, 1, c.out_scales != nullptr};
+  double least = 1e30;
+  for (const Cand& t : cands) {
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const bool whole = !c.out_scales || t.bn == 256 || (t.bn == 128 && !c.gated);
+    for (int s = 1; s <= 8; s *= 2) {
+      // (a split starts at a whole word of scales; partials are stored four columns at a time)
+      const bool join = s > 1 || !whole;
+      if (s > 1 && nk % (4 * s) != 0) break;
+      if (join && (N % 4 != 0 || (c.gated && c.N % 4 != 0))) break;
+      const double us = (double)((tiles * s + 255) / 256) * ((double)(nk / s) * t.stage + t.fixed) +
+                        (join ? 3.0 + (double)s * (double)M * (double)N * 8.0 / 4.5e6 : 0.0);
+      if (us < least) least = us, best = Plan{t.bm, t.bn, s, join};
+    }
+  }
+  return best;
+}
+
+int64_t encoded_bytes(const fs_linear& c) { return c.x_scales ? 0 : align256(c.M * c.K) + align256(scale_bytes(c.M, c.K)); }
+int64_t sums_bytes(const fs_linear& c, const Plan& p) {
+  return p.join ? (int64_t)p.splits * c.M * weight_rows(c) * (int64_t)sizeof(float) : 0;
+}
+
+template <class OUT>
+void launch_short(const Operands& P, const OUT& out, int bn, int64_t tiles, hipStream_t s) {
+  const int tn = bn / 16;
+  const dim3 grid((unsigned)((tiles + tn - 1) / tn));
+  if (tn == 4) linear_e4m3_short_kernel<OUT, 4, 2><<<grid, 512, 0, s>>>(P, out);
+  else if (tn == 2) linear_e4m3_short_kernel<OUT, 2, 4><<<grid, 512, 0, s>>>(P, out);
+  else if constexpr (!OUT::GATED) linear_e4m3_short_kernel<OUT, 1, 7><<<grid, 512, 0, s>>>(P, out);
+}
+
+// PARTS: a class of which only the sums in memory are asked for.
+template <class OUT, bool PARTS>
+void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
+  if (p.bn == 256) {
+    gemm_e4m3_long_kernel<OUT, PARTS><<<grid, 512, 0, s>>>(P, out);
+  } else if constexpr (!OUT::CODES || !OUT::GATED) {
+    if (p.bm == 256) gemm_e4m3_tile_kernel<OUT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, out);
+    else if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, out);
+    else if constexpr (!OUT::CODES) gemm_e4m3_tile_kernel<OUT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, out);
+  }
+}
+
+template <class OUT>
+int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t s) {
+  OUT out;
+  out.C = reinterpret_cast<uint16_t*>(c.out);
+  out.ldc = c.ldo;
+  out.R = reinterpret_cast<const uint16_t*>(c.residual);
+  out.ldr = c.ldr;
+  out.bias = c.bias;
+  out.up = c.N;
+  out.bias_dtype = c.bias_dtype;
+  out.act = c.activation;
+  out.vec = al16(c.out) && c.ldo % 8 == 0 && (!c.residual || (al16(c.residual) && c.ldr % 8 == 0));
+  out.bias_vec = al16(c.bias) && (!c.gated || c.N % 8 == 0);
+  out.scales = reinterpret_cast<uint8_t*>(c.out_scales);
+  out.rows = c.M;
+  out.part = nullptr;
+  if (p.join) {
+    typedef LinearOut<FS_BF16, false, false> Sums;   // (its type is of no account)
+    Sums sums{};
+    sums.part = part;
+    if (p.bm == SHORT_ROWS) launch_short(P, sums, p.bn, (P.N + 15) / 16, s);
+    else launch_tiles<Sums, true>(P, sums, p, s);
+    const uint32_t pieces = (uint32_t)((c.N + 7) / 8);
+    linear_e4m3_join_kernel<OUT><<<dim3((unsigned)((c.M * pieces + 255) / 256)), 256, 0, s>>>(part, p.splits, P.M, P.N, pieces,
+                                                                                             out);
+  } else if constexpr (!OUT::CODES) {
+    if (p.bm == SHORT_ROWS) launch_short(P, out, p.bn, c.gated ? 2 * ((c.N + 15) / 16) : (P.N + 15) / 16, s);
+    else launch_tiles<OUT, false>(P, out, p, s);
+  } else {
+    launch_tiles<OUT, false>(P, out, p, s);
+  }
+  return fs::launch_status("linear_e4m3");
+}
+
+int linear(const fs_linear& c, char* work, hipStream_t s) {
+  const Plan p = plan_for(c);
+  const int64_t N = weight_rows(c);
+  const uint8_t* x = reinterpret_cast<const uint8_t*>(c.x);
+  const uint8_t* xs = reinterpret_cast<const uint8_t*>(c.x_scales);
+  int64_t ldx = c.ldx;
+  if (!xs) {
+    uint8_t* codes = reinterpret_cast<uint8_t*>(work);
+    uint8_t* words = codes + align256(c.M * c.K);
+    fs::quantize_rows_e4m3(c.x, c.ldx, c.M, c.K, c.x_dtype, codes, c.K, reinterpret_cast<uint32_t*>(words), s);
+    x = codes;
+    xs = words;
+    ldx = c.K;
+  }
+  Operands P{x, reinterpret_cast<const uint8_t*>(c.w), xs, reinterpret_cast<const uint8_t*>(c.w_scales), ldx, c.ldw, c.M, N,
+             (int)(c.K / GROUP), (int)((c.M + p.bm - 1) / p.bm), 0};
+  P.ntiles = P.tiles_m * (int)((N + p.bn - 1) / p.bn);
+  float* part = reinterpret_cast<float*>(work + encoded_bytes(c));
+  if (c.out_scales)
+    return c.gated ? run<LinearOut<FS_BF16, true, true>>(c, P, p, part, s) : run<LinearOut<FS_BF16, false, true>>(c, P, p, part, s);
+  if (c.dtype == FS_BF16)
+    return c.gated ? run<LinearOut<FS_BF16, true, false>>(c, P, p, part, s) : run<LinearOut<FS_BF16, false, false>>(c, P, p, part, s);
+  return c.gated ? run<LinearOut<FS_F16, true, false>>(c, P, p, part, s) : run<LinearOut<FS_F16, false, false>>(c, P, p, part, s);
+}
+
+int check(const fs_linear* c, const char* what) {
+  FS_CHECK_ARG(c, "%s: null pointer", what);
+  FS_CHECK_ARG(c->M >= 0 && c->N > 0 && c->K > 0 && c->K % GROUP == 0, "%s: M %lld N %lld K %lld (K a multiple of %d)", what,
+               (long long)c->M, (long long)c->N, (long long)c->K, GROUP);
+  // a copy's offset inside its tile of rows, and a row's scale word inside its group of K, are 32 bits
+  FS_CHECK_ARG(c->K <= (1 << 22) && c->M < (1 << 29) && c->N < (1 << 28), "%s: M %lld N %lld K %lld", what, (long long)c->M,
+               (long long)c->N, (long long)c->K);
+  FS_CHECK_ARG(c->x_scales || c->M * ((c->K + 511) / 512) < 0x7fffffffLL, "%s: M %lld K %lld", what, (long long)c->M,
+               (long long)c->K);
+  FS_CHECK_ARG(!c->out_scales || c->N % GROUP == 0, "%s: codes of %lld columns (a multiple of %d)", what, (long long)c->N, GROUP);
+  FS_CHECK_ARG(!plan_for(*c).join || c->M * ((c->N + 7) / 8) < 0x7fffff00LL, "%s: M %lld N %lld", what, (long long)c->M,
+               (long long)c->N);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t fs_linear_e4m3_workspace_size(const fs_linear* c) {
+  if (check(c, "linear_e4m3_workspace_size")) return 0;
+  return encoded_bytes(*c) + sums_bytes(*c, plan_for(*c));
+}
+
+extern "C" int fs_linear_e4m3_plan(const fs_linear* c, int32_t* plan) {
+  FS_CHECK_ARG(plan, "linear_e4m3_plan: null pointer");
+  if (int e = check(c, "linear_e4m3_plan")) return e;
+  const Plan p = plan_for(*c);
+  plan[0] = p.bm;
+  plan[1] = p.bn;
+  plan[2] = p.splits;
+  plan[3] = p.join;
+  return 0;
+}
+
+extern "C" int fs_linear_e4m3(const fs_linear* call, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int e = check(call, "linear_e4m3")) return e;
+  const fs_linear& c = *call;
+  const int64_t N = weight_rows(c);
+  FS_CHECK_ARG(c.x && c.w && c.w_scales && c.out, "linear_e4m3: null pointer");
+  FS_CHECK_ARG(c.x_scales || c.x_dtype == FS_F32 || c.x_dtype == FS_BF16 || c.x_dtype == FS_F16, "linear_e4m3: rows of dtype %d",
+               c.x_dtype);
+  FS_CHECK_ARG(c.out_scales || c.dtype == FS_BF16 || c.dtype == FS_F16, "linear_e4m3: results are bf16, f16 or codes (dtype %d)",
+               c.dtype);
+  FS_CHECK_ARG(!c.bias || c.bias_dtype == FS_F32 || c.bias_dtype == FS_BF16 || c.bias_dtype == FS_F16,
+               "linear_e4m3: bias of dtype %d", c.bias_dtype);
+  FS_CHECK_ARG(c.activation >= FS_ACT_NONE && c.activation <= FS_ACT_GELU_TANH, "linear_e4m3: activation %d", c.activation);
+  FS_CHECK_ARG(!c.residual || !c.out_scales, "linear_e4m3: no residual is added to codes");
+  FS_CHECK_ARG(c.ldx >= c.K && c.ldw >= c.K && c.ldo >= c.N && (!c.residual || c.ldr >= c.N), "linear_e4m3: leading dimensions");
+  FS_CHECK_ARG(c.ldw % 16 == 0 && al16(c.w) && (!c.x_scales || (c.ldx % 16 == 0 && al16(c.x))) &&
+                   (!c.out_scales || (c.ldo % 16 == 0 && al16(c.out))),
+               "linear_e4m3: codes need 16-byte aligned rows");
+  FS_CHECK_ARG(((reinterpret_cast<uintptr_t>(c.w_scales) | reinterpret_cast<uintptr_t>(c.x_scales) |
+                 reinterpret_cast<uintptr_t>(c.out_scales)) & 3) == 0,
+               "linear_e4m3: scales need whole words");
+  FS_CHECK_ARG(c.ldw < (1 << 23) && (!c.x_scales || c.ldx < (1 << 23)), "linear_e4m3: ldx %lld ldw %lld", (long long)c.ldx,
+               (long long)c.ldw);
+  if (c.M == 0) return 0;
+  const int64_t need = fs_linear_e4m3_workspace_size(call);
+  FS_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+               "linear_e4m3: workspace %lld < %lld bytes (or not 256-byte aligned)", (long long)workspace_bytes, (long long)need);
+  return linear(c, reinterpret_cast<char*>(workspace), fs::as_stream(stream));
+}

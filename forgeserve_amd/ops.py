@@ -211,6 +211,166 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
     return out
 
 
+def _check_codes(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """A matrix of codes with quantize_e4m3's scales; its rows' alignment is the library's to check."""
+    n, k = codes.shape
+    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        raise ValueError(f"{what}: {name} must be float8_e4m3fn or uint8 codes, not {codes.dtype}")
+    if scales.dtype != torch.uint8 or scales.shape != (-(-k // 512), n, 4) or not scales.is_contiguous():
+        raise ValueError(f"{what}: {name}'s scales must be contiguous uint8 ({-(-k // 512)}, {n}, 4): {tuple(scales.shape)}")
+
+
+def _check_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All on the current device (a launch goes to its stream)."""
+    require_device(*tensors)
+    if any(t is not None and t.device != tensors[0].device for t in tensors):
+        raise ValueError(f"{what}: tensors on different devices")
+    _check_current(what, tensors[0])
+
+
+def _new_codes(m: int, n: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty((m, n), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((-(-n // 512), m, 4), dtype=torch.uint8, device=device))
+
+
+def dequantize_e4m3(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values (rows, K) that codes and scales of quantize_e4m3 (add_rmsnorm_e4m3, linear_e4m3_codes) stand for, rounded
+    to dtype: float32 and bfloat16 hold each exactly, float16 what lies in its range (infinite above)."""
+    _check_device("dequantize_e4m3", codes, scales, out)
+    m, ldc = _rows(codes)
+    k = codes.shape[1]
+    if k % 128 or k == 0:
+        raise ValueError(f"dequantize_e4m3: K {k} is not a multiple of 128")
+    _check_codes("dequantize_e4m3", "the matrix", codes, scales)
+    if out is None:
+        out = torch.empty((m, k), dtype=dtype, device=codes.device)
+    _, ldo = _rows(out)
+    if out.shape != (m, k) or out.dtype != dtype:
+        raise ValueError("dequantize_e4m3: out shape/dtype")
+    if m:
+        check(_lib.load().fs_dequantize_e4m3(ptr(codes), ldc, ptr(scales), m, k, _dt(out), ptr(out), ldo, stream_ptr()),
+              "dequantize_e4m3")
+    return out
+
+
+def add_rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optional[torch.Tensor] = None,
+                     x_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """add_rmsnorm with its output in 8-bit floating point, for the product over codes that reads it: (codes, scales) of
+    RMSNorm(x [+ delta]) (model.py:29-31), as quantize_e4m3 lays them out; with delta, x + delta is also written to x_out
+    (which may be x or delta). N is a multiple of 128. The norm is computed in float32 from the sum as rounded to x's dtype
+    (float32, bfloat16, float16), and rounded once, to the code: a value is kept as quantize_e4m3 keeps it. A row whose
+    squares' sum passes float32's range has zeros; of one with an infinite or NaN element that element, or all, are NaN."""
+    _check_device("add_rmsnorm_e4m3", x, weight, delta, x_out)
+    m, ldx = _rows(x)
+    n = x.shape[1]
+    if n % 128 or n == 0:
+        raise ValueError(f"add_rmsnorm_e4m3: N {n} is not a multiple of 128")
+    if weight.shape != (n,) or weight.dtype != x.dtype or not weight.is_contiguous():
+        raise ValueError("add_rmsnorm_e4m3: weight shape/dtype")
+    ldd = ldxo = 0
+    if (delta is None) != (x_out is None):
+        raise ValueError("add_rmsnorm_e4m3: delta needs x_out, and x_out delta")
+    if delta is not None:
+        _, ldd = _rows(delta)
+        _, ldxo = _rows(x_out)
+        if any(t.shape != x.shape or t.dtype != x.dtype for t in (delta, x_out)):
+            raise ValueError("add_rmsnorm_e4m3: delta or x_out shape/dtype")
+    dt = _dt(x)
+    codes, scales = _new_codes(m, n, x.device)
+    if m:
+        check(_lib.load().fs_add_rmsnorm_e4m3(ptr(x), ldx, ptr(delta), ldd, ptr(x_out), ldxo, ptr(weight), ptr(codes), n,
+                                              ptr(scales), m, n, float(eps), dt, stream_ptr()), "add_rmsnorm_e4m3")
+    return codes, scales
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # FS_ACT_*
+
+
+def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, residual, out, out_scales) -> None:
+    m, lda = _rows(a)
+    n, ldb = _rows(w)
+    k = a.shape[1]
+    if k % 128 or k == 0 or w.shape[1] != k or n == 0 or (gated and n % 2):
+        raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)} (K a multiple of 128, of a gated product an even "
+                         "number of rows)")
+    _check_codes(what, "w", w, w_scales)
+    if a_scales is not None:
+        _check_codes(what, "a", a, a_scales)
+        x_dtype = 0
+    else:
+        if a.dtype not in DTYPE_CODE:
+            raise ValueError(f"{what}: rows of {a.dtype} (codes need a_scales)")
+        x_dtype = DTYPE_CODE[a.dtype]
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation {activation!r} (one of {', '.join(map(str, ACTIVATIONS))})")
+    bias_dtype = ldr = 0
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype not in DTYPE_CODE or (n > 1 and bias.stride(0) != 1):
+            raise ValueError(f"{what}: bias must be contiguous ({n},) in float32, bfloat16 or float16")
+        bias_dtype = DTYPE_CODE[bias.dtype]
+    if residual is not None:
+        _, ldr = _rows(residual)
+        if residual.shape != out.shape or residual.dtype != out.dtype:
+            raise ValueError(f"{what}: residual shape/dtype")
+    if m == 0:
+        return
+    lib = _lib.load()
+    call = _lib.Linear(ptr(a), ptr(a_scales), ptr(w), ptr(w_scales), ptr(bias), ptr(residual), ptr(out), ptr(out_scales), lda, ldb,
+                       ldr, out.stride(0), m, out.shape[1], k, x_dtype, DTYPE_CODE.get(out.dtype, 0), bias_dtype,
+                       ACTIVATIONS[activation], int(gated), 0)
+    need = lib.fs_linear_e4m3_workspace_size(call)
+    ws = _ws(need, a.device) if need else None   # (of the current stream: calls on two do not share it)
+    check(lib.fs_linear_e4m3(call, ptr(ws), need, stream_ptr()), what)
+
+
+def linear_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scales: Optional[torch.Tensor] = None,
+                bias: Optional[torch.Tensor] = None, activation: Optional[str] = None, gated: bool = False,
+                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(a @ w.T + bias) + residual over 8-bit floating point, or with a gate, w (2F, K) and bias (2F,) holding the gate's
+    rows and then the others', act(gate) * up + residual (nn.Linear, SwiGLU.forward: model.py:57-60, 88-93, with the residual
+    add of model.py:105-106). w, w_scales as quantize_e4m3 leaves them; a likewise, with a_scales (from quantize_e4m3,
+    add_rmsnorm_e4m3 or linear_e4m3_codes), or rows of float32, bfloat16 or float16, which are encoded within the call.
+    activation: None, "relu", "silu", "gelu" (with the normal distribution's function) or "gelu_tanh". bias: float32,
+    bfloat16 or float16. The result is bfloat16 or float16: dtype, or out's, the residual's or a's, in that order, or
+    bfloat16; the residual has the same. K is a multiple of 128. Sums as gemm_e4m3's, the rest in float32, rounded once. A
+    row's last bit may depend on how many rows the call has. out may be the residual itself, but shares no memory with a
+    or w."""
+    _check_device("linear_e4m3", a, w, w_scales, a_scales, bias, residual, out)
+    if dtype is None:
+        dtype = next((t.dtype for t in (out, residual) if t is not None),
+                     a.dtype if a.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"linear_e4m3: results are bfloat16 or float16, not {dtype}")
+    if a.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"linear_e4m3: {tuple(a.shape)} x {tuple(w.shape)}")
+    shape = (a.shape[0], w.shape[0] // 2 if gated else w.shape[0])
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=a.device)
+    _rows(out)
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError("linear_e4m3: out shape/dtype")
+    _linear_e4m3("linear_e4m3", a, w, w_scales, a_scales, bias, activation, gated, residual, out, None)
+    return out
+
+
+def linear_e4m3_codes(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scales: Optional[torch.Tensor] = None,
+                      bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                      gated: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """linear_e4m3 with its result left in 8-bit floating point for the next product: (codes, scales) as quantize_e4m3 lays
+    them out, rounded once. The result's columns are a multiple of 128."""
+    _check_device("linear_e4m3_codes", a, w, w_scales, a_scales, bias)
+    if a.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"linear_e4m3_codes: {tuple(a.shape)} x {tuple(w.shape)}")
+    n = w.shape[0] // 2 if gated else w.shape[0]
+    if n % 128 or n == 0:
+        raise ValueError(f"linear_e4m3_codes: {n} columns are not a multiple of 128")
+    codes, scales = _new_codes(a.shape[0], n, a.device)
+    _linear_e4m3("linear_e4m3_codes", a, w, w_scales, a_scales, bias, activation, gated, None, codes, scales)
+    return codes, scales
+
+
 def gemm_add_rmsnorm(a: torch.Tensor, w: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor,
                      eps: float, x_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """x = a @ w.T + residual (nn.Linear then the residual add, model.py:105-106) and y = RMSNorm(x)

@@ -302,6 +302,58 @@ int64_t fs_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
  * there too. Internal tuning, no counterpart in the reference. */
 int fs_gemm_e4m3_plan(int64_t M, int64_t N, int64_t K, int32_t* plan);
 
+/* Codes [rows][K] with fs_quantize_e4m3's scales as the values they stand for, rounded to the dtype (f32 and bf16 hold each
+ * exactly; f16 what lies in its range, infinite above). out rows of any alignment. No counterpart in the reference. */
+int fs_dequantize_e4m3(const void* codes, int64_t ldc, const void* scales, int64_t rows, int64_t K, int32_t dtype, void* out,
+                       int64_t ldo, void* stream);
+
+/* fs_add_rmsnorm (model.py:29-31, 105-106) with its output in codes, as a product over codes reads it: v = x, or x + delta
+ * rounded to the dtype, which is then written to x_out; the codes of v * rsqrt(mean(v^2) + eps) * weight, computed in f32
+ * and rounded once. N % 128 == 0; code rows 16-byte aligned, scales 4-byte aligned. x_out may be x or delta itself. */
+int fs_add_rmsnorm_e4m3(const void* x, int64_t ldx, const void* delta, int64_t ldd, void* x_out, int64_t ldxo,
+                        const void* weight, void* codes, int64_t ldc, void* scales, int64_t M, int64_t N, float eps,
+                        int32_t dtype, void* stream);
+
+#define FS_ACT_NONE 0
+#define FS_ACT_RELU 1
+#define FS_ACT_SILU 2      /* z / (1 + e^-z) */
+#define FS_ACT_GELU 3      /* z Phi(z), the normal distribution's Phi */
+#define FS_ACT_GELU_TANH 4 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+
+/* A projection over codes and what follows it. With z = x . w^T + bias:
+ *   out = act(z) + residual, or, gated (w and bias hold the gate's N rows, then N others),
+ *   out = act(z[:, :N]) * z[:, N:] + residual                                     (SwiGLU.forward, model.py:88-93)
+ * Sums as fs_gemm_e4m3's, the rest in f32, rounded once: to rows of `dtype`, or, with out_scales, to codes.
+ * x_scales NULL: x holds rows of x_dtype, which are encoded within the call. bias (contiguous), residual: or NULL. The
+ * residual has `dtype`; none is added to codes. */
+typedef struct fs_linear {
+  const void* x;
+  const void* x_scales;
+  const void* w;
+  const void* w_scales;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* out_scales;
+  int64_t ldx, ldw, ldr, ldo; /* from row to row, in elements */
+  int64_t M, N, K;            /* N: columns of the result */
+  int32_t x_dtype, dtype, bias_dtype;
+  int32_t activation;         /* FS_ACT_* */
+  int32_t gated;
+  int32_t reserved;
+} fs_linear;
+
+/* nn.Linear with what the reference does to its output (model.py:57-60, 88-93, 105-106), over codes. K % 128 == 0, and
+ * N % 128 == 0 where codes are written; code rows 16-byte aligned, scales 4-byte aligned and contiguous, other rows of any
+ * stride and alignment. out may be the residual itself, but shares no memory with x or w. The order of a sum over K
+ * goes by M. workspace: at least fs_linear_e4m3_workspace_size bytes (0: none needed), 256-byte aligned. */
+int fs_linear_e4m3(const fs_linear* call, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t fs_linear_e4m3_workspace_size(const fs_linear* call);
+
+/* How fs_linear_e4m3 computes a call: the rows and columns of a workgroup's tile, the K splits and whether the sums go
+ * through memory, into plan[0..3]. Internal tuning, no counterpart in the reference. */
+int fs_linear_e4m3_plan(const fs_linear* call, int32_t* plan);
+
 /* One decoder block of fs_run_blocks: its weights (contiguous rows, the dtype of the run; w_qkv holds wq, wk and
  * wv one below the other, w_gate_up the gate then the up projection), the norm after the attention, the
  * norm that the block's output goes through next (NULL: none; the last block only), its cache layer with
