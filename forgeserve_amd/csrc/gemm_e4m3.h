@@ -32,13 +32,12 @@ FS_DEVICE i32x8 both_chunks(u32x4 a, u32x4 b) {
 FS_DEVICE int swap_of(int row) { return (row >> 1) & 7; }
 
 // What finishes results, a class of which a kernel gets an instance:
-//   DT             the type of results that leave as 16-bit rows
 //   GATED          a tile's columns are half gate's (rows 0 .. N/2 - 1 of W), half the others' (N/2 .. N - 1), and the
 //                  results have N/2 columns
 //   STAGED         a finished tile's sums go through LDS as floats, eight columns a thread: out.piece(v, up, row, col,
 //                  cols); else from the registers, rounded first
 //   finish(a, row, col0, cols)   four columns' sums, from col0 on, to what is rounded and stored (`cols`: how many there
-//                  are); with the others' sums behind the gate's where GATED
+//                  are), and store(a, row, col0, cols) that
 //   part           not null: the f32 sums as they are, [split][M][N], instead
 template <int DT_>
 struct ResidualOut {   // round(a (+ R))
@@ -62,15 +61,17 @@ struct ResidualOut {   // round(a (+ R))
         if (col0 + e < cols) a[e] += Elem<DT>::to_f32(R[row * ldr + col0 + e]);
     }
   }
+  FS_DEVICE void store(const float4_t& a, int64_t row, int64_t col0, int64_t cols) const {
+    store_row4<DT>(a, C + row * ldc, col0, cols, vec);
+  }
 };
 
-// Four columns' sums (where gated the gate's, then the others') finished and stored.
-template <class OUT, int S>
-FS_DEVICE void put4(const OUT& out, float4_t (&a)[S], int64_t row, int64_t col0, int64_t cols) {
+// Four columns' sums finished and stored.
+template <class OUT>
+FS_DEVICE void put4(const OUT& out, float4_t a, int64_t row, int64_t col0, int64_t cols) {
   if (col0 >= cols) return;
-  if constexpr (S == 2) out.finish(a[0], a[1], row, col0, cols);
-  else out.finish(a[0], row, col0, cols);
-  store_row4<OUT::DT>(a[0], out.C + row * out.ldc, col0, cols, out.vec);
+  out.finish(a, row, col0, cols);
+  out.store(a, row, col0, cols);
 }
 
 // A finished tile of ROWS x COLS sums in LDS, PITCH floats a row (where gated the gate's columns, then the others'):
@@ -98,45 +99,6 @@ FS_DEVICE void finish_tile(const OUT& out, const float* sums, int tid, int64_t m
 // ------------------------------------------------------------------------------------------------
 // up to 16 rows: one launch, bound by the weights' bytes
 // ------------------------------------------------------------------------------------------------
-// Row of W that lane l16 reads of a workgroup's column tile j; of a gated product even tiles are the gate's, odd ones the
-// others'.
-template <bool GATED>
-FS_DEVICE int64_t short_row(int64_t n0, int j, int l16, int64_t N) {
-  return GATED ? min(n0 / 2 + 16 * (j >> 1) + l16, N / 2 - 1) + (j & 1 ? N / 2 : 0) : min(n0 + 16 * j + l16, N - 1);
-}
-// The eight waves' sums of TN column tiles joined in order through LDS: wave j finishes tile j (where gated, tiles 2 j and
-// 2 j + 1); lane (l16, g) has row l16, columns 16 j + 4 g .. of it.
-template <class OUT, int TN>
-FS_DEVICE void short_results(const OUT& out, float4_t (*red)[TN][64], const float4_t (&acc)[TN], int w, int lane, int64_t n0,
-                             int M, int64_t N) {
-  static_assert(!OUT::GATED || TN % 2 == 0, "a gate's tile and its other's");
-  constexpr int STEP = OUT::GATED ? 2 : 1;
-  const int l16 = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int j = 0; j < TN; ++j) red[w][j][lane] = acc[j];
-  __syncthreads();
-  if (w >= TN / STEP) return;
-  float4_t a[STEP];
-#pragma unroll
-  for (int h = 0; h < STEP; ++h) {
-    a[h] = red[0][STEP * w + h][lane];
-#pragma unroll
-    for (int v = 1; v < 8; ++v) {
-      const float4_t b = red[v][STEP * w + h][lane];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) a[h][r] += b[r];
-    }
-  }
-  const int64_t col0 = n0 / STEP + 16 * w + 4 * g;
-  if constexpr (OUT::STAGED && !OUT::GATED) {
-    if (out.part) {   // (N % 4 == 0)
-      if (l16 < M && col0 < N) *reinterpret_cast<float4_t*>(out.part + l16 * N + col0) = a[0];
-      return;
-    }
-  }
-  if (l16 < M) put4(out, a, l16, col0, N / STEP);
-}
-
 // A workgroup takes 16 TN columns of C; its eight waves split K and are joined in order through LDS. Weights go straight
 // from HBM to registers in the instruction's own shape (a lane's two 16-byte chunks of a row's 128; a wave's load covers
 // whole lines), DEPTH stages ahead. While the first of them are on their way the workgroup encodes the rows into LDS,
@@ -183,7 +145,7 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
   int64_t srow[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int64_t n = short_row<OUT::GATED>(n0, j, l16, N);
+    const int64_t n = min(n0 + 16 * j + l16, N - 1);
     wrow[j] = W + n * ldw + 16 * g;
     srow[j] = 4 * n;
   }
@@ -247,7 +209,20 @@ __global__ void __launch_bounds__(512) gemm_e4m3_short_kernel(const uint16_t* __
     }
   }
   __syncthreads();   // every wave has read its codes
-  short_results(out, reinterpret_cast<float4_t(*)[TN][64]>(xcodes), acc, w, lane, n0, M, N);
+  float4_t(*red)[TN][64] = reinterpret_cast<float4_t(*)[TN][64]>(xcodes);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) red[w][j][lane] = acc[j];
+  __syncthreads();
+  if (w >= TN) return;
+  // wave j joins its columns' eight sums in order: lane (l16, g) has row l16, columns 16 j + 4 g ..
+  float4_t a = red[0][w][lane];
+#pragma unroll
+  for (int v = 1; v < 8; ++v) {
+    const float4_t b = red[v][w][lane];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] += b[r];
+  }
+  if (l16 < M) put4(out, a, l16, n0 + 16 * w + 4 * g, N);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -432,8 +407,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_e4m3_tile_kernel(Operands
       if (out.part) {   // (N % 4 == 0; never of a gated class)
         if (col0 < P.N) *reinterpret_cast<float4_t*>(out.part + ((int64_t)split * P.M + row) * P.N + col0) = acc[i][j];
       } else if constexpr (!OUT::STAGED) {
-        float4_t a[1] = {acc[i][j]};
-        put4(out, a, row, col0, P.N);
+        put4(out, acc[i][j], row, col0, P.N);
       }
     }
   }
@@ -681,42 +655,44 @@ __global__ void __launch_bounds__(512, 2) gemm_e4m3_long_kernel(Operands P, OUT 
     }
     return;
   }
-  // The wave's rounded results (the residual added before) to LDS, then out by whole rows, 16 bytes a lane. Every copy
-  // has landed and, past this barrier, every wave has read its last operands: the ring's space is free.
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  char* out = smem + wave * 128 * PITCH;
+  if constexpr (!OUT::STAGED) {
+    // The wave's rounded results (the residual added before) to LDS, then out by whole rows, 16 bytes a lane. Every copy
+    // has landed and, past this barrier, every wave has read its last operands: the ring's space is free.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    char* out = smem + wave * 128 * PITCH;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = m0 + wm * 128 + 32 * i + l32;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = m0 + wm * 128 + 32 * i + l32;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float4_t a = four(i, j, t);
-        const int64_t col0 = n0 + wn * 64 + 32 * j + 8 * t + 4 * half;
-        if (row < P.M) to.finish(a, row, col0, P.N);
-        *reinterpret_cast<u32x2_t*>(out + (32 * i + l32) * PITCH + 2 * (32 * j + 8 * t + 4 * half)) =
-            u32x2_t{(uint32_t)Elem<OUT::DT>::store_bits(a[0]) | ((uint32_t)Elem<OUT::DT>::store_bits(a[1]) << 16),
-                    (uint32_t)Elem<OUT::DT>::store_bits(a[2]) | ((uint32_t)Elem<OUT::DT>::store_bits(a[3]) << 16)};
-      }
-  }
-  const int64_t col = n0 + wn * 64 + 8 * (lane & 7);
-  uint16_t* C = to.C;
-  const int64_t ldc = to.ldc;
-  const bool wide = col + 8 <= P.N && (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
+        for (int t = 0; t < 4; ++t) {
+          float4_t a = four(i, j, t);
+          const int64_t col0 = n0 + wn * 64 + 32 * j + 8 * t + 4 * half;
+          if (row < P.M) to.finish(a, row, col0, P.N);
+          *reinterpret_cast<u32x2_t*>(out + (32 * i + l32) * PITCH + 2 * (32 * j + 8 * t + 4 * half)) =
+              u32x2_t{(uint32_t)Elem<OUT::DT>::store_bits(a[0]) | ((uint32_t)Elem<OUT::DT>::store_bits(a[1]) << 16),
+                      (uint32_t)Elem<OUT::DT>::store_bits(a[2]) | ((uint32_t)Elem<OUT::DT>::store_bits(a[3]) << 16)};
+        }
+    }
+    const int64_t col = n0 + wn * 64 + 8 * (lane & 7);
+    uint16_t* C = to.C;
+    const int64_t ldc = to.ldc;
+    const bool wide = col + 8 <= P.N && (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
 #pragma unroll 4
-  for (int it = 0; it < 16; ++it) {
-    const int lr = it * 8 + (lane >> 3);
-    const int64_t row = m0 + wm * 128 + lr;
-    const u32x4 o = *reinterpret_cast<const u32x4*>(out + lr * PITCH + 16 * (lane & 7));
-    if (row >= P.M) continue;
-    if (wide) {
-      *reinterpret_cast<u32x4*>(C + row * ldc + col) = o;
-    } else {
+    for (int it = 0; it < 16; ++it) {
+      const int lr = it * 8 + (lane >> 3);
+      const int64_t row = m0 + wm * 128 + lr;
+      const u32x4 o = *reinterpret_cast<const u32x4*>(out + lr * PITCH + 16 * (lane & 7));
+      if (row >= P.M) continue;
+      if (wide) {
+        *reinterpret_cast<u32x4*>(C + row * ldc + col) = o;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + e < P.N) C[row * ldc + col + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+        for (int e = 0; e < 8; ++e)
+          if (col + e < P.N) C[row * ldc + col + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+      }
     }
   }
 }

@@ -89,8 +89,7 @@ __global__ void __launch_bounds__(256) gemm_e4m3_join_kernel(const float* __rest
     for (int r = 0; r < 4; ++r) a[r] += b[r];
   }
   const ResidualOut<DT> out{C, ldc, R, ldr, vec, nullptr};
-  float4_t sum[1] = {a};
-  put4(out, sum, row, e - row * N, N);
+  put4(out, a, row, e - row * N, N);
 }
 
 struct Plan {

@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int SHORT_ROWS = 16;   // rows that the kernel without tiles takes
+constexpr int STREAM_ROWS = 32;   // rows that the kernels without tiles in LDS take
 
 // ------------------------------------------------------------------------------------------------
 // what is done with the sums
@@ -39,9 +39,8 @@ FS_DEVICE float gelu_erf(float z) {
   return z * (z < 0.f ? phi : 1.f - phi);
 }
 
-template <int DT_, bool GATED_, bool CODES_>
+template <bool GATED_, bool CODES_>
 struct LinearOut {
-  static constexpr int DT = DT_;
   static constexpr bool GATED = GATED_, CODES = CODES_, STAGED = true;
   uint16_t* C;            // rows, or codes
   int64_t ldc;            // in elements
@@ -49,11 +48,15 @@ struct LinearOut {
   int64_t ldr;
   const void* bias;
   int64_t up;             // where the others' bias begins
-  int32_t bias_dtype, act;
+  int32_t dtype, bias_dtype, act;
   bool vec, bias_vec;     // eight columns of C and R at a time; of the bias
   uint8_t* scales;        // of codes
   int64_t rows;
   float* part;
+
+  // a 16-bit value of the results' type, and a result as one
+  FS_DEVICE float value(uint32_t h) const { return dtype == FS_BF16 ? bf16_to_f32((uint16_t)h) : f16_to_f32((uint16_t)h); }
+  FS_DEVICE uint32_t bits(float v) const { return dtype == FS_BF16 ? f32_to_bf16(v) : f32_to_f16(v); }
 
   template <int NC>
   FS_DEVICE void add_bias(float (&v)[NC], int64_t at, int64_t left) const {
@@ -122,23 +125,27 @@ struct LinearOut {
         for (int h = 0; h < NC / 4; ++h) {
           const u32x2_t w = *reinterpret_cast<const u32x2_t*>(r + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * h + e] += half_of<DT>(w[e >> 1], e & 1);
+          for (int e = 0; e < 4; ++e) v[4 * h + e] += value(w[e >> 1] >> (16 * (e & 1)));
         }
       } else {
 #pragma unroll
         for (int e = 0; e < NC; ++e)
-          if (col + e < cols) v[e] += Elem<DT>::to_f32(r[e]);
+          if (col + e < cols) v[e] += value(r[e]);
       }
     }
   }
-  FS_DEVICE void finish(float4_t& a, int64_t row, int64_t col0, int64_t cols) const {
-    float4_t b = a;
-    finish(a, b, row, col0, cols);
-  }
-  FS_DEVICE void finish(float4_t& a, float4_t b, int64_t row, int64_t col0, int64_t cols) const {
+  // Four columns' sums (the others' in b where gated) finished and stored.
+  FS_DEVICE void four(const float4_t& a, const float4_t& b, int64_t row, int64_t col, int64_t cols) const {
     float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
-    compute(v, u, row, col0, cols);
-    a = float4_t{v[0], v[1], v[2], v[3]};
+    compute(v, u, row, col, cols);
+    uint16_t* c = C + row * ldc + col;
+    if (vec && col + 4 <= cols) {
+      *reinterpret_cast<u32x2_t*>(c) = u32x2_t{bits(v[0]) | bits(v[1]) << 16, bits(v[2]) | bits(v[3]) << 16};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < cols) c[e] = (uint16_t)bits(v[e]);
+    }
   }
   // Eight columns' sums finished and stored. For codes 16 lanes side by side hold a row's group (all in range, or none).
   FS_DEVICE void piece(float (&v)[8], float (&u)[8], int64_t row, int64_t col, int64_t cols) const {
@@ -160,16 +167,15 @@ struct LinearOut {
       }
     } else {
       uint16_t* c = C + row * ldc + col;
-      uint16_t o[8];
+      uint32_t o[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = Elem<DT>::store_bits(v[e]);
+      for (int e = 0; e < 8; ++e) o[e] = bits(v[e]);
       if (vec && col + 8 <= cols) {
-        *reinterpret_cast<u32x4*>(c) = u32x4{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16,
-                                             o[4] | (uint32_t)o[5] << 16, o[6] | (uint32_t)o[7] << 16};
+        *reinterpret_cast<u32x4*>(c) = u32x4{o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16};
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (col + e < cols) c[e] = o[e];
+          if (col + e < cols) c[e] = (uint16_t)o[e];
       }
     }
   }
@@ -204,62 +210,101 @@ __global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __re
 }
 
 // ------------------------------------------------------------------------------------------------
-// up to 16 rows: bound by the weight's bytes
+// up to 32 rows: bound by the weight's bytes
 // ------------------------------------------------------------------------------------------------
-// A workgroup takes 16 TN rows of W; its eight waves split K and are joined in order through LDS. Codes of both operands go
-// straight to registers in the instruction's own shape, DEPTH stages ahead: W's from HBM, x's (16 rows of them at most, the
-// same for every workgroup) from L2.
-template <class OUT, int TN, int DEPTH>
-__global__ void __launch_bounds__(512) linear_e4m3_short_kernel(Operands P, OUT out) {
-  __shared__ float4_t red[8][TN][64];
+// A workgroup takes `per` rows of W (of a gated product `per` columns of the results: as many rows of each half), so many
+// that the grid is one round of the CUs where it can be and each draws the same share; its eight waves split K and are joined
+// in order through LDS. Codes of both operands go straight to registers in the instruction's own shape, DEPTH stages ahead: W's
+// from HBM, x's (16 TM rows, the same for every workgroup, read once for TN tiles of W) from L2. A tile is 16 rows of W, or
+// eight columns' gate's rows and their others', so that any number of tiles may share a workgroup.
+template <class OUT, int TM, int TN, int DEPTH>
+__global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT out, int per) {
+  constexpr int TILES = TM * TN, CH = TILES < 8 ? TILES : 8, COLS = OUT::GATED ? 8 : 16;
+  __shared__ float4_t red[8][CH][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * TN);
+  const int64_t cols = OUT::GATED ? P.N / 2 : P.N, c0 = (int64_t)blockIdx.x * per, c1 = min(c0 + per, cols);
   const int k0 = (int)((int64_t)w * P.nk / 8), k1 = (int)((int64_t)(w + 1) * P.nk / 8);
   const int M = (int)P.M;
   struct Stage {
-    u32x4 c[TN][2], x[2];
-    uint32_t s[TN], xs;
+    u32x4 c[TN][2], x[TM][2];
+    uint32_t s[TN], xs[TM];
   } ring[DEPTH];
-  const int xrow = min(l16, M - 1);   // (lanes past the last row: results nobody stores)
-  const uint8_t* xp = P.x + xrow * P.ldx + 16 * g;
+  const uint8_t* xp[TM];
+  int xrow[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {   // (lanes past the last row: results nobody stores)
+    xrow[i] = min(16 * i + l16, M - 1);
+    xp[i] = P.x + xrow[i] * P.ldx + 16 * g;
+  }
   const uint8_t* wrow[TN];
   int64_t srow[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int64_t n = short_row<OUT::GATED>(n0, j, l16, P.N);
+    const int64_t c = min(c0 + COLS * j + (OUT::GATED ? l16 & 7 : l16), c1 - 1), n = OUT::GATED && l16 >= 8 ? c + cols : c;
     wrow[j] = P.w + n * P.ldw + 16 * g;
     srow[j] = 4 * n;
   }
   auto load = [&](int k, Stage& x) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      x.c[j][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP));
-      x.c[j][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP + 64));
+      x.c[j][0] = *reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP);
+      x.c[j][1] = *reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP + 64);
       x.s[j] = P.ws[(int64_t)(k >> 2) * 4 * P.N + srow[j] + (k & 3)];
     }
-    x.x[0] = *reinterpret_cast<const u32x4*>(xp + (int64_t)k * GROUP);
-    x.x[1] = *reinterpret_cast<const u32x4*>(xp + (int64_t)k * GROUP + 64);
-    x.xs = P.xs[((int64_t)(k >> 2) * M + xrow) * 4 + (k & 3)];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      x.x[i][0] = *reinterpret_cast<const u32x4*>(xp[i] + (int64_t)k * GROUP);
+      x.x[i][1] = *reinterpret_cast<const u32x4*>(xp[i] + (int64_t)k * GROUP + 64);
+      x.xs[i] = P.xs[((int64_t)(k >> 2) * M + xrow[i]) * 4 + (k & 3)];
+    }
   };
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
     if (k0 + d < k1) load(k0 + d, ring[d]);
-  float4_t acc[TN];
+  float4_t acc[TILES];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < TILES; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
   for (int kt = k0; kt < k1; kt += DEPTH) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (kt + d >= k1) break;   // (wave-uniform)
-      const i32x8 xf = both_chunks(ring[d].x[0], ring[d].x[1]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-        acc[j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), xf, acc[j], ring[d].s[j], ring[d].xs);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i * TN + j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), both_chunks(ring[d].x[i][0], ring[d].x[i][1]),
+                                          acc[i * TN + j], ring[d].s[j], ring[d].xs[i]);
       if (kt + d + DEPTH < k1) load(kt + d + DEPTH, ring[d]);
     }
   }
-  short_results(out, red, acc, w, lane, n0, M, P.N);
+  // CH tiles at a time: wave t joins tile t's eight sums in order; lane (l16, g) has row l16, and of the tile's rows of W
+  // (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
+#pragma unroll
+  for (int first = 0; first < TILES; first += CH) {
+    if (first) __syncthreads();
+#pragma unroll
+    for (int t = first; t < first + CH && t < TILES; ++t) red[w][t - first][lane] = acc[t];
+    __syncthreads();
+    const int t = first + w;
+    if (w >= CH || t >= TILES) continue;
+    float4_t a = red[0][w][lane], b = a;
+    if (OUT::GATED) b = red[0][w][(lane + 32) & 63];
+#pragma unroll
+    for (int v = 1; v < 8; ++v) {
+      const float4_t p = red[v][w][lane], q = OUT::GATED ? red[v][w][(lane + 32) & 63] : p;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        a[r] += p[r];
+        b[r] += q[r];
+      }
+    }
+    const int row = 16 * (t / TN) + l16;
+    const int64_t col = c0 + COLS * (t % TN) + 4 * g;
+    if (row >= M || col >= c1 || (OUT::GATED && g >= 2)) continue;
+    if (!OUT::GATED && out.part) *reinterpret_cast<float4_t*>(out.part + row * P.N + col) = a;   // (N % 4 == 0)
+    else if constexpr (!OUT::CODES) out.four(a, b, row, col, cols);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -271,14 +316,24 @@ struct Plan {
 };
 int64_t weight_rows(const fs_linear& c) { return c.gated ? 2 * c.N : c.N; }
 
+// Columns of the results that a workgroup of the kernel without tiles takes, of `cols`: a multiple of eight, so many that the
+// grid is one round of the 256 CUs, or the fewest rounds where that is more than seven tiles; and the tiles of its kernel.
+int64_t stream_columns(int64_t cols, bool gated) {
+  const int64_t most = 256 * (gated ? 56 : 112), rounds = (cols + most - 1) / most;
+  return ((cols + 256 * rounds - 1) / (256 * rounds) + 7) / 8 * 8;
+}
+int stream_tiles(int64_t cols, bool gated) {
+  const int64_t tiles = gated ? stream_columns(cols, true) / 8 : (stream_columns(cols, false) + 15) / 16;
+  return tiles <= 2 ? (int)tiles : tiles <= 4 ? 4 : 7;
+}
+
 // Tiles as gemm_e4m3.hip's rule has them. Codes leave a tile of 256 x 256, or of 128 columns without a gate, by themselves;
 // sums that go through memory are written and read at 4.5 TB/s and cost a launch of 3 us.
 Plan plan_for(const fs_linear& c) {
   const int64_t M = c.M, N = weight_rows(c), nk = c.K / GROUP;
-  if (M <= SHORT_ROWS) {
-    const int64_t tiles = c.gated ? 2 * ((c.N + 15) / 16) : (N + 15) / 16;
-    const int tn = tiles <= 256 && !c.gated ? 1 : tiles <= 512 ? 2 : 4;
-    return Plan{SHORT_ROWS, 16 * tn, 1, c.out_scales != nullptr};
+  if (M <= STREAM_ROWS) {
+    const int tiles = c.out_scales ? stream_tiles(N, false) : stream_tiles(c.N, c.gated != 0);
+    return Plan{M <= 16 ? 16 : 32, 16 * tiles, 1, c.out_scales != nullptr};
   }
   struct Cand {
     int bm, bn;
@@ -308,13 +363,21 @@ int64_t sums_bytes(const fs_linear& c, const Plan& p) {
   return p.join ? (int64_t)p.splits * c.M * weight_rows(c) * (int64_t)sizeof(float) : 0;
 }
 
+// DEPTH stages of TN tiles each: 14 to 16 KB of W on their way a wave, less where the registers are the sums'.
+template <class OUT, int TM>
+void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
+  const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
+  const dim3 grid((unsigned)((cols + per - 1) / per));
+  if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1, TM == 1 ? 7 : 4><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2, TM == 1 ? 4 : 3><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else linear_e4m3_stream_kernel<OUT, TM, 7, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
+}
 template <class OUT>
-void launch_short(const Operands& P, const OUT& out, int bn, int64_t tiles, hipStream_t s) {
-  const int tn = bn / 16;
-  const dim3 grid((unsigned)((tiles + tn - 1) / tn));
-  if (tn == 4) linear_e4m3_short_kernel<OUT, 4, 2><<<grid, 512, 0, s>>>(P, out);
-  else if (tn == 2) linear_e4m3_short_kernel<OUT, 2, 4><<<grid, 512, 0, s>>>(P, out);
-  else if constexpr (!OUT::GATED) linear_e4m3_short_kernel<OUT, 1, 7><<<grid, 512, 0, s>>>(P, out);
+void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
+  const int tn = p.bn / 16;
+  if (p.bm == 16) launch_stream<OUT, 1>(P, out, tn, per, s);
+  else launch_stream<OUT, 2>(P, out, tn, per, s);
 }
 
 // PARTS: a class of which only the sums in memory are asked for.
@@ -332,6 +395,7 @@ void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t 
 
 template <class OUT>
 int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t s) {
+  const bool stream = c.M <= STREAM_ROWS;
   OUT out;
   out.C = reinterpret_cast<uint16_t*>(c.out);
   out.ldc = c.ldo;
@@ -339,6 +403,7 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
   out.ldr = c.ldr;
   out.bias = c.bias;
   out.up = c.N;
+  out.dtype = c.dtype;
   out.bias_dtype = c.bias_dtype;
   out.act = c.activation;
   out.vec = al16(c.out) && c.ldo % 8 == 0 && (!c.residual || (al16(c.residual) && c.ldr % 8 == 0));
@@ -347,16 +412,16 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
   out.rows = c.M;
   out.part = nullptr;
   if (p.join) {
-    typedef LinearOut<FS_BF16, false, false> Sums;   // (its type is of no account)
+    typedef LinearOut<false, false> Sums;
     Sums sums{};
     sums.part = part;
-    if (p.bm == SHORT_ROWS) launch_short(P, sums, p.bn, (P.N + 15) / 16, s);
+    if (stream) launch_stream(P, sums, p, stream_columns(P.N, false), s);   // (rows of W in their order, gated or not)
     else launch_tiles<Sums, true>(P, sums, p, s);
     const uint32_t pieces = (uint32_t)((c.N + 7) / 8);
     linear_e4m3_join_kernel<OUT><<<dim3((unsigned)((c.M * pieces + 255) / 256)), 256, 0, s>>>(part, p.splits, P.M, P.N, pieces,
                                                                                              out);
   } else if constexpr (!OUT::CODES) {
-    if (p.bm == SHORT_ROWS) launch_short(P, out, p.bn, c.gated ? 2 * ((c.N + 15) / 16) : (P.N + 15) / 16, s);
+    if (stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
     else launch_tiles<OUT, false>(P, out, p, s);
   } else {
     launch_tiles<OUT, false>(P, out, p, s);
@@ -382,11 +447,8 @@ int linear(const fs_linear& c, char* work, hipStream_t s) {
              (int)(c.K / GROUP), (int)((c.M + p.bm - 1) / p.bm), 0};
   P.ntiles = P.tiles_m * (int)((N + p.bn - 1) / p.bn);
   float* part = reinterpret_cast<float*>(work + encoded_bytes(c));
-  if (c.out_scales)
-    return c.gated ? run<LinearOut<FS_BF16, true, true>>(c, P, p, part, s) : run<LinearOut<FS_BF16, false, true>>(c, P, p, part, s);
-  if (c.dtype == FS_BF16)
-    return c.gated ? run<LinearOut<FS_BF16, true, false>>(c, P, p, part, s) : run<LinearOut<FS_BF16, false, false>>(c, P, p, part, s);
-  return c.gated ? run<LinearOut<FS_F16, true, false>>(c, P, p, part, s) : run<LinearOut<FS_F16, false, false>>(c, P, p, part, s);
+  if (c.out_scales) return c.gated ? run<LinearOut<true, true>>(c, P, p, part, s) : run<LinearOut<false, true>>(c, P, p, part, s);
+  return c.gated ? run<LinearOut<true, false>>(c, P, p, part, s) : run<LinearOut<false, false>>(c, P, p, part, s);
 }
 
 int check(const fs_linear* c, const char* what) {

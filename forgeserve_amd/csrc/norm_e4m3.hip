@@ -80,19 +80,21 @@ struct NormArgs {
   float eps;
 };
 
-// T threads a row, WG / T rows a workgroup, a thread's pieces of eight columns t, t + T, ... (G of them). G == 0: rows of any
-// length, v read again for the codes.
-template <int DT, bool VEC, int T, int WG, int G>
+// T threads a row, WG / T rows a workgroup, a thread's pieces of eight columns t, t + T, ... (G of them). The squares of 512
+// columns, a wave's, are added across it and these sums in order, whatever T and G. G == 0: rows of any length, v read again
+// for the codes.
+template <int DT, bool VEC, bool DELTA, int T, int WG, int G>
 __global__ void __launch_bounds__(WG) add_rmsnorm_e4m3_kernel(NormArgs a) {
   typedef typename Elem<DT>::T E;
   static_assert(T == 64 || T == WG, "a wave or a workgroup a row");
-  __shared__ float red[WG / 64];
+  constexpr int SUMS = G > 0 ? G * (T / 64) : WG / 64;   // of 512 columns each, or a wave's
+  __shared__ float red[T > 64 ? SUMS : 1];
   const int t = threadIdx.x % T, lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * (WG / T) + threadIdx.x / T;
   if (T == 64 && row >= a.M) return;
   const E* x = static_cast<const E*>(a.x) + row * a.ldx;
-  const E* delta = a.delta ? static_cast<const E*>(a.delta) + row * a.ldd : nullptr;
-  E* xo = a.delta ? static_cast<E*>(a.x_out) + row * a.ldxo : nullptr;
+  const E* delta = DELTA ? static_cast<const E*>(a.delta) + row * a.ldd : nullptr;
+  E* xo = DELTA ? static_cast<E*>(a.x_out) + row * a.ldxo : nullptr;
   const E* w = static_cast<const E*>(a.w);
   const int np = a.N / 8;
   uint8_t* codes = a.codes + row * a.ldc;
@@ -102,22 +104,19 @@ __global__ void __launch_bounds__(WG) add_rmsnorm_e4m3_kernel(NormArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e] = value_of<DT>(xr, e);
-      if (delta) v[e] = Elem<DT>::round(v[e] + value_of<DT>(dr, e));
+      if (DELTA) v[e] = Elem<DT>::round(v[e] + value_of<DT>(dr, e));
       sq += v[e] * v[e];
     }
-    if (delta) store8<DT, VEC>(xo + 8 * p, v);
+    if (DELTA) store8<DT, VEC>(xo + 8 * p, v);
     return sq;
   };
-  auto scale_of = [&](float sq) {
-    sq = wave_sum(sq);
-    if (T > 64) {
-      if (lane == 0) red[threadIdx.x >> 6] = sq;
-      __syncthreads();
-      sq = 0.f;
+  auto scale_of = [&](float sum) { return 1.0f / sqrtf(sum / (float)a.N + a.eps); };
+  auto added = [&]() {
+    __syncthreads();
+    float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < WG / 64; ++i) sq += red[i];
-    }
-    return 1.0f / sqrtf(sq / (float)a.N + a.eps);
+    for (int i = 0; i < SUMS; ++i) sum += red[i];
+    return sum;
   };
   auto codes_of = [&](int p, const float (&v)[8], const Eight<DT>& wr, float r) {   // p: all of a wave's in turn
     float y[8];
@@ -132,20 +131,26 @@ __global__ void __launch_bounds__(WG) add_rmsnorm_e4m3_kernel(NormArgs a) {
     for (int u = 0; u < G; ++u) {   // every load in flight before any arithmetic
       const int p = min(t + T * u, np - 1);
       xr[u] = load8<DT, VEC>(x + 8 * p);
-      if (delta) dr[u] = load8<DT, VEC>(delta + 8 * p);
-      wr[u] = load8<DT, VEC>(w + 8 * p);
+      if (DELTA) dr[u] = load8<DT, VEC>(delta + 8 * p);
     }
-    float v[G][8], sq = 0.f;
+#pragma unroll
+    for (int u = 0; u < G; ++u) wr[u] = load8<DT, VEC>(w + 8 * min(t + T * u, np - 1));
+    __builtin_amdgcn_sched_barrier(0);   // (the compiler would wait for each piece's before it loads the next)
+    float v[G][8], sum = 0.f;
 #pragma unroll
     for (int u = 0; u < G; ++u) {
+      float sq = 0.f;
       if (t + T * u < np) {
-        sq += sum_piece(t + T * u, xr[u], dr[u], v[u]);
+        sq = sum_piece(t + T * u, xr[u], dr[u], v[u]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
       }
+      sq = wave_sum(sq);
+      if (T == 64) sum += sq;
+      else if (lane == 0) red[(t >> 6) + (T / 64) * u] = sq;
     }
-    const float r = scale_of(sq);
+    const float r = scale_of(T == 64 ? sum : added());
 #pragma unroll
     for (int u = 0; u < G; ++u)
       if (((t & ~63) + T * u) < np) codes_of(t + T * u, v[u], wr[u], r);   // (wave-uniform)
@@ -153,11 +158,13 @@ __global__ void __launch_bounds__(WG) add_rmsnorm_e4m3_kernel(NormArgs a) {
     float sq = 0.f;
     for (int p = t; p < np; p += T) {
       float v[8];
-      const Eight<DT> xr = load8<DT, VEC>(x + 8 * p), dr = delta ? load8<DT, VEC>(delta + 8 * p) : xr;
+      const Eight<DT> xr = load8<DT, VEC>(x + 8 * p), dr = DELTA ? load8<DT, VEC>(delta + 8 * p) : xr;
       sq += sum_piece(p, xr, dr, v);
     }
-    const float r = scale_of(sq);
-    const E* again = delta ? xo : x;   // (a thread reads what it wrote itself)
+    sq = wave_sum(sq);
+    if (lane == 0) red[t >> 6] = sq;
+    const float r = scale_of(added());
+    const E* again = DELTA ? xo : x;   // (a thread reads what it wrote itself)
     for (int p = t; (p & ~63) < np; p += T) {
       float v[8];
       const int at = 8 * min(p, np - 1);
@@ -190,17 +197,27 @@ __global__ void __launch_bounds__(256) dequantize_e4m3_kernel(const uint8_t* __r
 
 bool dtype_ok(int32_t dt) { return dt == FS_F32 || dt == FS_BF16 || dt == FS_F16; }
 
-// Threads and pieces a thread by the row's length alone.
-template <int DT, bool VEC>
+// Up to four rows a CU are held by their latency: one piece a thread (64 x 4096 bf16 with delta 3.8 us, two pieces 4.2; 64 x
+// 8192 4.7, four pieces 5.7); longer batches by HBM, where fewer, larger threads draw more (8005 x 4096 22.2 us without delta,
+// one piece 25.9). The results are the same.
+template <int DT, bool VEC, bool DELTA>
 void launch_norm(const NormArgs& a, hipStream_t s) {
   const unsigned rows = (unsigned)a.M, rows4 = (unsigned)((a.M + 3) / 4);
-  if (a.N <= 512) add_rmsnorm_e4m3_kernel<DT, VEC, 64, 256, 1><<<rows4, 256, 0, s>>>(a);
-  else if (a.N <= 1024) add_rmsnorm_e4m3_kernel<DT, VEC, 64, 256, 2><<<rows4, 256, 0, s>>>(a);
-  else if (a.N <= 2048) add_rmsnorm_e4m3_kernel<DT, VEC, 256, 256, 1><<<rows, 256, 0, s>>>(a);
-  else if (a.N <= 4096) add_rmsnorm_e4m3_kernel<DT, VEC, 256, 256, 2><<<rows, 256, 0, s>>>(a);
-  else if (a.N <= 8192) add_rmsnorm_e4m3_kernel<DT, VEC, 256, 256, 4><<<rows, 256, 0, s>>>(a);
-  else if (a.N <= 16384) add_rmsnorm_e4m3_kernel<DT, VEC, 1024, 1024, 2><<<rows, 1024, 0, s>>>(a);
-  else add_rmsnorm_e4m3_kernel<DT, VEC, 1024, 1024, 0><<<rows, 1024, 0, s>>>(a);
+  const bool few = a.M <= 1024;
+#define FS_LAUNCH(T, WG, G) add_rmsnorm_e4m3_kernel<DT, VEC, DELTA, T, WG, G><<<T == 64 ? rows4 : rows, WG, 0, s>>>(a)
+  if (a.N <= 512) FS_LAUNCH(64, 256, 1);
+  else if (a.N <= 1024) FS_LAUNCH(64, 256, 2);
+  else if (a.N <= 2048) FS_LAUNCH(256, 256, 1);
+  else if (a.N <= 4096) few ? FS_LAUNCH(512, 512, 1) : FS_LAUNCH(256, 256, 2);
+  else if (a.N <= 8192) few ? FS_LAUNCH(1024, 1024, 1) : FS_LAUNCH(256, 256, 4);
+  else if (a.N <= 16384) few ? FS_LAUNCH(1024, 1024, 2) : FS_LAUNCH(512, 512, 4);
+  else FS_LAUNCH(1024, 1024, 0);
+#undef FS_LAUNCH
+}
+template <int DT>
+void launch_norm(const NormArgs& a, bool vec, hipStream_t s) {
+  if (a.delta) vec ? launch_norm<DT, true, true>(a, s) : launch_norm<DT, false, true>(a, s);
+  else vec ? launch_norm<DT, true, false>(a, s) : launch_norm<DT, false, false>(a, s);
 }
 
 }  // namespace
@@ -222,9 +239,9 @@ extern "C" int fs_add_rmsnorm_e4m3(const void* x, int64_t ldx, const void* delta
   const int64_t per = dtype == FS_F32 ? 4 : 8;
   const bool vec = al16(x) && al16(weight) && ldx % per == 0 &&
                    (!delta || (al16(delta) && al16(x_out) && ldd % per == 0 && ldxo % per == 0));
-  if (dtype == FS_F32) vec ? launch_norm<FS_F32, true>(a, s) : launch_norm<FS_F32, false>(a, s);
-  else if (dtype == FS_BF16) vec ? launch_norm<FS_BF16, true>(a, s) : launch_norm<FS_BF16, false>(a, s);
-  else vec ? launch_norm<FS_F16, true>(a, s) : launch_norm<FS_F16, false>(a, s);
+  if (dtype == FS_F32) launch_norm<FS_F32>(a, vec, s);
+  else if (dtype == FS_BF16) launch_norm<FS_BF16>(a, vec, s);
+  else launch_norm<FS_F16>(a, vec, s);
   return fs::launch_status("add_rmsnorm_e4m3");
 }
 

@@ -211,46 +211,61 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
     return out
 
 
-def _check_codes(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
-    """A matrix of codes with quantize_e4m3's scales; its rows' alignment is the library's to check."""
-    n, k = codes.shape
-    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8):
-        raise ValueError(f"{what}: {name} must be float8_e4m3fn or uint8 codes, not {codes.dtype}")
-    if scales.dtype != torch.uint8 or scales.shape != (-(-k // 512), n, 4) or not scales.is_contiguous():
-        raise ValueError(f"{what}: {name}'s scales must be contiguous uint8 ({-(-k // 512)}, {n}, 4): {tuple(scales.shape)}")
-
-
-def _check_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """All on the current device (a launch goes to its stream)."""
+# The calls on codes below take 5 to 30 us on the GPU: their checks are written so that a good call pays few microseconds.
+def _stream_of(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The current stream, with every tensor on the current device (a launch goes to its stream)."""
+    index = first.get_device()
+    if index >= 0 and index == torch._C._cuda_getDevice():
+        for t in others:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return torch._C._cuda_getCurrentRawStream(index)
+    tensors = (first, *others)
     require_device(*tensors)
-    if any(t is not None and t.device != tensors[0].device for t in tensors):
+    if any(t is not None and t.device != first.device for t in tensors):
         raise ValueError(f"{what}: tensors on different devices")
-    _check_current(what, tensors[0])
+    _check_current(what, first)
+    return 0   # (of tensors that are on no GPU: only for checks without one)
+
+
+_CODES = (torch.float8_e4m3fn, torch.uint8)
+
+
+def _code_rows(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
+    """The row stride of a matrix of codes with quantize_e4m3's scales; its rows' alignment is the library's to check."""
+    n, k = codes.shape
+    if codes.dtype not in _CODES:
+        raise ValueError(f"{what}: {name} must be float8_e4m3fn or uint8 codes, not {codes.dtype}")
+    if scales.dtype is not torch.uint8 or scales.shape != ((k + 511) // 512, n, 4) or not scales.is_contiguous():
+        raise ValueError(f"{what}: {name}'s scales must be contiguous uint8 ({(k + 511) // 512}, {n}, 4): {tuple(scales.shape)}")
+    return _rows(codes)[1]
 
 
 def _new_codes(m: int, n: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
     return (torch.empty((m, n), dtype=torch.float8_e4m3fn, device=device),
-            torch.empty((-(-n // 512), m, 4), dtype=torch.uint8, device=device))
+            torch.empty(((n + 511) // 512, m, 4), dtype=torch.uint8, device=device))
 
 
 def dequantize_e4m3(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values (rows, K) that codes and scales of quantize_e4m3 (add_rmsnorm_e4m3, linear_e4m3_codes) stand for, rounded
     to dtype: float32 and bfloat16 hold each exactly, float16 what lies in its range (infinite above)."""
-    _check_device("dequantize_e4m3", codes, scales, out)
-    m, ldc = _rows(codes)
-    k = codes.shape[1]
+    stream = _stream_of("dequantize_e4m3", codes, scales, out)
+    m, k = codes.shape if codes.dim() == 2 else (0, 0)
     if k % 128 or k == 0:
-        raise ValueError(f"dequantize_e4m3: K {k} is not a multiple of 128")
-    _check_codes("dequantize_e4m3", "the matrix", codes, scales)
+        raise ValueError(f"dequantize_e4m3: {tuple(codes.shape)}: K is not a multiple of 128")
+    ldc = _code_rows("dequantize_e4m3", "the matrix", codes, scales)
+    code = DTYPE_CODE.get(dtype)
+    if code is None:
+        raise ValueError(f"dequantize_e4m3: dtype {dtype} (float32, bfloat16, float16)")
     if out is None:
         out = torch.empty((m, k), dtype=dtype, device=codes.device)
-    _, ldo = _rows(out)
-    if out.shape != (m, k) or out.dtype != dtype:
+    elif out.shape != codes.shape or out.dtype is not dtype:
         raise ValueError("dequantize_e4m3: out shape/dtype")
     if m:
-        check(_lib.load().fs_dequantize_e4m3(ptr(codes), ldc, ptr(scales), m, k, _dt(out), ptr(out), ldo, stream_ptr()),
-              "dequantize_e4m3")
+        check(_lib.load().fs_dequantize_e4m3(codes.data_ptr(), ldc, scales.data_ptr(), m, k, code, out.data_ptr(), _rows(out)[1],
+                                             stream), "dequantize_e4m3")
     return out
 
 
@@ -261,67 +276,84 @@ def add_rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: O
     (which may be x or delta). N is a multiple of 128. The norm is computed in float32 from the sum as rounded to x's dtype
     (float32, bfloat16, float16), and rounded once, to the code: a value is kept as quantize_e4m3 keeps it. A row whose
     squares' sum passes float32's range has zeros; of one with an infinite or NaN element that element, or all, are NaN."""
-    _check_device("add_rmsnorm_e4m3", x, weight, delta, x_out)
+    stream = _stream_of("add_rmsnorm_e4m3", x, weight, delta, x_out)
     m, ldx = _rows(x)
     n = x.shape[1]
+    dt = _dt(x)
     if n % 128 or n == 0:
         raise ValueError(f"add_rmsnorm_e4m3: N {n} is not a multiple of 128")
-    if weight.shape != (n,) or weight.dtype != x.dtype or not weight.is_contiguous():
+    if weight.shape != (n,) or weight.dtype is not x.dtype or not weight.is_contiguous():
         raise ValueError("add_rmsnorm_e4m3: weight shape/dtype")
-    ldd = ldxo = 0
+    ldd = ldxo = pd = pxo = 0
     if (delta is None) != (x_out is None):
         raise ValueError("add_rmsnorm_e4m3: delta needs x_out, and x_out delta")
     if delta is not None:
-        _, ldd = _rows(delta)
-        _, ldxo = _rows(x_out)
-        if any(t.shape != x.shape or t.dtype != x.dtype for t in (delta, x_out)):
+        if any(t.shape != x.shape or t.dtype is not x.dtype for t in (delta, x_out)):
             raise ValueError("add_rmsnorm_e4m3: delta or x_out shape/dtype")
-    dt = _dt(x)
+        ldd, ldxo, pd, pxo = _rows(delta)[1], _rows(x_out)[1], delta.data_ptr(), x_out.data_ptr()
     codes, scales = _new_codes(m, n, x.device)
     if m:
-        check(_lib.load().fs_add_rmsnorm_e4m3(ptr(x), ldx, ptr(delta), ldd, ptr(x_out), ldxo, ptr(weight), ptr(codes), n,
-                                              ptr(scales), m, n, float(eps), dt, stream_ptr()), "add_rmsnorm_e4m3")
+        check(_lib.load().fs_add_rmsnorm_e4m3(x.data_ptr(), ldx, pd, ldd, pxo, ldxo, weight.data_ptr(), codes.data_ptr(), n,
+                                              scales.data_ptr(), m, n, eps, dt, stream), "add_rmsnorm_e4m3")
     return codes, scales
 
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # FS_ACT_*
 
 
-def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, residual, out, out_scales) -> None:
-    m, lda = _rows(a)
-    n, ldb = _rows(w)
-    k = a.shape[1]
-    if k % 128 or k == 0 or w.shape[1] != k or n == 0 or (gated and n % 2):
+def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, residual, out, dtype):
+    """Both calls below: (out, None), or with dtype torch.float8_e4m3fn (codes, scales)."""
+    stream = _stream_of(what, a, w, w_scales, a_scales, bias, residual, out)
+    if a.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)}")
+    m, k = a.shape
+    rows = w.shape[0]
+    n = rows // 2 if gated else rows
+    if k % 128 or k == 0 or w.shape[1] != k or n == 0 or (gated and rows % 2):
         raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)} (K a multiple of 128, of a gated product an even "
                          "number of rows)")
-    _check_codes(what, "w", w, w_scales)
+    ldw = _code_rows(what, "w", w, w_scales)
     if a_scales is not None:
-        _check_codes(what, "a", a, a_scales)
-        x_dtype = 0
+        lda, pas, x_dtype = _code_rows(what, "a", a, a_scales), a_scales.data_ptr(), 0
     else:
-        if a.dtype not in DTYPE_CODE:
+        lda, pas, x_dtype = _rows(a)[1], 0, DTYPE_CODE.get(a.dtype)
+        if x_dtype is None:
             raise ValueError(f"{what}: rows of {a.dtype} (codes need a_scales)")
-        x_dtype = DTYPE_CODE[a.dtype]
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"{what}: activation {activation!r} (one of {', '.join(map(str, ACTIVATIONS))})")
-    bias_dtype = ldr = 0
+    bias_dtype = pb = ldr = pr = 0
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype not in DTYPE_CODE or (n > 1 and bias.stride(0) != 1):
-            raise ValueError(f"{what}: bias must be contiguous ({n},) in float32, bfloat16 or float16")
-        bias_dtype = DTYPE_CODE[bias.dtype]
-    if residual is not None:
-        _, ldr = _rows(residual)
-        if residual.shape != out.shape or residual.dtype != out.dtype:
-            raise ValueError(f"{what}: residual shape/dtype")
-    if m == 0:
-        return
-    lib = _lib.load()
-    call = _lib.Linear(ptr(a), ptr(a_scales), ptr(w), ptr(w_scales), ptr(bias), ptr(residual), ptr(out), ptr(out_scales), lda, ldb,
-                       ldr, out.stride(0), m, out.shape[1], k, x_dtype, DTYPE_CODE.get(out.dtype, 0), bias_dtype,
-                       ACTIVATIONS[activation], int(gated), 0)
-    need = lib.fs_linear_e4m3_workspace_size(call)
-    ws = _ws(need, a.device) if need else None   # (of the current stream: calls on two do not share it)
-    check(lib.fs_linear_e4m3(call, ptr(ws), need, stream_ptr()), what)
+        bias_dtype, pb = DTYPE_CODE.get(bias.dtype), bias.data_ptr()
+        if bias.shape != (rows,) or bias_dtype is None or not bias.is_contiguous():
+            raise ValueError(f"{what}: bias must be contiguous ({rows},) in float32, bfloat16 or float16")
+    scales = None
+    if dtype is torch.float8_e4m3fn:
+        if n % 128:
+            raise ValueError(f"{what}: {n} columns are not a multiple of 128")
+        out, scales = _new_codes(m, n, a.device)
+        ldo, pos = n, scales.data_ptr()
+    else:
+        pos = 0
+        if out is None:
+            out = torch.empty((m, n), dtype=dtype, device=a.device)
+            ldo = n
+        else:
+            ldo = _rows(out)[1]
+            if out.shape != (m, n) or out.dtype is not dtype:
+                raise ValueError(f"{what}: out shape/dtype")
+        if residual is not None:
+            if residual.shape != (m, n) or residual.dtype is not dtype:
+                raise ValueError(f"{what}: residual shape/dtype")
+            ldr, pr = _rows(residual)[1], residual.data_ptr()
+    if m:
+        lib = _lib.load()
+        call = _lib.Linear(a.data_ptr(), pas, w.data_ptr(), w_scales.data_ptr(), pb, pr, out.data_ptr(), pos, lda, ldw, ldr, ldo,
+                           m, n, k, x_dtype, DTYPE_CODE.get(dtype, 0), bias_dtype, act, 1 if gated else 0, 0)
+        need = lib.fs_linear_e4m3_workspace_size(call)
+        ws = _ws(need, a.device) if need else None   # (of the current stream: calls on two do not share it)
+        check(lib.fs_linear_e4m3(call, ws.data_ptr() if need else 0, need, stream), what)
+    return out, scales
 
 
 def linear_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scales: Optional[torch.Tensor] = None,
@@ -337,22 +369,12 @@ def linear_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scal
     bfloat16; the residual has the same. K is a multiple of 128. Sums as gemm_e4m3's, the rest in float32, rounded once. A
     row's last bit may depend on how many rows the call has. out may be the residual itself, but shares no memory with a
     or w."""
-    _check_device("linear_e4m3", a, w, w_scales, a_scales, bias, residual, out)
     if dtype is None:
-        dtype = next((t.dtype for t in (out, residual) if t is not None),
-                     a.dtype if a.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16)
-    if dtype not in (torch.bfloat16, torch.float16):
+        dtype = (out.dtype if out is not None else residual.dtype if residual is not None else
+                 a.dtype if a.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16)
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"linear_e4m3: results are bfloat16 or float16, not {dtype}")
-    if a.dim() != 2 or w.dim() != 2:
-        raise ValueError(f"linear_e4m3: {tuple(a.shape)} x {tuple(w.shape)}")
-    shape = (a.shape[0], w.shape[0] // 2 if gated else w.shape[0])
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=a.device)
-    _rows(out)
-    if out.shape != shape or out.dtype != dtype:
-        raise ValueError("linear_e4m3: out shape/dtype")
-    _linear_e4m3("linear_e4m3", a, w, w_scales, a_scales, bias, activation, gated, residual, out, None)
-    return out
+    return _linear_e4m3("linear_e4m3", a, w, w_scales, a_scales, bias, activation, gated, residual, out, dtype)[0]
 
 
 def linear_e4m3_codes(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scales: Optional[torch.Tensor] = None,
@@ -360,15 +382,7 @@ def linear_e4m3_codes(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, 
                       gated: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """linear_e4m3 with its result left in 8-bit floating point for the next product: (codes, scales) as quantize_e4m3 lays
     them out, rounded once. The result's columns are a multiple of 128."""
-    _check_device("linear_e4m3_codes", a, w, w_scales, a_scales, bias)
-    if a.dim() != 2 or w.dim() != 2:
-        raise ValueError(f"linear_e4m3_codes: {tuple(a.shape)} x {tuple(w.shape)}")
-    n = w.shape[0] // 2 if gated else w.shape[0]
-    if n % 128 or n == 0:
-        raise ValueError(f"linear_e4m3_codes: {n} columns are not a multiple of 128")
-    codes, scales = _new_codes(a.shape[0], n, a.device)
-    _linear_e4m3("linear_e4m3_codes", a, w, w_scales, a_scales, bias, activation, gated, None, codes, scales)
-    return codes, scales
+    return _linear_e4m3("linear_e4m3_codes", a, w, w_scales, a_scales, bias, activation, gated, None, None, torch.float8_e4m3fn)
 
 
 def gemm_add_rmsnorm(a: torch.Tensor, w: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor,

@@ -109,77 +109,58 @@ def operands(m, n, k, gated, dtype, seed=0, bias_dtype=None):
 # ------------------------------------------------------------------------------------------------
 # (m, n, k, gated, codes out) -> its plan; tiles that the rows and columns end inside of
 SIZES = {
-    # up to 16 rows: 16, 32 and 64 rows of W a workgroup
-    (1, 7, 128, False, False): (16, 16, 1, 0), (5, 530, 1152, False, False): (16, 16, 1, 0),
-    (16, 6145, 1024, False, False): (16, 32, 1, 0), (3, 9001, 640, False, False): (16, 64, 1, 0),
-    (1, 3, 128, True, False): (16, 32, 1, 0), (9, 2050, 896, True, False): (16, 32, 1, 0),
-    (16, 5003, 512, True, False): (16, 64, 1, 0),
-    (1, 128, 384, False, True): (16, 16, 1, 1), (13, 640, 4096, False, True): (16, 16, 1, 1),
-    (2, 6144, 256, False, True): (16, 32, 1, 1), (7, 1152, 2048, True, True): (16, 32, 1, 1),
-    (16, 14336, 512, True, True): (16, 64, 1, 1),
-    # tiles
-    (133, 2096, 16384, False, False): (256, 128, 8, 1),
-    (136, 4152, 16384, False, False): (256, 256, 8, 1),
-    (1, 8320, 128, False, True): (16, 64, 1, 1),
-    (131, 4224, 16384, False, True): (256, 256, 8, 1),
-    (131, 2112, 16384, True, False): (256, 256, 8, 1),
-    (17, 1, 128, False, False): (64, 64, 1, 0),
-    (17, 4, 5120, False, False): (64, 64, 2, 1),
-    (18, 4, 2048, False, False): (64, 64, 4, 1),
-    (18, 4, 4096, False, False): (64, 64, 8, 1),
-    (75, 8703, 128, False, False): (128, 128, 1, 0),
-    (24, 8740, 9216, False, False): (128, 128, 2, 1),
-    (20, 4212, 8192, False, False): (128, 128, 4, 1),
-    (2243, 4, 12288, False, False): (128, 128, 8, 1),
-    (392, 9127, 128, False, False): (256, 128, 1, 0),
-    (241, 9004, 15360, False, False): (256, 128, 2, 1),
-    (214, 5356, 14336, False, False): (256, 128, 4, 1),
-    (1026, 7613, 128, False, False): (256, 256, 1, 0),
-    (401, 8236, 10240, False, False): (256, 256, 2, 1),
-    (418, 5148, 12288, False, False): (256, 256, 4, 1),
-    (17, 128, 640, False, True): (64, 64, 1, 1),
-    (17, 128, 1024, False, True): (64, 64, 2, 1),
-    (17, 128, 2048, False, True): (64, 64, 4, 1),
-    (17, 128, 4096, False, True): (64, 64, 8, 1),
-    (17, 128, 128, False, True): (128, 128, 1, 0),
-    (17, 9216, 6144, False, True): (128, 128, 2, 1),
-    (18, 4480, 8192, False, True): (128, 128, 4, 1),
-    (73, 2304, 4096, False, True): (128, 128, 8, 1),
-    (422, 8704, 128, False, True): (256, 128, 1, 0),
-    (132, 9088, 9216, False, True): (256, 128, 2, 1),
-    (161, 4992, 10240, False, True): (256, 128, 4, 1),
-    (1230, 6656, 128, False, True): (256, 256, 1, 0),
-    (475, 8576, 9216, False, True): (256, 256, 2, 1),
-    (314, 5632, 12288, False, True): (256, 256, 4, 1),
-    (18, 1, 128, True, False): (64, 64, 1, 0),
-    (17, 4, 5120, True, False): (64, 64, 2, 1),
-    (17, 4, 2048, True, False): (64, 64, 4, 1),
-    (21, 4, 4096, True, False): (64, 64, 8, 1),
-    (21, 8309, 128, True, False): (128, 128, 1, 0),
-    (40, 4100, 8192, True, False): (128, 128, 2, 1),
-    (17, 3316, 8192, True, False): (128, 128, 4, 1),
-    (2065, 4, 12288, True, False): (128, 128, 8, 1),
-    (277, 6084, 128, True, False): (256, 128, 1, 0),
-    (141, 4604, 9216, True, False): (256, 128, 2, 1),
-    (293, 1492, 10240, True, False): (256, 128, 4, 1),
-    (518, 6557, 128, True, False): (256, 256, 1, 0),
-    (190, 8900, 14336, True, False): (256, 256, 2, 1),
-    (204, 5012, 12288, True, False): (256, 256, 4, 1),
-    (17, 128, 128, True, True): (64, 64, 1, 1),
-    (17, 128, 1024, True, True): (64, 64, 2, 1),
-    (17, 128, 2048, True, True): (64, 64, 4, 1),
-    (17, 128, 4096, True, True): (64, 64, 8, 1),
-    (26, 8320, 128, True, True): (128, 128, 1, 1),
-    (66, 4224, 1024, True, True): (128, 128, 2, 1),
-    (69, 2432, 2048, True, True): (128, 128, 4, 1),
-    (82, 1280, 8192, True, True): (128, 128, 8, 1),
-    (131, 8448, 1152, True, True): (256, 128, 1, 1),
-    (142, 4224, 4096, True, True): (256, 128, 2, 1),
-    (139, 2304, 8192, True, True): (256, 128, 4, 1),
-    (333, 2432, 128, True, True): (256, 256, 1, 0),
-    (170, 8832, 4096, True, True): (256, 256, 2, 1),
-    (129, 4224, 8192, True, True): (256, 256, 4, 1),
-    (135, 2176, 12288, True, True): (256, 256, 8, 1),
+    (5, 1, 512, False, False): (16, 16, 1, 0), (1, 7, 128, False, False): (16, 16, 1, 0),
+    (1, 3, 128, True, False): (16, 16, 1, 0), (5, 1, 512, True, False): (16, 16, 1, 0),
+    (5, 128, 512, False, True): (16, 16, 1, 1), (13, 640, 4096, False, True): (16, 16, 1, 1),
+    (5, 128, 512, True, True): (16, 16, 1, 1), (5, 4305, 512, False, False): (16, 32, 1, 0),
+    (5, 2441, 512, True, False): (16, 32, 1, 0), (9, 2050, 896, True, False): (16, 32, 1, 0),
+    (6, 4224, 512, False, True): (16, 32, 1, 1), (5, 2176, 512, True, True): (16, 32, 1, 1),
+    (5, 8444, 512, False, False): (16, 64, 1, 0), (5, 4420, 512, True, False): (16, 64, 1, 0),
+    (16, 5003, 512, True, False): (16, 64, 1, 0), (6, 8448, 512, False, True): (16, 64, 1, 1),
+    (6, 4352, 512, True, True): (16, 64, 1, 1), (5, 16852, 512, False, False): (16, 112, 1, 0),
+    (5, 8954, 512, True, False): (16, 112, 1, 0), (5, 17024, 640, False, True): (16, 112, 1, 1),
+    (16, 14336, 512, True, True): (16, 112, 1, 1), (5, 8704, 512, True, True): (16, 112, 1, 1),
+    (31, 1537, 640, False, False): (32, 16, 1, 0), (17, 1, 512, False, False): (32, 16, 1, 0),
+    (17, 1, 512, True, False): (32, 16, 1, 0), (17, 128, 512, False, True): (32, 16, 1, 1),
+    (17, 128, 512, True, True): (32, 16, 1, 1), (17, 4443, 512, False, False): (32, 32, 1, 0),
+    (19, 2097, 512, True, False): (32, 32, 1, 0), (17, 4864, 512, False, True): (32, 32, 1, 1),
+    (17, 2432, 512, True, True): (32, 32, 1, 1), (17, 9604, 512, False, False): (32, 64, 1, 0),
+    (17, 4204, 512, True, False): (32, 64, 1, 0), (18, 8576, 512, False, True): (32, 64, 1, 1),
+    (20, 4224, 512, True, True): (32, 64, 1, 1), (17, 17300, 512, False, False): (32, 112, 1, 0),
+    (19, 8301, 512, True, False): (32, 112, 1, 0), (17, 16640, 512, False, True): (32, 112, 1, 1),
+    (19, 9088, 512, True, True): (32, 112, 1, 1), (34, 1, 512, False, False): (64, 64, 1, 0),
+    (33, 1, 512, True, False): (64, 64, 1, 0), (33, 128, 640, False, True): (64, 64, 1, 1),
+    (33, 128, 512, True, True): (64, 64, 1, 1), (38, 4, 5120, False, False): (64, 64, 2, 1),
+    (33, 128, 1024, False, True): (64, 64, 2, 1), (35, 4, 5120, True, False): (64, 64, 2, 1),
+    (33, 128, 1024, True, True): (64, 64, 2, 1), (33, 4, 2048, False, False): (64, 64, 4, 1),
+    (33, 128, 2048, False, True): (64, 64, 4, 1), (33, 4, 2048, True, False): (64, 64, 4, 1),
+    (33, 128, 2048, True, True): (64, 64, 4, 1), (33, 4, 4096, False, False): (64, 64, 8, 1),
+    (33, 128, 4096, False, True): (64, 64, 8, 1), (33, 4, 4096, True, False): (64, 64, 8, 1),
+    (33, 128, 4096, True, True): (64, 64, 8, 1), (66, 8316, 512, False, False): (128, 128, 1, 0),
+    (33, 128, 512, False, True): (128, 128, 1, 0), (67, 4187, 512, True, False): (128, 128, 1, 0),
+    (66, 4224, 512, True, True): (128, 128, 1, 1), (72, 8204, 4096, False, False): (128, 128, 2, 1),
+    (34, 9088, 4096, False, True): (128, 128, 2, 1), (35, 4284, 8192, True, False): (128, 128, 2, 1),
+    (71, 4480, 1024, True, True): (128, 128, 2, 1), (69, 4420, 4096, False, False): (128, 128, 4, 1),
+    (68, 4864, 2048, False, True): (128, 128, 4, 1), (73, 2124, 4096, True, False): (128, 128, 4, 1),
+    (75, 2304, 2048, True, True): (128, 128, 4, 1), (2318, 4, 12288, False, False): (128, 128, 8, 1),
+    (65, 2304, 4096, False, True): (128, 128, 8, 1), (2085, 4, 16384, True, False): (128, 128, 8, 1),
+    (68, 1152, 4096, True, True): (128, 128, 8, 1), (148, 16385, 512, False, False): (256, 128, 1, 0),
+    (133, 17280, 512, False, True): (256, 128, 1, 0), (136, 9354, 512, True, False): (256, 128, 1, 0),
+    (150, 8448, 1536, True, True): (256, 128, 1, 1), (131, 11364, 15360, False, False): (256, 128, 2, 1),
+    (158, 10496, 15360, False, True): (256, 128, 2, 1), (266, 3260, 11264, True, False): (256, 128, 2, 1),
+    (135, 4224, 4096, True, True): (256, 128, 2, 1), (177, 4164, 10240, False, False): (256, 128, 4, 1),
+    (142, 4224, 8192, False, True): (256, 128, 4, 1), (155, 2180, 10240, True, False): (256, 128, 4, 1),
+    (146, 2176, 8192, True, True): (256, 128, 4, 1), (146, 2188, 16384, False, False): (256, 128, 8, 1),
+    (130, 2432, 16384, False, True): (256, 128, 8, 1), (2119, 72, 16384, True, False): (256, 128, 8, 1),
+    (129, 1152, 16384, True, True): (256, 128, 8, 1), (569, 13171, 512, False, False): (256, 256, 1, 0),
+    (395, 17024, 512, False, True): (256, 256, 1, 0), (152, 17738, 512, True, False): (256, 256, 1, 0),
+    (33, 17152, 512, True, True): (256, 256, 1, 0), (166, 17036, 8192, False, False): (256, 256, 2, 1),
+    (143, 16512, 8192, False, True): (256, 256, 2, 1), (258, 5508, 8192, True, False): (256, 256, 2, 1),
+    (142, 8576, 4096, True, True): (256, 256, 2, 1), (155, 8300, 8192, False, False): (256, 256, 4, 1),
+    (130, 8320, 8192, False, True): (256, 256, 4, 1), (141, 4956, 10240, True, False): (256, 256, 4, 1),
+    (132, 4608, 8192, True, True): (256, 256, 4, 1), (140, 4236, 16384, False, False): (256, 256, 8, 1),
+    (136, 4352, 16384, False, True): (256, 256, 8, 1), (131, 2060, 16384, True, False): (256, 256, 8, 1),
+    (131, 2176, 16384, True, True): (256, 256, 8, 1),
 }
 
 

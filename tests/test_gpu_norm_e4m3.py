@@ -22,7 +22,7 @@ def values(codes, scales):
 
 def check(codes, scales, v, w, eps):
     """codes against the norm of v (CPU, in its type). The kernel's r: a sum of squares of at most 40 additions in a thread and
-    20 across them, a mean, a root and a quotient, then two products: 64 roundings of 2^-24 together at most, 2^-18. A code
+    40 across them (half of them between sums of 512 columns), a mean, a root and a quotient, then two products: 64 roundings of 2^-24 at most with the halving by the root, 2^-18. A code
     is off by half a step, 2^-4 of the value or 2^-10 of the scale, which is at most 2 / 448 of the group's largest."""
     m, n = v.shape
     assert codes.shape == (m, n) and codes.dtype == torch.float8_e4m3fn and scales.shape == (-(-n // 512), m, 4)
@@ -72,11 +72,13 @@ def test_norm(dtype, m, n):
             over.copy_(keep)
 
 
-@pytest.mark.parametrize("n", [384, 1024, 4096, 16512])
+@pytest.mark.parametrize("n", [384, 1024, 2048, 2176, 4096, 8192, 14336, 16512])
 def test_a_row_does_not_depend_on_its_batch(n):
+    """Short batches and long ones, whose threads hold other pieces of a row."""
     x, _, w = (t.to(DEV) for t in rows(37, n, BF16, n))
+    x = x.repeat(40, 1)
     codes, scales = ops.add_rmsnorm_e4m3(x, w, 1e-5)
-    for i in (0, 20, 36):
+    for i in (0, 20, 36, 1400):
         c, s = ops.add_rmsnorm_e4m3(x[i: i + 1], w, 1e-5)
         assert torch.equal(c.view(torch.uint8), codes[i: i + 1].view(torch.uint8)) and torch.equal(s[:, 0], scales[:, i])
 
