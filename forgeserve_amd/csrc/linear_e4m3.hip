@@ -11,7 +11,11 @@
 
 namespace {
 
-constexpr int STREAM_ROWS = 32;   // rows that the kernels without tiles in LDS take
+// Rows that the kernels without tiles in LDS may take, and, of more than 32, their codes: every workgroup reads them, for one
+// or two tiles of W (64 x 4096 x 4096 8.2 us, in tiles 11.9; 128 x 6144 x 4096 13.5 and 14.5; 64 x 2048 x 8192 10.3 and 13.2;
+// over the limit 64 x 4096 x 14336 24.4 and 19.8, 96 x 2048 x 8192 14.6 and 13.5; four tiles, 64 x 16384 x 2048, 11.1 and 9.8).
+constexpr int STREAM_ROWS = 128;
+constexpr int64_t STREAM_BYTES = 600 * 1024;
 
 // ------------------------------------------------------------------------------------------------
 // what is done with the sums
@@ -210,74 +214,136 @@ __global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __re
 }
 
 // ------------------------------------------------------------------------------------------------
-// up to 32 rows: bound by the weight's bytes
+// short batches: bound by the weight's bytes
 // ------------------------------------------------------------------------------------------------
 // A workgroup takes `per` rows of W (of a gated product `per` columns of the results: as many rows of each half), so many
 // that the grid is one round of the CUs where it can be and each draws the same share; its eight waves split K and are joined
-// in order through LDS. Codes of both operands go straight to registers in the instruction's own shape, DEPTH stages ahead: W's
-// from HBM, x's (16 TM rows, the same for every workgroup, read once for TN tiles of W) from L2. A tile is 16 rows of W, or
-// eight columns' gate's rows and their others', so that any number of tiles may share a workgroup.
-template <class OUT, int TM, int TN, int DEPTH>
+// in order through LDS. A tile is 16 rows of W, or eight columns' gate's rows and their others', so that any number of tiles
+// may share a workgroup, and x's codes. A wave streams its part of K on its own, without a barrier: pieces of 16 rows x 128
+// codes, in each stage x's TM and then W's TN, pass through the wave's SLOTS places in LDS, copied there by whole lines SLOTS
+// pieces ahead: 16 KB a wave, 128 KB a CU on their way. With many rows a workgroup the waves take stages in turn, so that they
+// read a row's next 1 KB together (1 x 28672 x 4096 gated 26.7 -> 25.6 us); with few, eight parts of K, whose words of four
+// stages' scales serve them all (1 x 2048 x 8192 7.1 -> 6.3 us).
+//
+// Straight to registers, in the instruction's own shape, a load runs at a quarter of the rate, 38 GB/s a CU from L2 for 150,
+// for four lanes side by side are four rows: 8 x 6144 x 4096 took 8.6 us so and takes 7.3, 32 x 4096 x 4096 9.8 and 7.1. Now
+// HBM bounds it: 1 x 28672 x 4096 in 25.6 us, 2.3 of them the launch, draws 5.0 TB/s, 1 x 128256 x 4096 5.4; smaller weights
+// are on their way before the CUs' 128 KB each have come (4096 x 4096 in 6.6 us).
+template <class OUT, int TM, int TN>
 __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT out, int per) {
   constexpr int TILES = TM * TN, CH = TILES < 8 ? TILES : 8, COLS = OUT::GATED ? 8 : 16;
-  __shared__ float4_t red[8][CH][64];
+  constexpr int SLOTS = 8, PIECE = 16 * GROUP, PPS = TM + TN;   // pieces a stage
+  constexpr int XQ = (16 * TM + 63) / 64, WQ = (16 * TN + 63) / 64, WORDS = 64 * (XQ + WQ);   // a stage's words: x's rows, W's
+  constexpr bool TURNS = TN >= 4;
+  // Places for words: of the stages that SLOTS pieces reach ahead, or of fours of them, four ahead at most.
+  constexpr int PLACES = TURNS && (PPS - 1 + SLOTS) / PPS > 1 ? 4 : 2;
+  static_assert(PPS >= 2 && (!TURNS || (PPS - 1 + SLOTS) / PPS < PLACES), "words stay until they are used");
+  __shared__ __attribute__((aligned(1024))) char ring[8][SLOTS * PIECE];
+  __shared__ __attribute__((aligned(256))) uint32_t words[8][PLACES][WORDS];
+  static_assert(sizeof(ring) >= 8 * CH * 64 * sizeof(float4_t), "the sums take the ring's place");
+  typedef __attribute__((address_space(3))) const u32x4 LdsFrag;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N, c0 = (int64_t)blockIdx.x * per, c1 = min(c0 + per, cols);
-  const int k0 = (int)((int64_t)w * P.nk / 8), k1 = (int)((int64_t)(w + 1) * P.nk / 8);
+  // the wave's stages: w, w + 8, ..., or the w-th eighth
+  const int k0 = TURNS ? w : (int)((int64_t)w * P.nk / 8);
+  const int ni = TURNS ? (P.nk - w + 7) / 8 : (int)((int64_t)(w + 1) * P.nk / 8) - k0;
+  auto stage_of = [&](int i) { return TURNS ? w + 8 * i : k0 + i; };
+  auto has_words = [&](int i) { return TURNS || i == 0 || (stage_of(i) & 3) == 0; };
+  auto place_of = [&](int i) { return (TURNS ? i : stage_of(i) >> 2) & (PLACES - 1); };
   const int M = (int)P.M;
-  struct Stage {
-    u32x4 c[TN][2], x[TM][2];
-    uint32_t s[TN], xs[TM];
-  } ring[DEPTH];
-  const uint8_t* xp[TM];
-  int xrow[TM];
+
+  // copies: 8 rows of 128 bytes each; lane l takes row l >> 3, physical chunk l & 7 of it (swap_of)
+  const uint32_t slots = (uint32_t)(uintptr_t)ring[w], words0 = (uint32_t)(uintptr_t)words[w];
+  const char* xbase = reinterpret_cast<const char*>(P.x);
+  const char* wbase[2];
+  uint32_t xoff[TM][2], woff[TN][2];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {   // (lanes past the last row: results nobody stores)
-    xrow[i] = min(16 * i + l16, M - 1);
-    xp[i] = P.x + xrow[i] * P.ldx + 16 * g;
+  for (int h = 0; h < 2; ++h) {
+    const int row = 8 * h + (lane >> 3), c = 16 * ((lane & 7) ^ swap_of(row));
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xoff[i][h] = (uint32_t)(min(16 * i + row, M - 1) * P.ldx + c);   // (rows past the last: nobody's)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      woff[j][h] = (uint32_t)((min(c0 + COLS * j + (OUT::GATED ? row & 7 : row), c1 - 1) - c0) * P.ldw + c);
+    wbase[h] = reinterpret_cast<const char*>(P.w + (c0 + (OUT::GATED && h ? cols : 0)) * P.ldw);
   }
-  const uint8_t* wrow[TN];
-  int64_t srow[TN];
+  uint32_t wword[WQ];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int64_t c = min(c0 + COLS * j + (OUT::GATED ? l16 & 7 : l16), c1 - 1), n = OUT::GATED && l16 >= 8 ? c + cols : c;
-    wrow[j] = P.w + n * P.ldw + 16 * g;
-    srow[j] = 4 * n;
+  for (int q = 0; q < WQ; ++q) {
+    const int r = min(64 * q + lane, 16 * TN - 1);
+    const int64_t c = min(c0 + COLS * (r >> 4) + (OUT::GATED ? r & 7 : r & 15), c1 - 1);
+    wword[q] = (uint32_t)(4 * (OUT::GATED && (r & 8) ? c + cols : c));
   }
-  auto load = [&](int k, Stage& x) {
+  uint32_t xword[XQ];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      x.c[j][0] = *reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP);
-      x.c[j][1] = *reinterpret_cast<const u32x4*>(wrow[j] + (int64_t)k * GROUP + 64);
-      x.s[j] = P.ws[(int64_t)(k >> 2) * 4 * P.N + srow[j] + (k & 3)];
+  for (int q = 0; q < XQ; ++q) xword[q] = (uint32_t)(4 * min(64 * q + lane, M - 1));
+  int slot = 0;   // of the stage's first piece
+  // piece t of the wave's stage i into place (slot + at) % SLOTS; ahead of a stage's first, its words
+  auto copy = [&](int i, int t, int at) {
+    const int64_t k = stage_of(i);
+    const uint32_t to = slots + (uint32_t)(((slot + at) & (SLOTS - 1)) * PIECE);
+    if (t == 0 && has_words(i)) {
+      const uint32_t wto = words0 + (uint32_t)(place_of(i) * WORDS * 4);
+#pragma unroll
+      for (int q = 0; q < XQ; ++q) dma4_at(P.xs + (k >> 2) * 4 * M, xword[q], wto + 256 * q);
+#pragma unroll
+      for (int q = 0; q < WQ; ++q) dma4_at(P.ws + (k >> 2) * 4 * P.N, wword[q], wto + 256 * (XQ + q));
     }
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      x.x[i][0] = *reinterpret_cast<const u32x4*>(xp[i] + (int64_t)k * GROUP);
-      x.x[i][1] = *reinterpret_cast<const u32x4*>(xp[i] + (int64_t)k * GROUP + 64);
-      x.xs[i] = P.xs[((int64_t)(k >> 2) * M + xrow[i]) * 4 + (k & 3)];
+    for (int h = 0; h < 2; ++h) {
+      if (t < TM) dma16_at(xbase + k * GROUP, xoff[t < TM ? t : 0][h], to + 1024 * h);
+      else dma16_at(wbase[h] + k * GROUP, woff[t < TM ? 0 : t - TM][h], to + 1024 * h);
     }
   };
+  const uint32_t at0 = (uint32_t)(l16 * GROUP + 16 * (g ^ swap_of(l16))), at1 = (uint32_t)(l16 * GROUP + 16 * ((4 + g) ^ swap_of(l16)));
+  // piece t of stage i from its place, once it has landed (SLOTS - 1 pieces may be behind it), and the next into it
+  auto take = [&](int i, int t) {
+    if (i + (t + SLOTS - 1) / PPS < ni) wait_vm<2 * (SLOTS - 1)>();
+    else wait_vm<0>();
+    const uint32_t from = slots + (uint32_t)(((slot + t) & (SLOTS - 1)) * PIECE);
+    const i32x8 f = both_chunks(*(LdsFrag*)(uintptr_t)(from + at0), *(LdsFrag*)(uintptr_t)(from + at1));
+    if (i + (t + SLOTS) / PPS < ni) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      copy(i + (t + SLOTS) / PPS, (t + SLOTS) % PPS, t + SLOTS);
+    }
+    return f;
+  };
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (k0 + d < k1) load(k0 + d, ring[d]);
+  for (int t = 0; t < SLOTS; ++t)
+    if (t / PPS < ni) copy(t / PPS, t % PPS, t);
   float4_t acc[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-  for (int kt = k0; kt < k1; kt += DEPTH) {
+  uint32_t xs[TM], ws[TN];
+  for (int i = 0; i < ni; ++i) {
+    i32x8 xf[TM];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      if (kt + d >= k1) break;   // (wave-uniform)
+    for (int r = 0; r < TM; ++r) xf[r] = take(i, r);
+    if (has_words(i)) {   // (landed before x's first piece)
+      const uint32_t* p = words[w][place_of(i)];
+      const int shift = 8 * (stage_of(i) & 3);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int r = 0; r < TM; ++r) xs[r] = p[16 * r + l16] >> shift;
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i * TN + j] = mfma_codes<0>(both_chunks(ring[d].c[j][0], ring[d].c[j][1]), both_chunks(ring[d].x[i][0], ring[d].x[i][1]),
-                                          acc[i * TN + j], ring[d].s[j], ring[d].xs[i]);
-      if (kt + d + DEPTH < k1) load(kt + d + DEPTH, ring[d]);
+      for (int j = 0; j < TN; ++j) ws[j] = p[64 * XQ + 16 * j + l16] >> shift;
     }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const i32x8 wf = take(i, TM + j);
+#pragma unroll
+      for (int r = 0; r < TM; ++r) acc[r * TN + j] = mfma_codes<0>(wf, xf[r], acc[r * TN + j], ws[j], xs[r]);
+    }
+    if (!TURNS) {
+#pragma unroll
+      for (int r = 0; r < TM; ++r) xs[r] >>= 8;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) ws[j] >>= 8;
+    }
+    slot = (slot + PPS) & (SLOTS - 1);
   }
+  __syncthreads();   // every wave has read its last pieces, and no copy is on its way
+  float4_t(*red)[CH][64] = reinterpret_cast<float4_t(*)[CH][64]>(&ring[0][0]);
   // CH tiles at a time: wave t joins tile t's eight sums in order; lane (l16, g) has row l16, and of the tile's rows of W
   // (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
 #pragma unroll
@@ -312,7 +378,8 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
 // ------------------------------------------------------------------------------------------------
 struct Plan {
   int bm, bn, splits;
-  bool join;   // through memory
+  bool join;     // the sums through memory
+  bool stream;   // no tiles in LDS
 };
 int64_t weight_rows(const fs_linear& c) { return c.gated ? 2 * c.N : c.N; }
 
@@ -333,14 +400,15 @@ Plan plan_for(const fs_linear& c) {
   const int64_t M = c.M, N = weight_rows(c), nk = c.K / GROUP;
   if (M <= STREAM_ROWS) {
     const int tiles = c.out_scales ? stream_tiles(N, false) : stream_tiles(c.N, c.gated != 0);
-    return Plan{M <= 16 ? 16 : 32, 16 * tiles, 1, c.out_scales != nullptr};
+    const int rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    if (rows <= 32 || (tiles <= 2 && rows * c.K <= STREAM_BYTES)) return Plan{rows, 16 * tiles, 1, c.out_scales != nullptr, true};
   }
   struct Cand {
     int bm, bn;
     double stage, fixed;
   };
   static const Cand cands[] = {{64, 64, 0.43, 3.0}, {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0}, {256, 256, 1.5, 10.0}};
-  Plan best{64, 64, 1, c.out_scales != nullptr};
+  Plan best{64, 64, 1, c.out_scales != nullptr, false};
   double least = 1e30;
   for (const Cand& t : cands) {
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -352,7 +420,7 @@ Plan plan_for(const fs_linear& c) {
       if (join && (N % 4 != 0 || (c.gated && c.N % 4 != 0))) break;
       const double us = (double)((tiles * s + 255) / 256) * ((double)(nk / s) * t.stage + t.fixed) +
                         (join ? 3.0 + (double)s * (double)M * (double)N * 8.0 / 4.5e6 : 0.0);
-      if (us < least) least = us, best = Plan{t.bm, t.bn, s, join};
+      if (us < least) least = us, best = Plan{t.bm, t.bn, s, join, false};
     }
   }
   return best;
@@ -363,21 +431,23 @@ int64_t sums_bytes(const fs_linear& c, const Plan& p) {
   return p.join ? (int64_t)p.splits * c.M * weight_rows(c) * (int64_t)sizeof(float) : 0;
 }
 
-// DEPTH stages of TN tiles each: 14 to 16 KB of W on their way a wave, less where the registers are the sums'.
 template <class OUT, int TM>
 void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
   const dim3 grid((unsigned)((cols + per - 1) / per));
-  if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1, TM == 1 ? 7 : 4><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2, TM == 1 ? 4 : 3><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else linear_e4m3_stream_kernel<OUT, TM, 7, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
+  if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else if constexpr (TM > 2) return;   // (not planned)
+  else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per);
+  else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per);
 }
 template <class OUT>
 void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
   const int tn = p.bn / 16;
   if (p.bm == 16) launch_stream<OUT, 1>(P, out, tn, per, s);
-  else launch_stream<OUT, 2>(P, out, tn, per, s);
+  else if (p.bm == 32) launch_stream<OUT, 2>(P, out, tn, per, s);
+  else if (p.bm == 64) launch_stream<OUT, 4>(P, out, tn, per, s);
+  else launch_stream<OUT, 8>(P, out, tn, per, s);
 }
 
 // PARTS: a class of which only the sums in memory are asked for.
@@ -395,7 +465,6 @@ void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t 
 
 template <class OUT>
 int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t s) {
-  const bool stream = c.M <= STREAM_ROWS;
   OUT out;
   out.C = reinterpret_cast<uint16_t*>(c.out);
   out.ldc = c.ldo;
@@ -415,13 +484,13 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
     typedef LinearOut<false, false> Sums;
     Sums sums{};
     sums.part = part;
-    if (stream) launch_stream(P, sums, p, stream_columns(P.N, false), s);   // (rows of W in their order, gated or not)
+    if (p.stream) launch_stream(P, sums, p, stream_columns(P.N, false), s);   // (rows of W in their order, gated or not)
     else launch_tiles<Sums, true>(P, sums, p, s);
     const uint32_t pieces = (uint32_t)((c.N + 7) / 8);
     linear_e4m3_join_kernel<OUT><<<dim3((unsigned)((c.M * pieces + 255) / 256)), 256, 0, s>>>(part, p.splits, P.M, P.N, pieces,
                                                                                              out);
   } else if constexpr (!OUT::CODES) {
-    if (stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
+    if (p.stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
     else launch_tiles<OUT, false>(P, out, p, s);
   } else {
     launch_tiles<OUT, false>(P, out, p, s);

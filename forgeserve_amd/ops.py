@@ -229,6 +229,13 @@ def _stream_of(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) 
     return 0   # (of tensors that are on no GPU: only for checks without one)
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    strides = t.stride()
+    if len(strides) != 2 or (strides[1] != 1 and t.shape[1] > 1):
+        raise ValueError(f"expected a 2-D tensor with a contiguous last dim, got {tuple(t.shape)} {strides}")
+    return strides[0]
+
+
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 
 
@@ -239,7 +246,7 @@ def _code_rows(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor) 
         raise ValueError(f"{what}: {name} must be float8_e4m3fn or uint8 codes, not {codes.dtype}")
     if scales.dtype is not torch.uint8 or scales.shape != ((k + 511) // 512, n, 4) or not scales.is_contiguous():
         raise ValueError(f"{what}: {name}'s scales must be contiguous uint8 ({(k + 511) // 512}, {n}, 4): {tuple(scales.shape)}")
-    return _rows(codes)[1]
+    return _row_stride(codes)
 
 
 def _new_codes(m: int, n: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -260,12 +267,14 @@ def dequantize_e4m3(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
     if code is None:
         raise ValueError(f"dequantize_e4m3: dtype {dtype} (float32, bfloat16, float16)")
     if out is None:
-        out = torch.empty((m, k), dtype=dtype, device=codes.device)
+        out, ldo = torch.empty((m, k), dtype=dtype, device=codes.device), k
     elif out.shape != codes.shape or out.dtype is not dtype:
         raise ValueError("dequantize_e4m3: out shape/dtype")
+    else:
+        ldo = _row_stride(out)
     if m:
-        check(_lib.load().fs_dequantize_e4m3(codes.data_ptr(), ldc, scales.data_ptr(), m, k, code, out.data_ptr(), _rows(out)[1],
-                                             stream), "dequantize_e4m3")
+        check(_lib.load().fs_dequantize_e4m3(codes.data_ptr(), ldc, scales.data_ptr(), m, k, code, out.data_ptr(), ldo, stream),
+              "dequantize_e4m3")
     return out
 
 
@@ -277,20 +286,21 @@ def add_rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: O
     (float32, bfloat16, float16), and rounded once, to the code: a value is kept as quantize_e4m3 keeps it. A row whose
     squares' sum passes float32's range has zeros; of one with an infinite or NaN element that element, or all, are NaN."""
     stream = _stream_of("add_rmsnorm_e4m3", x, weight, delta, x_out)
-    m, ldx = _rows(x)
-    n = x.shape[1]
-    dt = _dt(x)
-    if n % 128 or n == 0:
-        raise ValueError(f"add_rmsnorm_e4m3: N {n} is not a multiple of 128")
-    if weight.shape != (n,) or weight.dtype is not x.dtype or not weight.is_contiguous():
+    ldx = _row_stride(x)
+    m, n = x.shape
+    dtype = x.dtype
+    dt = DTYPE_CODE.get(dtype)
+    if n % 128 or n == 0 or dt is None:
+        raise ValueError(f"add_rmsnorm_e4m3: {tuple(x.shape)} {dtype} (N a multiple of 128; float32, bfloat16, float16)")
+    if weight.shape != (n,) or weight.dtype is not dtype or not weight.is_contiguous():
         raise ValueError("add_rmsnorm_e4m3: weight shape/dtype")
     ldd = ldxo = pd = pxo = 0
     if (delta is None) != (x_out is None):
         raise ValueError("add_rmsnorm_e4m3: delta needs x_out, and x_out delta")
     if delta is not None:
-        if any(t.shape != x.shape or t.dtype is not x.dtype for t in (delta, x_out)):
+        if delta.shape != (m, n) or x_out.shape != (m, n) or delta.dtype is not dtype or x_out.dtype is not dtype:
             raise ValueError("add_rmsnorm_e4m3: delta or x_out shape/dtype")
-        ldd, ldxo, pd, pxo = _rows(delta)[1], _rows(x_out)[1], delta.data_ptr(), x_out.data_ptr()
+        ldd, ldxo, pd, pxo = _row_stride(delta), _row_stride(x_out), delta.data_ptr(), x_out.data_ptr()
     codes, scales = _new_codes(m, n, x.device)
     if m:
         check(_lib.load().fs_add_rmsnorm_e4m3(x.data_ptr(), ldx, pd, ldd, pxo, ldxo, weight.data_ptr(), codes.data_ptr(), n,
@@ -307,16 +317,16 @@ def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, r
     if a.dim() != 2 or w.dim() != 2:
         raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)}")
     m, k = a.shape
-    rows = w.shape[0]
+    rows, wk = w.shape
     n = rows // 2 if gated else rows
-    if k % 128 or k == 0 or w.shape[1] != k or n == 0 or (gated and rows % 2):
+    if k % 128 or k == 0 or wk != k or n == 0 or (gated and rows % 2):
         raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)} (K a multiple of 128, of a gated product an even "
                          "number of rows)")
     ldw = _code_rows(what, "w", w, w_scales)
     if a_scales is not None:
         lda, pas, x_dtype = _code_rows(what, "a", a, a_scales), a_scales.data_ptr(), 0
     else:
-        lda, pas, x_dtype = _rows(a)[1], 0, DTYPE_CODE.get(a.dtype)
+        lda, pas, x_dtype = _row_stride(a), 0, DTYPE_CODE.get(a.dtype)
         if x_dtype is None:
             raise ValueError(f"{what}: rows of {a.dtype} (codes need a_scales)")
     act = ACTIVATIONS.get(activation)
@@ -339,19 +349,19 @@ def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, r
             out = torch.empty((m, n), dtype=dtype, device=a.device)
             ldo = n
         else:
-            ldo = _rows(out)[1]
+            ldo = _row_stride(out)
             if out.shape != (m, n) or out.dtype is not dtype:
                 raise ValueError(f"{what}: out shape/dtype")
         if residual is not None:
             if residual.shape != (m, n) or residual.dtype is not dtype:
                 raise ValueError(f"{what}: residual shape/dtype")
-            ldr, pr = _rows(residual)[1], residual.data_ptr()
+            ldr, pr = _row_stride(residual), residual.data_ptr()
     if m:
         lib = _lib.load()
         call = _lib.Linear(a.data_ptr(), pas, w.data_ptr(), w_scales.data_ptr(), pb, pr, out.data_ptr(), pos, lda, ldw, ldr, ldo,
                            m, n, k, x_dtype, DTYPE_CODE.get(dtype, 0), bias_dtype, act, 1 if gated else 0, 0)
         need = lib.fs_linear_e4m3_workspace_size(call)
-        ws = _ws(need, a.device) if need else None   # (of the current stream: calls on two do not share it)
+        ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None   # (of this stream alone)
         check(lib.fs_linear_e4m3(call, ws.data_ptr() if need else 0, need, stream), what)
     return out, scales
 
