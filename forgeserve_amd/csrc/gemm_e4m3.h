@@ -34,8 +34,8 @@ FS_DEVICE int swap_of(int row) { return (row >> 1) & 7; }
 // What finishes results, a class of which a kernel gets an instance:
 //   GATED          a tile's columns are half gate's (rows 0 .. N/2 - 1 of W), half the others' (N/2 .. N - 1), and the
 //                  results have N/2 columns
-//   STAGED         a finished tile's sums go through LDS as floats, eight columns a thread: out.piece(v, up, row, col,
-//                  cols); else from the registers, rounded first
+//   STAGED         a finished tile's sums go through LDS as floats, eight columns a thread: out.piece<WHOLE>(v, up, row,
+//                  col, cols), WHOLE being out.whole; else from the registers, rounded first
 //   finish(a, row, col0, cols)   four columns' sums, from col0 on, to what is rounded and stored (`cols`: how many there
 //                  are), and store(a, row, col0, cols) that
 //   part           not null: the f32 sums as they are, [split][M][N], instead
@@ -76,8 +76,8 @@ FS_DEVICE void put4(const OUT& out, float4_t a, int64_t row, int64_t col0, int64
 
 // A finished tile of ROWS x COLS sums in LDS, PITCH floats a row (where gated the gate's columns, then the others'):
 // finished by all of the workgroup's THREADS, eight columns of the results at a time, row by row.
-template <class OUT, int ROWS, int COLS, int PITCH, int THREADS>
-FS_DEVICE void finish_tile(const OUT& out, const float* sums, int tid, int64_t m0, int64_t M, int64_t c0, int64_t cols) {
+template <class OUT, bool WHOLE, int ROWS, int COLS, int PITCH, int THREADS>
+FS_DEVICE void finish_pieces(const OUT& out, const float* sums, int tid, int64_t m0, int64_t M, int64_t c0, int64_t cols) {
   constexpr int OC = OUT::GATED ? COLS / 2 : COLS, PIECES = OC / 8;
   static_assert(ROWS * PIECES % THREADS == 0 && PITCH % 4 == 0, "whole rounds");
 #pragma unroll 1
@@ -92,8 +92,13 @@ FS_DEVICE void finish_tile(const OUT& out, const float* sums, int tid, int64_t m
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[4 * h + e] = a[e], up[4 * h + e] = b[e];
     }
-    if (m0 + r < M && c0 + 8 * p < cols) out.piece(v, up, m0 + r, c0 + 8 * p, cols);
+    if (m0 + r < M && c0 + 8 * p < cols) out.template piece<WHOLE>(v, up, m0 + r, c0 + 8 * p, cols);
   }
+}
+template <class OUT, int ROWS, int COLS, int PITCH, int THREADS>
+FS_DEVICE void finish_tile(const OUT& out, const float* sums, int tid, int64_t m0, int64_t M, int64_t c0, int64_t cols) {
+  if (out.whole) finish_pieces<OUT, true, ROWS, COLS, PITCH, THREADS>(out, sums, tid, m0, M, c0, cols);
+  else finish_pieces<OUT, false, ROWS, COLS, PITCH, THREADS>(out, sums, tid, m0, M, c0, cols);
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -53,50 +53,66 @@ struct LinearOut {
   const void* bias;
   int64_t up;             // where the others' bias begins
   int32_t dtype, bias_dtype, act;
-  bool vec, bias_vec;     // eight columns of C and R at a time; of the bias
+  bool whole;             // eight columns of C, R and the bias at a time, all there
   uint8_t* scales;        // of codes
   int64_t rows;
   float* part;
 
-  // a 16-bit value of the results' type, and a result as one
+  // a 16-bit value of the results' type
   FS_DEVICE float value(uint32_t h) const { return dtype == FS_BF16 ? bf16_to_f32((uint16_t)h) : f16_to_f32((uint16_t)h); }
-  FS_DEVICE uint32_t bits(float v) const { return dtype == FS_BF16 ? f32_to_bf16(v) : f32_to_f16(v); }
-
-  template <int NC>
+  // two results rounded to it
+  FS_DEVICE uint32_t pair(float a, float b) const {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return dtype == FS_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b16x2))
+                            : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h16x2));
+  }
+  FS_DEVICE float bias_at(int64_t i) const {
+    return bias_dtype == FS_F32 ? static_cast<const float*>(bias)[i]
+                                : bias_dtype == FS_BF16 ? bf16_to_f32(static_cast<const uint16_t*>(bias)[i])
+                                                        : f16_to_f32(static_cast<const uint16_t*>(bias)[i]);
+  }
+  // WHOLE: `whole`, and so no bounds and no single elements: little code, for it is fetched when every CU comes to need it
+  template <bool WHOLE, int NC>
   FS_DEVICE void add_bias(float (&v)[NC], int64_t at, int64_t left) const {
-    if (bias_vec && left >= NC) {
-      if (bias_dtype == FS_F32) {
-#pragma unroll
-        for (int h = 0; h < NC / 4; ++h) {
-          const float4_t b = *reinterpret_cast<const float4_t*>(static_cast<const float*>(bias) + at + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * h + e] += b[e];
-        }
-        return;
-      }
+    if (WHOLE && bias_dtype == FS_F32) {
 #pragma unroll
       for (int h = 0; h < NC / 4; ++h) {
-        const u32x2_t b = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(bias) + at + 4 * h);
+        const float4_t b = *reinterpret_cast<const float4_t*>(static_cast<const float*>(bias) + at + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[4 * h + e] += bias_dtype == FS_BF16 ? half_of<FS_BF16>(b[e >> 1], e & 1) : half_of<FS_F16>(b[e >> 1], e & 1);
+        for (int e = 0; e < 4; ++e) v[4 * h + e] += b[e];
       }
-      return;
-    }
+    } else if (WHOLE) {
+      uint32_t b[NC / 2];
 #pragma unroll
-    for (int e = 0; e < NC; ++e) {
-      if (e >= left) break;
-      if (bias_dtype == FS_F32) v[e] += static_cast<const float*>(bias)[at + e];
-      else if (bias_dtype == FS_BF16) v[e] += bf16_to_f32(static_cast<const uint16_t*>(bias)[at + e]);
-      else v[e] += f16_to_f32(static_cast<const uint16_t*>(bias)[at + e]);
+      for (int h = 0; h < NC / 4; ++h) {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(bias) + at + 4 * h);
+        b[2 * h] = w[0];
+        b[2 * h + 1] = w[1];
+      }
+#pragma unroll
+      for (int e = 0; e < NC; ++e) {
+        const uint32_t w = b[e >> 1] >> (16 * (e & 1));
+        v[e] += bias_dtype == FS_BF16 ? bf16_to_f32((uint16_t)w) : f16_to_f32((uint16_t)w);
+      }
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < NC; ++e) {
+        if (e >= left) break;
+        const float b = bias_at(at + e);
+#pragma unroll
+        for (int f = 0; f < NC; ++f) v[f] += f == e ? b : 0.f;
+      }
     }
   }
   // NC columns' sums from col on, of `cols`, to what is rounded
-  template <int NC>
+  template <bool WHOLE, int NC>
   FS_DEVICE void compute(float (&v)[NC], float (&u)[NC], int64_t row, int64_t col, int64_t cols) const {
     if (bias) {
-      add_bias(v, col, cols - col);
-      if (GATED) add_bias(u, up + col, cols - col);
+      add_bias<WHOLE>(v, col, cols - col);
+      if (GATED) add_bias<WHOLE>(u, up + col, cols - col);
     }
     switch (act) {
       case FS_ACT_RELU:
@@ -124,7 +140,7 @@ struct LinearOut {
     }
     if (!CODES && R) {
       const uint16_t* r = R + row * ldr + col;
-      if (vec && col + NC <= cols) {
+      if (WHOLE) {
 #pragma unroll
         for (int h = 0; h < NC / 4; ++h) {
           const u32x2_t w = *reinterpret_cast<const u32x2_t*>(r + 4 * h);
@@ -132,28 +148,35 @@ struct LinearOut {
           for (int e = 0; e < 4; ++e) v[4 * h + e] += value(w[e >> 1] >> (16 * (e & 1)));
         }
       } else {
+#pragma unroll 1
+        for (int e = 0; e < NC; ++e) {
+          if (col + e >= cols) break;
+          const float b = value(r[e]);
 #pragma unroll
-        for (int e = 0; e < NC; ++e)
-          if (col + e < cols) v[e] += value(r[e]);
+          for (int f = 0; f < NC; ++f) v[f] += f == e ? b : 0.f;
+        }
       }
     }
   }
   // Four columns' sums (the others' in b where gated) finished and stored.
   FS_DEVICE void four(const float4_t& a, const float4_t& b, int64_t row, int64_t col, int64_t cols) const {
     float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
-    compute(v, u, row, col, cols);
     uint16_t* c = C + row * ldc + col;
-    if (vec && col + 4 <= cols) {
-      *reinterpret_cast<u32x2_t*>(c) = u32x2_t{bits(v[0]) | bits(v[1]) << 16, bits(v[2]) | bits(v[3]) << 16};
+    if (whole) {
+      compute<true>(v, u, row, col, cols);
+      *reinterpret_cast<u32x2_t*>(c) = u32x2_t{pair(v[0], v[1]), pair(v[2], v[3])};
     } else {
+      compute<false>(v, u, row, col, cols);
+      const uint32_t o[2] = {pair(v[0], v[1]), pair(v[2], v[3])};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (col + e < cols) c[e] = (uint16_t)bits(v[e]);
+        if (col + e < cols) c[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
     }
   }
   // Eight columns' sums finished and stored. For codes 16 lanes side by side hold a row's group (all in range, or none).
+  template <bool WHOLE>
   FS_DEVICE void piece(float (&v)[8], float (&u)[8], int64_t row, int64_t col, int64_t cols) const {
-    compute(v, u, row, col, cols);
+    compute<WHOLE>(v, u, row, col, cols);
     if constexpr (CODES) {
       float m = 0.f;
 #pragma unroll
@@ -171,46 +194,51 @@ struct LinearOut {
       }
     } else {
       uint16_t* c = C + row * ldc + col;
-      uint32_t o[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = bits(v[e]);
-      if (vec && col + 8 <= cols) {
-        *reinterpret_cast<u32x4*>(c) = u32x4{o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16};
+      const u32x4 o = {pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+      if (WHOLE) {
+        *reinterpret_cast<u32x4*>(c) = o;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (col + e < cols) c[e] = (uint16_t)o[e];
+          if (col + e < cols) c[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
       }
     }
   }
 };
 
-// The splits' sums added in order and finished, eight columns of the results a thread (N % 4 == 0: rows of W).
-template <class OUT>
-__global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __restrict__ part, int splits, int64_t M, int64_t N,
+// The SPLITS sums in memory added in order and finished, eight columns of the results a thread (N % 4 == 0: rows of W); every
+// load ahead of the first addition.
+template <class OUT, int SPLITS>
+__global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __restrict__ part, int64_t M, int64_t N,
                                                                uint32_t pieces, OUT out) {
-  const int64_t cols = OUT::GATED ? N / 2 : N;
+  constexpr int H = OUT::GATED ? 2 : 1;   // the gate's, the others'
+  const int64_t cols = N / H;
   const uint32_t unit = blockIdx.x * 256u + threadIdx.x;   // (M * pieces < 2^31)
   const int64_t row = unit / pieces, col = 8 * (int64_t)(unit % pieces);
   if (row >= M) return;   // (by groups of 16 lanes where codes are written: pieces % 16 == 0)
-  float v[8], u[8];
-  auto add = [&](float (&to)[8], const float* p, bool set) {
+  const float* p = part + row * N + col;
+  const bool two = col + 4 < cols;   // (else the second four are those of the first, and nobody's)
+  float4_t a[SPLITS][H][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (col + 4 * h >= cols) continue;
-      const float4_t a = *reinterpret_cast<const float4_t*>(p + 4 * h);
+  for (int s = 0; s < SPLITS; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to[4 * h + e] = set ? a[e] : to[4 * h + e] + a[e];
+    for (int h = 0; h < H; ++h) {
+      const float* q = p + (int64_t)s * M * N + h * cols;
+      a[s][h][0] = *reinterpret_cast<const float4_t*>(q);
+      a[s][h][1] = *reinterpret_cast<const float4_t*>(q + (two ? 4 : 0));
     }
-  };
+  __builtin_amdgcn_sched_barrier(0);
+  float v[H][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float* p = part + ((int64_t)s * M + row) * N + col;
-    add(v, p, s == 0);
-    if (OUT::GATED) add(u, p + cols, s == 0);
-  }
-  out.piece(v, u, row, col, cols);
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[h][e] = a[0][h][e >> 2][e & 3];
+#pragma unroll
+      for (int s = 1; s < SPLITS; ++s) v[h][e] += a[s][h][e >> 2][e & 3];
+    }
+  if (out.whole) out.template piece<true>(v[0], v[H - 1], row, col, cols);
+  else out.template piece<false>(v[0], v[H - 1], row, col, cols);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -407,13 +435,17 @@ Plan plan_for(const fs_linear& c) {
     int bm, bn;
     double stage, fixed;
   };
-  static const Cand cands[] = {{64, 64, 0.43, 3.0}, {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0}, {256, 256, 1.5, 10.0}};
+  // (the two before the last: only for a gate's codes)
+  static const Cand cands[] = {{64, 64, 0.43, 3.0},  {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0},
+                               {64, 256, 0.85, 4.0}, {128, 256, 1.05, 6.0}, {256, 256, 1.5, 10.0}};
   Plan best{64, 64, 1, c.out_scales != nullptr, false};
   double least = 1e30;
   for (const Cand& t : cands) {
+    const bool gate_codes = c.out_scales && c.gated;
+    if (t.bn == 256 && t.bm < 256 && !gate_codes) continue;
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
     const bool whole = !c.out_scales || t.bn == 256 || (t.bn == 128 && !c.gated);
-    for (int s = 1; s <= 8; s *= 2) {
+    for (int s = 1; s <= (t.bn == 256 && t.bm < 256 ? 1 : 8); s *= 2) {
       // (a split starts at a whole word of scales; partials are stored four columns at a time)
       const bool join = s > 1 || !whole;
       if (s > 1 && nk % (4 * s) != 0) break;
@@ -454,9 +486,12 @@ void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per
 template <class OUT, bool PARTS>
 void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
-  if (p.bn == 256) {
+  if (p.bn == 256 && p.bm == 256) {
     gemm_e4m3_long_kernel<OUT, PARTS><<<grid, 512, 0, s>>>(P, out);
-  } else if constexpr (!OUT::CODES || !OUT::GATED) {
+  } else if constexpr (OUT::CODES && OUT::GATED) {
+    if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 256, 2, 4, 3><<<grid, 512, 0, s>>>(P, out);
+    else gemm_e4m3_tile_kernel<OUT, 64, 256, 1, 8, 3><<<grid, 512, 0, s>>>(P, out);
+  } else {
     if (p.bm == 256) gemm_e4m3_tile_kernel<OUT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, out);
     else if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, out);
     else if constexpr (!OUT::CODES) gemm_e4m3_tile_kernel<OUT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, out);
@@ -475,8 +510,7 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
   out.dtype = c.dtype;
   out.bias_dtype = c.bias_dtype;
   out.act = c.activation;
-  out.vec = al16(c.out) && c.ldo % 8 == 0 && (!c.residual || (al16(c.residual) && c.ldr % 8 == 0));
-  out.bias_vec = al16(c.bias) && (!c.gated || c.N % 8 == 0);
+  out.whole = c.N % 8 == 0 && al16(c.out) && c.ldo % 8 == 0 && al16(c.residual) && c.ldr % 8 == 0 && al16(c.bias);
   out.scales = reinterpret_cast<uint8_t*>(c.out_scales);
   out.rows = c.M;
   out.part = nullptr;
@@ -487,8 +521,11 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
     if (p.stream) launch_stream(P, sums, p, stream_columns(P.N, false), s);   // (rows of W in their order, gated or not)
     else launch_tiles<Sums, true>(P, sums, p, s);
     const uint32_t pieces = (uint32_t)((c.N + 7) / 8);
-    linear_e4m3_join_kernel<OUT><<<dim3((unsigned)((c.M * pieces + 255) / 256)), 256, 0, s>>>(part, p.splits, P.M, P.N, pieces,
-                                                                                             out);
+    const dim3 grid((unsigned)((c.M * pieces + 255) / 256));
+    if (p.splits == 8) linear_e4m3_join_kernel<OUT, 8><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
+    else if (p.splits == 4) linear_e4m3_join_kernel<OUT, 4><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
+    else if (p.splits == 2) linear_e4m3_join_kernel<OUT, 2><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
+    else linear_e4m3_join_kernel<OUT, 1><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
   } else if constexpr (!OUT::CODES) {
     if (p.stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
     else launch_tiles<OUT, false>(P, out, p, s);

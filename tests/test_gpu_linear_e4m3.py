@@ -134,41 +134,41 @@ SIZES = {
     (35, 2105, 512, True, False): (64, 32, 1, 0), (36, 4736, 512, False, True): (64, 32, 1, 1),
     (36, 2176, 512, True, True): (64, 32, 1, 1), (134, 1, 512, False, False): (64, 64, 1, 0),
     (134, 1, 512, True, False): (64, 64, 1, 0), (129, 128, 640, False, True): (64, 64, 1, 1),
-    (129, 128, 512, True, True): (64, 64, 1, 1), (35, 4, 11264, False, False): (64, 64, 2, 1),
+    (129, 128, 640, True, True): (64, 64, 1, 1), (35, 4, 11264, False, False): (64, 64, 2, 1),
     (129, 128, 1024, False, True): (64, 64, 2, 1), (73, 4, 5120, True, False): (64, 64, 2, 1),
     (129, 128, 1024, True, True): (64, 64, 2, 1), (135, 4, 2048, False, False): (64, 64, 4, 1),
     (129, 128, 2048, False, True): (64, 64, 4, 1), (134, 4, 2048, True, False): (64, 64, 4, 1),
     (129, 128, 2048, True, True): (64, 64, 4, 1), (129, 4, 4096, False, False): (64, 64, 8, 1),
     (33, 128, 12288, False, True): (64, 64, 8, 1), (129, 4, 4096, True, False): (64, 64, 8, 1),
-    (33, 128, 12288, True, True): (64, 64, 8, 1), (65, 1, 512, False, False): (128, 16, 1, 0),
-    (65, 1, 512, True, False): (128, 16, 1, 0), (65, 128, 512, False, True): (128, 16, 1, 1),
-    (65, 128, 512, True, True): (128, 16, 1, 1), (67, 4172, 512, False, False): (128, 32, 1, 0),
-    (66, 2074, 512, True, False): (128, 32, 1, 0), (72, 4224, 512, False, True): (128, 32, 1, 1),
-    (72, 2176, 512, True, True): (128, 32, 1, 1), (66, 8316, 512, False, False): (128, 128, 1, 0),
-    (129, 128, 512, False, True): (128, 128, 1, 0), (67, 4187, 512, True, False): (128, 128, 1, 0),
-    (66, 4224, 512, True, True): (128, 128, 1, 1), (72, 8204, 4096, False, False): (128, 128, 2, 1),
-    (34, 9088, 4096, False, True): (128, 128, 2, 1), (35, 4284, 8192, True, False): (128, 128, 2, 1),
-    (71, 4480, 1024, True, True): (128, 128, 2, 1), (2123, 68, 10240, False, False): (128, 128, 4, 1),
-    (147, 2816, 2048, False, True): (128, 128, 4, 1), (2754, 68, 4096, True, False): (128, 128, 4, 1),
-    (135, 1408, 4096, True, True): (128, 128, 4, 1), (2318, 4, 12288, False, False): (128, 128, 8, 1),
-    (133, 1408, 4096, False, True): (128, 128, 8, 1), (2085, 4, 16384, True, False): (128, 128, 8, 1),
-    (129, 768, 4096, True, True): (128, 128, 8, 1), (148, 16385, 512, False, False): (256, 128, 1, 0),
+    (33, 128, 12288, True, True): (64, 64, 8, 1), (129, 128, 512, True, True): (64, 256, 1, 0),
+    (65, 1, 512, False, False): (128, 16, 1, 0), (65, 1, 512, True, False): (128, 16, 1, 0),
+    (65, 128, 512, False, True): (128, 16, 1, 1), (65, 128, 512, True, True): (128, 16, 1, 1),
+    (67, 4172, 512, False, False): (128, 32, 1, 0), (66, 2074, 512, True, False): (128, 32, 1, 0),
+    (72, 4224, 512, False, True): (128, 32, 1, 1), (72, 2176, 512, True, True): (128, 32, 1, 1),
+    (66, 8316, 512, False, False): (128, 128, 1, 0), (129, 128, 512, False, True): (128, 128, 1, 0),
+    (67, 4187, 512, True, False): (128, 128, 1, 0), (36, 8576, 3456, True, True): (128, 128, 1, 1),
+    (72, 8204, 4096, False, False): (128, 128, 2, 1), (34, 9088, 4096, False, True): (128, 128, 2, 1),
+    (35, 4284, 8192, True, False): (128, 128, 2, 1), (33, 4224, 4096, True, True): (128, 128, 2, 1),
+    (2123, 68, 10240, False, False): (128, 128, 4, 1), (147, 2816, 2048, False, True): (128, 128, 4, 1),
+    (2754, 68, 4096, True, False): (128, 128, 4, 1), (135, 1408, 4096, True, True): (128, 128, 4, 1),
+    (2318, 4, 12288, False, False): (128, 128, 8, 1), (133, 1408, 4096, False, True): (128, 128, 8, 1),
+    (2085, 4, 16384, True, False): (128, 128, 8, 1), (129, 768, 4096, True, True): (128, 128, 8, 1),
+    (71, 17024, 512, True, True): (128, 256, 1, 0), (148, 16385, 512, False, False): (256, 128, 1, 0),
     (133, 17280, 512, False, True): (256, 128, 1, 0), (136, 9354, 512, True, False): (256, 128, 1, 0),
-    (150, 8448, 1536, True, True): (256, 128, 1, 1), (131, 11364, 15360, False, False): (256, 128, 2, 1),
-    (158, 10496, 15360, False, True): (256, 128, 2, 1), (266, 3260, 11264, True, False): (256, 128, 2, 1),
-    (135, 4224, 4096, True, True): (256, 128, 2, 1), (177, 4164, 10240, False, False): (256, 128, 4, 1),
-    (142, 4224, 8192, False, True): (256, 128, 4, 1), (155, 2180, 10240, True, False): (256, 128, 4, 1),
-    (146, 2176, 8192, True, True): (256, 128, 4, 1), (146, 2188, 16384, False, False): (256, 128, 8, 1),
-    (130, 2432, 16384, False, True): (256, 128, 8, 1), (2119, 72, 16384, True, False): (256, 128, 8, 1),
-    (129, 1152, 16384, True, True): (256, 128, 8, 1), (569, 13171, 512, False, False): (256, 256, 1, 0),
-    (395, 17024, 512, False, True): (256, 256, 1, 0), (152, 17738, 512, True, False): (256, 256, 1, 0),
-    (33, 17152, 512, True, True): (256, 256, 1, 0), (166, 17036, 8192, False, False): (256, 256, 2, 1),
-    (143, 16512, 8192, False, True): (256, 256, 2, 1), (258, 5508, 8192, True, False): (256, 256, 2, 1),
-    (142, 8576, 4096, True, True): (256, 256, 2, 1), (155, 8300, 8192, False, False): (256, 256, 4, 1),
-    (130, 8320, 8192, False, True): (256, 256, 4, 1), (141, 4956, 10240, True, False): (256, 256, 4, 1),
-    (132, 4608, 8192, True, True): (256, 256, 4, 1), (140, 4236, 16384, False, False): (256, 256, 8, 1),
-    (136, 4352, 16384, False, True): (256, 256, 8, 1), (131, 2060, 16384, True, False): (256, 256, 8, 1),
-    (131, 2176, 16384, True, True): (256, 256, 8, 1),
+    (131, 11364, 15360, False, False): (256, 128, 2, 1), (158, 10496, 15360, False, True): (256, 128, 2, 1),
+    (266, 3260, 11264, True, False): (256, 128, 2, 1), (135, 4224, 4096, True, True): (256, 128, 2, 1),
+    (177, 4164, 10240, False, False): (256, 128, 4, 1), (142, 4224, 8192, False, True): (256, 128, 4, 1),
+    (155, 2180, 10240, True, False): (256, 128, 4, 1), (146, 2176, 8192, True, True): (256, 128, 4, 1),
+    (146, 2188, 16384, False, False): (256, 128, 8, 1), (130, 2432, 16384, False, True): (256, 128, 8, 1),
+    (2119, 72, 16384, True, False): (256, 128, 8, 1), (129, 1152, 16384, True, True): (256, 128, 8, 1),
+    (569, 13171, 512, False, False): (256, 256, 1, 0), (395, 17024, 512, False, True): (256, 256, 1, 0),
+    (152, 17738, 512, True, False): (256, 256, 1, 0), (200, 17920, 512, True, True): (256, 256, 1, 0),
+    (166, 17036, 8192, False, False): (256, 256, 2, 1), (143, 16512, 8192, False, True): (256, 256, 2, 1),
+    (258, 5508, 8192, True, False): (256, 256, 2, 1), (137, 11264, 8192, True, True): (256, 256, 2, 1),
+    (155, 8300, 8192, False, False): (256, 256, 4, 1), (130, 8320, 8192, False, True): (256, 256, 4, 1),
+    (141, 4956, 10240, True, False): (256, 256, 4, 1), (132, 4608, 8192, True, True): (256, 256, 4, 1),
+    (140, 4236, 16384, False, False): (256, 256, 8, 1), (136, 4352, 16384, False, True): (256, 256, 8, 1),
+    (131, 2060, 16384, True, False): (256, 256, 8, 1), (131, 2176, 16384, True, True): (256, 256, 8, 1),
 }
 
 
