@@ -79,7 +79,7 @@ FS_DEVICE void put4(const OUT& out, float4_t a, int64_t row, int64_t col0, int64
 template <class OUT, bool WHOLE, int ROWS, int COLS, int PITCH, int THREADS>
 FS_DEVICE void finish_pieces(const OUT& out, const float* sums, int tid, int64_t m0, int64_t M, int64_t c0, int64_t cols) {
   constexpr int OC = OUT::GATED ? COLS / 2 : COLS, PIECES = OC / 8;
-  static_assert(ROWS * PIECES % THREADS == 0 && PITCH % 4 == 0, "whole rounds");
+  static_assert(ROWS * PIECES % 64 == 0 && PITCH % 4 == 0, "whole waves");
 #pragma unroll 1
   for (int u = tid; u < ROWS * PIECES; u += THREADS) {
     const int r = u / PIECES, p = u % PIECES;

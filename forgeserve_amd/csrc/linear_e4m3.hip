@@ -16,6 +16,10 @@ namespace {
 // over the limit 64 x 4096 x 14336 24.4 and 19.8, 96 x 2048 x 8192 14.6 and 13.5; four tiles, 64 x 16384 x 2048, 11.1 and 9.8).
 constexpr int STREAM_ROWS = 128;
 constexpr int64_t STREAM_BYTES = 600 * 1024;
+// Codes leave these kernels by themselves, up to 16 rows and without a gate, a group of 128 columns a workgroup, where there
+// are so many groups that their CUs draw nearly what all of them would (16 x 8192 x 2048 7.6 us, through memory 8.6; 16 x 4096
+// x 4096 10.1 and 9.1; a gate's, twice the bytes a CU: 16 x 28672 x 4096 31.6 and 26.8).
+constexpr int STREAM_CODES = 56 * GROUP;
 
 // ------------------------------------------------------------------------------------------------
 // what is done with the sums
@@ -178,13 +182,8 @@ struct LinearOut {
   FS_DEVICE void piece(float (&v)[8], float (&u)[8], int64_t row, int64_t col, int64_t cols) const {
     compute<WHOLE>(v, u, row, col, cols);
     if constexpr (CODES) {
-      float m = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_magnitude(v[e]));
-      const int e = scale_exponent<FS_F32>(group_max<16>(m));
-      const float inv = scale_inverse(e);
-      *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(C) + row * ldc + col) =
-          u32x2_t{encode4(v[0], v[1], v[2], v[3], inv), encode4(v[4], v[5], v[6], v[7], inv)};
+      int e;
+      *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(C) + row * ldc + col) = encode_eight(v, e);
       if ((col & (GROUP - 1)) == 0) {
         const int g = (int)(col / GROUP);
         uint8_t* word = scales + ((int64_t)(g >> 2) * rows + row) * 4;
@@ -372,7 +371,11 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
   }
   __syncthreads();   // every wave has read its last pieces, and no copy is on its way
   float4_t(*red)[CH][64] = reinterpret_cast<float4_t(*)[CH][64]>(&ring[0][0]);
-  // CH tiles at a time: wave t joins tile t's eight sums in order; lane (l16, g) has row l16, and of the tile's rows of W
+  constexpr int PITCH = GROUP + 4;
+  float* rows = reinterpret_cast<float*>(&ring[4][0]);
+  static_assert(!OUT::CODES || (!OUT::GATED && TN * COLS == GROUP && sizeof(red[0]) * 8 <= sizeof(ring) / 2 &&
+                                16 * TM * PITCH * sizeof(float) <= sizeof(ring) / 2), "a group, beside the sums");
+  // CH tiles at a time: wave t joins tile t's eight sums in order (codes': into rows of a group's, behind the ring's first half); lane (l16, g) has row l16, and of the tile's rows of W
   // (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
 #pragma unroll
   for (int first = 0; first < TILES; first += CH) {
@@ -395,9 +398,17 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
     }
     const int row = 16 * (t / TN) + l16;
     const int64_t col = c0 + COLS * (t % TN) + 4 * g;
+    if constexpr (OUT::CODES) {
+      *reinterpret_cast<float4_t*>(rows + row * PITCH + COLS * (t % TN) + 4 * g) = a;
+      continue;
+    }
     if (row >= M || col >= c1 || (OUT::GATED && g >= 2)) continue;
     if (!OUT::GATED && out.part) *reinterpret_cast<float4_t*>(out.part + row * P.N + col) = a;   // (N % 4 == 0)
     else if constexpr (!OUT::CODES) out.four(a, b, row, col, cols);
+  }
+  if constexpr (OUT::CODES) {
+    __syncthreads();
+    finish_tile<OUT, 16 * TM, GROUP, PITCH, 512>(out, rows, threadIdx.x, 0, M, c0, cols);
   }
 }
 
@@ -422,36 +433,45 @@ int stream_tiles(int64_t cols, bool gated) {
   return tiles <= 2 ? (int)tiles : tiles <= 4 ? 4 : 7;
 }
 
-// Tiles as gemm_e4m3.hip's rule has them. Codes leave a tile of 256 x 256, or of 128 columns without a gate, by themselves;
-// sums that go through memory are written and read at 4.5 TB/s and cost a launch of 3 us.
+// Tiles: the cheapest of what a sweep over 26 shapes of 40 to 4000 rows fits (us; by 4 to 12 % rms, and its choice is within
+// 1.4 % of the best one's time on average, 9 % at most): `first` for a grid, `round` for each further round of the CUs' places
+// (two of the smaller tiles share a CU: stage2 for both), a stage of 128, and a MB of results or of sums in memory. Codes
+// leave tiles of 128 columns by themselves, a gate's tiles of 256; other sums go through memory, as those of K splits do.
 Plan plan_for(const fs_linear& c) {
   const int64_t M = c.M, N = weight_rows(c), nk = c.K / GROUP;
+  const bool codes = c.out_scales != nullptr;
   if (M <= STREAM_ROWS) {
-    const int tiles = c.out_scales ? stream_tiles(N, false) : stream_tiles(c.N, c.gated != 0);
     const int rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    if (rows <= 32 || (tiles <= 2 && rows * c.K <= STREAM_BYTES)) return Plan{rows, 16 * tiles, 1, c.out_scales != nullptr, true};
+    if (codes && !c.gated && rows == 16 && c.N >= STREAM_CODES) return Plan{rows, GROUP, 1, false, true};
+    const int tiles = codes ? stream_tiles(N, false) : stream_tiles(c.N, c.gated != 0);
+    if (rows <= 32 || (tiles <= 2 && rows * c.K <= STREAM_BYTES)) return Plan{rows, 16 * tiles, 1, codes, true};
   }
   struct Cand {
     int bm, bn;
-    double stage, fixed;
+    double first, round, stage, stage2, sums_mb, out_mb;   // stage2 0: one a CU
   };
-  // (the two before the last: only for a gate's codes)
-  static const Cand cands[] = {{64, 64, 0.43, 3.0},  {128, 128, 0.66, 5.0}, {256, 128, 1.05, 7.0},
-                               {64, 256, 0.85, 4.0}, {128, 256, 1.05, 6.0}, {256, 256, 1.5, 10.0}};
-  Plan best{64, 64, 1, c.out_scales != nullptr, false};
+  static const Cand cands[] = {{64, 64, 3.9, 0.6, 0.32, 0.46, 0.14, 0.26},   {64, 128, 3.9, 0.1, 0.46, 0.64, 0.18, 0.30},
+                               {128, 128, 4.7, 2.6, 0.56, 0.0, 0.13, 0.31},  {256, 128, 5.2, 2.1, 0.85, 0.0, 0.18, 0.44},
+                               {64, 256, 4.0, 2.6, 0.67, 0.0, 0.0, 0.23},    {128, 256, 5.5, 3.9, 0.86, 0.0, 0.0, 0.38},
+                               {256, 256, 9.7, 16.7, 0.97, 0.0, 0.21, 0.44}};
+  Plan best{64, 64, 1, codes, false};
   double least = 1e30;
   for (const Cand& t : cands) {
-    const bool gate_codes = c.out_scales && c.gated;
-    if (t.bn == 256 && t.bm < 256 && !gate_codes) continue;
+    if (t.bn == 256 && t.bm < 256 && !(codes && c.gated)) continue;   // (no other kernels of these)
+    if (t.bm == 64 && t.bn == 128 && codes && c.gated) continue;
+    const bool whole = !codes || t.bn == 256 || (t.bn == 128 && !c.gated);
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-    const bool whole = !c.out_scales || t.bn == 256 || (t.bn == 128 && !c.gated);
-    for (int s = 1; s <= (t.bn == 256 && t.bm < 256 ? 1 : 8); s *= 2) {
+    for (int s = 1; s <= 8; s *= 2) {
       // (a split starts at a whole word of scales; partials are stored four columns at a time)
       const bool join = s > 1 || !whole;
-      if (s > 1 && nk % (4 * s) != 0) break;
-      if (join && (N % 4 != 0 || (c.gated && c.N % 4 != 0))) break;
-      const double us = (double)((tiles * s + 255) / 256) * ((double)(nk / s) * t.stage + t.fixed) +
-                        (join ? 3.0 + (double)s * (double)M * (double)N * 8.0 / 4.5e6 : 0.0);
+      if (s > 1 && (nk % (4 * s) != 0 || (t.bn == 256 && t.bm < 256))) break;
+      if (join && (N % 4 != 0 || c.N % 4 != 0)) break;
+      const int64_t wgs = tiles * s, places = t.stage2 > 0.0 ? 512 : 256, rest = wgs % places;
+      const double one = t.stage2 > 0.0 ? (rest > 0 && rest <= 256) : (double)(wgs / places + (rest > 0));
+      const double two = t.stage2 > 0.0 ? (double)(wgs / places + (rest > 256)) : 0.0;
+      const double out_mb = (double)M * (double)N * 2e-6, sums_mb = 2.0 * s * out_mb;
+      const double us = t.first + t.round * (one + two - 1.0) + (double)(nk / s) * (one * t.stage + two * t.stage2) +
+                        (join ? t.sums_mb * sums_mb + 2.9 + 0.125 * sums_mb + 0.05 * out_mb : t.out_mb * out_mb);
       if (us < least) least = us, best = Plan{t.bm, t.bn, s, join, false};
     }
   }
@@ -467,11 +487,15 @@ template <class OUT, int TM>
 void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
   const dim3 grid((unsigned)((cols + per - 1) / per));
-  if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else if constexpr (TM > 2) return;   // (not planned)
-  else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per);
-  else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per);
+  if constexpr (OUT::CODES) {
+    if constexpr (TM == 1 && !OUT::GATED) linear_e4m3_stream_kernel<OUT, TM, 8><<<grid, 512, 0, s>>>(P, out, (int)per);
+  } else {
+    if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
+    else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
+    else if constexpr (TM > 2) return;   // (not planned)
+    else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per);
+    else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per);
+  }
 }
 template <class OUT>
 void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
@@ -494,6 +518,7 @@ void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t 
   } else {
     if (p.bm == 256) gemm_e4m3_tile_kernel<OUT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, out);
     else if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, out);
+    else if (p.bn == 128) gemm_e4m3_tile_kernel<OUT, 64, 128, 2, 2, 3><<<grid, 256, 0, s>>>(P, out);
     else if constexpr (!OUT::CODES) gemm_e4m3_tile_kernel<OUT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, out);
   }
 }
@@ -526,9 +551,8 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
     else if (p.splits == 4) linear_e4m3_join_kernel<OUT, 4><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else if (p.splits == 2) linear_e4m3_join_kernel<OUT, 2><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else linear_e4m3_join_kernel<OUT, 1><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
-  } else if constexpr (!OUT::CODES) {
-    if (p.stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
-    else launch_tiles<OUT, false>(P, out, p, s);
+  } else if (p.stream) {
+    launch_stream(P, out, p, OUT::CODES ? GROUP : stream_columns(c.N, c.gated != 0), s);
   } else {
     launch_tiles<OUT, false>(P, out, p, s);
   }

@@ -55,13 +55,9 @@ FS_DEVICE void store8(typename Elem<DT>::T* p, const float (&v)[8]) {
 // The codes of eight normed values a lane, 16 lanes a group, a wave 512 columns: the row's word k4 with them. `in`: whether
 // the lane's columns exist (whole groups).
 FS_DEVICE void store_codes(const float (&y)[8], bool in, uint8_t* codes, uint32_t* word, int lane) {
-  float m = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_magnitude(y[e]));
-  const int e = scale_exponent<FS_F32>(group_max<16>(m));
-  const float inv = scale_inverse(e);
-  if (in)
-    *reinterpret_cast<u32x2_t*>(codes) = u32x2_t{encode4(y[0], y[1], y[2], y[3], inv), encode4(y[4], y[5], y[6], y[7], inv)};
+  int e;
+  const u32x2_t c = encode_eight(y, e);
+  if (in) *reinterpret_cast<u32x2_t*>(codes) = c;
   uint32_t w = (lane & 15) == 0 && in ? (uint32_t)e << (8 * (lane >> 4)) : 0u;   // lane 16 g holds byte g, zeros past the row
   w |= (uint32_t)__shfl_xor((int)w, 16, 64);
   w |= (uint32_t)__shfl_xor((int)w, 32, 64);

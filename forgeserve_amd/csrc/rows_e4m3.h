@@ -93,6 +93,36 @@ FS_DEVICE void encode_group(const uint32_t (&w)[NW], int& e, uint32_t (&c)[NW / 
   for (int i = 0; i < NW / 2; ++i) c[i] = encode_words<DT>(w[2 * i], w[2 * i + 1], e, far);
 }
 
+// A group of 128 values in 32 bits, eight in each of 16 lanes: the exponent byte of its scale, and the lane's codes. One
+// conversion divides by the scale and rounds to nearest even; what is not finite, or more than the largest scale's 448, takes
+// the way of encode4, for all of the wave.
+FS_DEVICE u32x2_t encode_eight(const float (&v)[8], int& e) {
+  typedef short v2s __attribute__((ext_vector_type(2)));
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  m = group_max<16>(m);
+  if (__any(m > 0x7f600000u)) {   // 448 * 2^119
+    float f = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f = fmaxf(f, finite_magnitude(v[i]));
+    e = scale_exponent<FS_F32>(group_max<16>(f));
+    const float inv = scale_inverse(e);
+    return u32x2_t{encode4(v[0], v[1], v[2], v[3], inv), encode4(v[4], v[5], v[6], v[7], inv)};
+  }
+  e = scale_exponent<FS_F32>(__uint_as_float(m));
+  const float s = scale_value(e);
+  u32x2_t c;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v2s w = {0, 0};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * h], v[4 * h + 1], s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * h + 2], v[4 * h + 3], s, true);
+    c[h] = __builtin_bit_cast(uint32_t, w);
+  }
+  return c;
+}
+
 // ------------------------------------------------------------------------------------------------
 // results
 // ------------------------------------------------------------------------------------------------
