@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
   float* rows = reinterpret_cast<float*>(&ring[4][0]);
   static_assert(!OUT::CODES || (!OUT::GATED && TN * COLS == GROUP && sizeof(red[0]) * 8 <= sizeof(ring) / 2 &&
                                 16 * TM * PITCH * sizeof(float) <= sizeof(ring) / 2), "a group, beside the sums");
-  // CH tiles at a time: wave t joins tile t's eight sums in order (codes': into rows of a group's, behind the ring's first half); lane (l16, g) has row l16, and of the tile's rows of W
-  // (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
+  // CH tiles at a time: wave t joins tile t's eight sums in order (codes': into rows of a group's, behind the ring's first
+  // half); lane (l16, g) has row l16, and of the tile's rows of W (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
 #pragma unroll
   for (int first = 0; first < TILES; first += CH) {
     if (first) __syncthreads();
