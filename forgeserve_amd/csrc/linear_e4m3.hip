@@ -588,11 +588,14 @@ int check(const fs_linear* c, const char* what) {
   // a copy's offset inside its tile of rows, and a row's scale word inside its group of K, are 32 bits
   FS_CHECK_ARG(c->K <= (1 << 22) && c->M < (1 << 29) && c->N < (1 << 28), "%s: M %lld N %lld K %lld", what, (long long)c->M,
                (long long)c->N, (long long)c->K);
-  FS_CHECK_ARG(c->x_scales || c->M * ((c->K + 511) / 512) < 0x7fffffffLL, "%s: M %lld K %lld", what, (long long)c->M,
+  // 2^32 threads a launch: 64 for a row's 512 columns that are encoded, 512 a tile, one for eight columns from memory
+  FS_CHECK_ARG(c->x_scales || c->M * ((c->K + 511) / 512) < (1 << 26), "%s: M %lld K %lld", what, (long long)c->M,
                (long long)c->K);
   FS_CHECK_ARG(!c->out_scales || c->N % GROUP == 0, "%s: codes of %lld columns (a multiple of %d)", what, (long long)c->N, GROUP);
-  FS_CHECK_ARG(!plan_for(*c).join || c->M * ((c->N + 7) / 8) < 0x7fffff00LL, "%s: M %lld N %lld", what, (long long)c->M,
-               (long long)c->N);
+  const Plan p = plan_for(*c);
+  FS_CHECK_ARG((!p.join || c->M * ((c->N + 7) / 8) < 0x7fffff00LL) &&
+                   (p.stream || ((c->M + p.bm - 1) / p.bm) * ((weight_rows(*c) + p.bn - 1) / p.bn) < (1 << 22)),
+               "%s: M %lld N %lld", what, (long long)c->M, (long long)c->N);
   return 0;
 }
 

@@ -233,7 +233,7 @@ def _row_stride(t: torch.Tensor) -> int:
     strides = t.stride()
     if len(strides) != 2 or (strides[1] != 1 and t.shape[1] > 1):
         raise ValueError(f"expected a 2-D tensor with a contiguous last dim, got {tuple(t.shape)} {strides}")
-    return strides[0]
+    return strides[0] if len(t) > 1 else t.shape[1]   # (a single row's may be anything)
 
 
 _CODES = (torch.float8_e4m3fn, torch.uint8)

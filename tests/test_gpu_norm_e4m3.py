@@ -22,8 +22,9 @@ def values(codes, scales):
 
 def check(codes, scales, v, w, eps):
     """codes against the norm of v (CPU, in its type). The kernel's r: a sum of squares of at most 40 additions in a thread and
-    40 across them (half of them between sums of 512 columns), a mean, a root and a quotient, then two products: 64 roundings of 2^-24 at most with the halving by the root, 2^-18. A code
-    is off by half a step, 2^-4 of the value or 2^-10 of the scale, which is at most 2 / 448 of the group's largest."""
+    40 across them (half of them between sums of 512 columns), a mean, a root and a quotient, then two products: 64 roundings
+    of 2^-24 at most with the halving by the root, 2^-18. A code is off by
+    half a step, 2^-4 of the value or 2^-10 of the scale, which is at most 2 / 448 of the group's largest."""
     m, n = v.shape
     assert codes.shape == (m, n) and codes.dtype == torch.float8_e4m3fn and scales.shape == (-(-n // 512), m, 4)
     x = v.double()
@@ -102,6 +103,40 @@ def test_rows_of_zeros_and_what_is_not_finite(dtype, n):
     if abs(tiny) > 448 * 2.0 ** -117:   # (the smallest scale keeps less of what is smaller)
         assert abs(got[4, 130] - tiny) <= (2.0 ** -4 + 2.0 ** -16) * abs(tiny)
     assert (got[4, torch.arange(n) != 130] == 0).all()
+
+
+@pytest.mark.parametrize("other", [None, float("nan"), float("inf"), 2.0 ** 127 * 1.9])
+def test_every_value_is_encoded_by_its_definition(other):
+    """Rows of ones leave the weight itself (1 / sqrt(mean) = 1), so its codes are those of any 32-bit value, exactly:
+    subnormal ones, ties, what the smallest and the largest scale leave. `other`: in another group of the same wave."""
+    g = torch.Generator().manual_seed(5)
+    n = 16384
+    w = torch.randint(0, 1 << 23, (n,), generator=g, dtype=torch.int32)
+    w = torch.where(torch.rand(n, generator=g) < 0.5, w & ~0x7ffff, w)                        # ties and whole codes
+    top = torch.randint(0, 254, (n // 128, 1), generator=g)                                     # a group's largest exponent
+    ex = (top - torch.randint(0, 20, (n // 128, 128), generator=g)).clamp(min=0).flatten().int()
+    w = (w | ex << 23 | torch.randint(0, 2, (n,), generator=g, dtype=torch.int32) << 31).view(F32)
+    if other is not None:
+        w[128 * 3 + 7 :: 512] = other
+    c, e = ref.encode(w.view(-1, 128), ALL)
+    for m in (1, 1030):
+        codes, scales = ops.add_rmsnorm_e4m3(torch.ones(m, n, device=DEV), w.to(DEV), 0.0)
+        got = codes.view(torch.uint8)
+        assert torch.equal(got, got[:1].expand(m, -1)) and torch.equal(scales, scales[:, :1].expand(-1, m, -1))
+        assert torch.equal(scales[:, 0].cpu().flatten(), e)
+        nan = (c.flatten() & 127) == 127
+        assert torch.equal(torch.where(nan, c.flatten(), got[0].cpu()), c.flatten())
+        assert (got[0].cpu()[nan] & 127 == 127).all()
+
+
+def test_single_rows_of_any_stride():
+    x, w = torch.randn(512, 1, device=DEV).t(), torch.randn(512, device=DEV)
+    want = ops.add_rmsnorm_e4m3(x.contiguous(), w, 1e-5)
+    got = ops.add_rmsnorm_e4m3(x, w, 1e-5)
+    assert x.stride() == (1, 1) and torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
+    assert torch.equal(got[1], want[1])
+    out = torch.zeros(512, 1, device=DEV).t()
+    assert torch.equal(ops.dequantize_e4m3(*want, F32, out=out), ops.dequantize_e4m3(*want, F32))
 
 
 def test_no_rows():

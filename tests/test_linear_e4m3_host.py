@@ -38,7 +38,8 @@ def test_linear_refusals(lib):
                 dict(m=-1), dict(ldx=255), dict(ldw=240), dict(ldw=264), dict(ldo=127), dict(residual=256, ldr=127), dict(w=264),
                 dict(x=264), dict(ldx=264), dict(out_scales=256, out=264), dict(out_scales=256, ldo=136), dict(w_scales=258),
                 dict(x_scales=257), dict(out_scales=258), dict(m=1 << 29), dict(n=1 << 28, ldo=1 << 29),
-                dict(k=1 << 23, ldx=1 << 23, ldw=1 << 23), dict(ldw=1 << 23), dict(ldx=1 << 23)]:
+                dict(m=1 << 26, x_scales=None, x_dtype=_lib.F32),
+                dict(m=1 << 28, n=1 << 20, ldo=1 << 20), dict(k=1 << 23, ldx=1 << 23, ldw=1 << 23), dict(ldw=1 << 23), dict(ldx=1 << 23)]:
         assert call(**bad) == -1, bad
         assert b"linear_e4m3" in lib.fs_last_error()
     assert lib.fs_linear_e4m3(None, 256, 1 << 30, None) == -1
@@ -60,6 +61,7 @@ def test_norm_and_values_refusals(lib):
     assert norm() == 0 and norm(d=256, ldd=256, xo=256, ldxo=256) == 0
     for bad in [dict(x=None), dict(w=None), dict(c=None), dict(s=None), dict(d=256, ldd=256), dict(dt=5), dict(m=-1), dict(n=200),
                 dict(n=0), dict(ldx=255), dict(ldc=255), dict(ldc=264), dict(c=264), dict(s=258), dict(m=1 << 31),
+                dict(m=1 << 26), dict(m=1 << 22, n=2048, ldx=2048, ldc=2048),
                 dict(d=256, ldd=255, xo=256, ldxo=256), dict(d=256, ldd=256, xo=256, ldxo=255)]:
         assert norm(**bad) == -1, bad
 
@@ -68,7 +70,8 @@ def test_norm_and_values_refusals(lib):
 
     assert values() == 0
     for bad in [dict(c=None), dict(s=None), dict(out=None), dict(dt=5), dict(k=100), dict(k=0), dict(rows=-1), dict(ldc=255),
-                dict(ldo=255), dict(ldc=264), dict(c=264), dict(s=257), dict(rows=1 << 31)]:
+                dict(ldo=255), dict(ldc=264), dict(c=264), dict(s=257), dict(rows=1 << 26),
+                dict(rows=1 << 62), dict(rows=1 << 25, k=1024, ldc=1024, ldo=1024)]:
         assert values(**bad) == -1, bad
 
 
