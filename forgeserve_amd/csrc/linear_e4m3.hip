@@ -559,8 +559,7 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
   return fs::launch_status("linear_e4m3");
 }
 
-int linear(const fs_linear& c, char* work, hipStream_t s) {
-  const Plan p = plan_for(c);
+int linear(const fs_linear& c, const Plan& p, char* work, hipStream_t s) {
   const int64_t N = weight_rows(c);
   const uint8_t* x = reinterpret_cast<const uint8_t*>(c.x);
   const uint8_t* xs = reinterpret_cast<const uint8_t*>(c.x_scales);
@@ -581,7 +580,8 @@ int linear(const fs_linear& c, char* work, hipStream_t s) {
   return c.gated ? run<LinearOut<true, false>>(c, P, p, part, s) : run<LinearOut<false, false>>(c, P, p, part, s);
 }
 
-int check(const fs_linear* c, const char* what) {
+// What sizes are refused for; and the plan of the others.
+int check(const fs_linear* c, const char* what, Plan& p) {
   FS_CHECK_ARG(c, "%s: null pointer", what);
   FS_CHECK_ARG(c->M >= 0 && c->N > 0 && c->K > 0 && c->K % GROUP == 0, "%s: M %lld N %lld K %lld (K a multiple of %d)", what,
                (long long)c->M, (long long)c->N, (long long)c->K, GROUP);
@@ -592,7 +592,7 @@ int check(const fs_linear* c, const char* what) {
   FS_CHECK_ARG(c->x_scales || c->M * ((c->K + 511) / 512) < (1 << 26), "%s: M %lld K %lld", what, (long long)c->M,
                (long long)c->K);
   FS_CHECK_ARG(!c->out_scales || c->N % GROUP == 0, "%s: codes of %lld columns (a multiple of %d)", what, (long long)c->N, GROUP);
-  const Plan p = plan_for(*c);
+  p = plan_for(*c);
   FS_CHECK_ARG((!p.join || c->M * ((c->N + 7) / 8) < 0x7fffff00LL) &&
                    (p.stream || ((c->M + p.bm - 1) / p.bm) * ((weight_rows(*c) + p.bn - 1) / p.bn) < (1 << 22)),
                "%s: M %lld N %lld", what, (long long)c->M, (long long)c->N);
@@ -602,14 +602,14 @@ int check(const fs_linear* c, const char* what) {
 }  // namespace
 
 extern "C" int64_t fs_linear_e4m3_workspace_size(const fs_linear* c) {
-  if (check(c, "linear_e4m3_workspace_size")) return 0;
-  return encoded_bytes(*c) + sums_bytes(*c, plan_for(*c));
+  Plan p;
+  return check(c, "linear_e4m3_workspace_size", p) ? 0 : encoded_bytes(*c) + sums_bytes(*c, p);
 }
 
 extern "C" int fs_linear_e4m3_plan(const fs_linear* c, int32_t* plan) {
   FS_CHECK_ARG(plan, "linear_e4m3_plan: null pointer");
-  if (int e = check(c, "linear_e4m3_plan")) return e;
-  const Plan p = plan_for(*c);
+  Plan p;
+  if (int e = check(c, "linear_e4m3_plan", p)) return e;
   plan[0] = p.bm;
   plan[1] = p.bn;
   plan[2] = p.splits;
@@ -618,9 +618,9 @@ extern "C" int fs_linear_e4m3_plan(const fs_linear* c, int32_t* plan) {
 }
 
 extern "C" int fs_linear_e4m3(const fs_linear* call, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (int e = check(call, "linear_e4m3")) return e;
+  Plan p;
+  if (int e = check(call, "linear_e4m3", p)) return e;
   const fs_linear& c = *call;
-  const int64_t N = weight_rows(c);
   FS_CHECK_ARG(c.x && c.w && c.w_scales && c.out, "linear_e4m3: null pointer");
   FS_CHECK_ARG(c.x_scales || c.x_dtype == FS_F32 || c.x_dtype == FS_BF16 || c.x_dtype == FS_F16, "linear_e4m3: rows of dtype %d",
                c.x_dtype);
@@ -640,8 +640,8 @@ extern "C" int fs_linear_e4m3(const fs_linear* call, void* workspace, int64_t wo
   FS_CHECK_ARG(c.ldw < (1 << 23) && (!c.x_scales || c.ldx < (1 << 23)), "linear_e4m3: ldx %lld ldw %lld", (long long)c.ldx,
                (long long)c.ldw);
   if (c.M == 0) return 0;
-  const int64_t need = fs_linear_e4m3_workspace_size(call);
+  const int64_t need = encoded_bytes(c) + sums_bytes(c, p);
   FS_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
                "linear_e4m3: workspace %lld < %lld bytes (or not 256-byte aligned)", (long long)workspace_bytes, (long long)need);
-  return linear(c, reinterpret_cast<char*>(workspace), fs::as_stream(stream));
+  return linear(c, p, reinterpret_cast<char*>(workspace), fs::as_stream(stream));
 }
