@@ -229,29 +229,31 @@ def _stream_of(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) 
     return 0   # (of tensors that are on no GPU: only for checks without one)
 
 
-def _row_stride(t: torch.Tensor) -> int:
+def _row_stride(t: torch.Tensor, n: int) -> int:
+    """The row stride of a 2-D tensor of n columns whose last dim is contiguous (of a single row: any that holds it)."""
+    if t.is_contiguous():
+        return n
     strides = t.stride()
-    if len(strides) != 2 or (strides[1] != 1 and t.shape[1] > 1):
+    if len(strides) != 2 or (strides[1] != 1 and n > 1):
         raise ValueError(f"expected a 2-D tensor with a contiguous last dim, got {tuple(t.shape)} {strides}")
-    return strides[0] if len(t) > 1 else t.shape[1]   # (a single row's may be anything)
+    return strides[0] if len(t) > 1 else n
 
 
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 
 
-def _code_rows(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
-    """The row stride of a matrix of codes with quantize_e4m3's scales; its rows' alignment is the library's to check."""
-    n, k = codes.shape
+def _code_rows(what: str, name: str, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int) -> int:
+    """The row stride of (n, k) codes with quantize_e4m3's scales; its rows' alignment is the library's to check."""
     if codes.dtype not in _CODES:
         raise ValueError(f"{what}: {name} must be float8_e4m3fn or uint8 codes, not {codes.dtype}")
     if scales.dtype is not torch.uint8 or scales.shape != ((k + 511) // 512, n, 4) or not scales.is_contiguous():
         raise ValueError(f"{what}: {name}'s scales must be contiguous uint8 ({(k + 511) // 512}, {n}, 4): {tuple(scales.shape)}")
-    return _row_stride(codes)
+    return _row_stride(codes, k)
 
 
 def _new_codes(m: int, n: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty((m, n), dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(((n + 511) // 512, m, 4), dtype=torch.uint8, device=device))
+    return (torch.empty(m, n, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((n + 511) // 512, m, 4, dtype=torch.uint8, device=device))
 
 
 def dequantize_e4m3(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype,
@@ -262,16 +264,16 @@ def dequantize_e4m3(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
     m, k = codes.shape if codes.dim() == 2 else (0, 0)
     if k % 128 or k == 0:
         raise ValueError(f"dequantize_e4m3: {tuple(codes.shape)}: K is not a multiple of 128")
-    ldc = _code_rows("dequantize_e4m3", "the matrix", codes, scales)
+    ldc = _code_rows("dequantize_e4m3", "the matrix", codes, scales, m, k)
     code = DTYPE_CODE.get(dtype)
     if code is None:
         raise ValueError(f"dequantize_e4m3: dtype {dtype} (float32, bfloat16, float16)")
     if out is None:
-        out, ldo = torch.empty((m, k), dtype=dtype, device=codes.device), k
+        out, ldo = torch.empty(m, k, dtype=dtype, device=codes.device), k
     elif out.shape != codes.shape or out.dtype is not dtype:
         raise ValueError("dequantize_e4m3: out shape/dtype")
     else:
-        ldo = _row_stride(out)
+        ldo = _row_stride(out, k)
     if m:
         check(_lib.load().fs_dequantize_e4m3(codes.data_ptr(), ldc, scales.data_ptr(), m, k, code, out.data_ptr(), ldo, stream),
               "dequantize_e4m3")
@@ -286,21 +288,21 @@ def add_rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: O
     (float32, bfloat16, float16), and rounded once, to the code: a value is kept as quantize_e4m3 keeps it. A row whose
     squares' sum passes float32's range has zeros; of one with an infinite or NaN element that element, or all, are NaN."""
     stream = _stream_of("add_rmsnorm_e4m3", x, weight, delta, x_out)
-    ldx = _row_stride(x)
-    m, n = x.shape
-    dtype = x.dtype
+    shape, dtype = x.shape, x.dtype
+    m, n = shape if len(shape) == 2 else (0, 0)
     dt = DTYPE_CODE.get(dtype)
     if n % 128 or n == 0 or dt is None:
         raise ValueError(f"add_rmsnorm_e4m3: {tuple(x.shape)} {dtype} (N a multiple of 128; float32, bfloat16, float16)")
     if weight.shape != (n,) or weight.dtype is not dtype or not weight.is_contiguous():
         raise ValueError("add_rmsnorm_e4m3: weight shape/dtype")
+    ldx = _row_stride(x, n)
     ldd = ldxo = pd = pxo = 0
     if (delta is None) != (x_out is None):
         raise ValueError("add_rmsnorm_e4m3: delta needs x_out, and x_out delta")
     if delta is not None:
-        if delta.shape != (m, n) or x_out.shape != (m, n) or delta.dtype is not dtype or x_out.dtype is not dtype:
+        if delta.shape != shape or x_out.shape != shape or delta.dtype is not dtype or x_out.dtype is not dtype:
             raise ValueError("add_rmsnorm_e4m3: delta or x_out shape/dtype")
-        ldd, ldxo, pd, pxo = _row_stride(delta), _row_stride(x_out), delta.data_ptr(), x_out.data_ptr()
+        ldd, ldxo, pd, pxo = _row_stride(delta, n), _row_stride(x_out, n), delta.data_ptr(), x_out.data_ptr()
     codes, scales = _new_codes(m, n, x.device)
     if m:
         check(_lib.load().fs_add_rmsnorm_e4m3(x.data_ptr(), ldx, pd, ldd, pxo, ldxo, weight.data_ptr(), codes.data_ptr(), n,
@@ -314,19 +316,20 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # FS_
 def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, residual, out, dtype):
     """Both calls below: (out, None), or with dtype torch.float8_e4m3fn (codes, scales)."""
     stream = _stream_of(what, a, w, w_scales, a_scales, bias, residual, out)
-    if a.dim() != 2 or w.dim() != 2:
-        raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)}")
-    m, k = a.shape
-    rows, wk = w.shape
+    x_shape, w_shape = a.shape, w.shape
+    if len(x_shape) != 2 or len(w_shape) != 2:
+        raise ValueError(f"{what}: {tuple(x_shape)} x {tuple(w_shape)}")
+    m, k = x_shape
+    rows, wk = w_shape
     n = rows // 2 if gated else rows
     if k % 128 or k == 0 or wk != k or n == 0 or (gated and rows % 2):
         raise ValueError(f"{what}: {tuple(a.shape)} x {tuple(w.shape)} (K a multiple of 128, of a gated product an even "
                          "number of rows)")
-    ldw = _code_rows(what, "w", w, w_scales)
+    ldw = _code_rows(what, "w", w, w_scales, rows, k)
     if a_scales is not None:
-        lda, pas, x_dtype = _code_rows(what, "a", a, a_scales), a_scales.data_ptr(), 0
+        lda, pas, x_dtype = _code_rows(what, "a", a, a_scales, m, k), a_scales.data_ptr(), 0
     else:
-        lda, pas, x_dtype = _row_stride(a), 0, DTYPE_CODE.get(a.dtype)
+        lda, pas, x_dtype = _row_stride(a, k), 0, DTYPE_CODE.get(a.dtype)
         if x_dtype is None:
             raise ValueError(f"{what}: rows of {a.dtype} (codes need a_scales)")
     act = ACTIVATIONS.get(activation)
@@ -346,16 +349,16 @@ def _linear_e4m3(what: str, a, w, w_scales, a_scales, bias, activation, gated, r
     else:
         pos = 0
         if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=a.device)
+            out = torch.empty(m, n, dtype=dtype, device=a.device)
             ldo = n
         else:
-            ldo = _row_stride(out)
             if out.shape != (m, n) or out.dtype is not dtype:
                 raise ValueError(f"{what}: out shape/dtype")
+            ldo = _row_stride(out, n)
         if residual is not None:
             if residual.shape != (m, n) or residual.dtype is not dtype:
                 raise ValueError(f"{what}: residual shape/dtype")
-            ldr, pr = _row_stride(residual), residual.data_ptr()
+            ldr, pr = _row_stride(residual, n), residual.data_ptr()
     if m:
         lib = _lib.load()
         call = _lib.Linear(a.data_ptr(), pas, w.data_ptr(), w_scales.data_ptr(), pb, pr, out.data_ptr(), pos, lda, ldw, ldr, ldo,
