@@ -20,6 +20,10 @@ constexpr int64_t STREAM_BYTES = 600 * 1024;
 // are so many groups that their CUs draw nearly what all of them would (16 x 8192 x 2048 7.6 us, through memory 8.6; 16 x 4096
 // x 4096 10.1 and 9.1; a gate's, twice the bytes a CU: 16 x 28672 x 4096 31.6 and 26.8).
 constexpr int STREAM_CODES = 56 * GROUP;
+// Bytes of W from which they are read past the caches (`nt`): of a weight's size several pass between two calls that read the
+// same one, and then the caches have none of it (1 x 4096 x 14336 12.9 -> 11.8 us; with the next comment's turns 1 x 128256 x
+// 4096 91.4 -> 82.5). Smaller ones may still be there (8 x 6144 x 4096 7.1 us, read past them 8.0; out of HBM 8.0 and 7.3).
+constexpr int64_t READ_ONCE = 32 << 20;
 
 // ------------------------------------------------------------------------------------------------
 // what is done with the sums
@@ -249,15 +253,17 @@ __global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __re
 // may share a workgroup, and x's codes. A wave streams its part of K on its own, without a barrier: pieces of 16 rows x 128
 // codes, in each stage x's TM and then W's TN, pass through the wave's SLOTS places in LDS, copied there by whole lines SLOTS
 // pieces ahead: 16 KB a wave, 128 KB a CU on their way. With many rows a workgroup the waves take stages in turn, so that they
-// read a row's next 1 KB together (1 x 28672 x 4096 gated 26.7 -> 25.6 us); with few, eight parts of K, whose words of four
-// stages' scales serve them all (1 x 2048 x 8192 7.1 -> 6.3 us).
+// read a row's next 1 KB together (1 x 28672 x 4096 gated 26.7 -> 25.6 us), and workgroups begin at different KB of their rows,
+// an XCD's at all of them: rows of 4 KB read at the same KB by every CU draw from few of the memory's channels (1 x 28672 x
+// 4096 24.1 -> 22.5, 1 x 128256 x 4096 98.2 -> 91.2). With few rows, eight parts of K, whose words of four stages' scales serve
+// them all (1 x 2048 x 8192 7.1 -> 6.3 us).
 //
 // Straight to registers, in the instruction's own shape, a load runs at a quarter of the rate, 38 GB/s a CU from L2 for 150,
 // for four lanes side by side are four rows: 8 x 6144 x 4096 took 8.6 us so and takes 7.3, 32 x 4096 x 4096 9.8 and 7.1. Now
-// HBM bounds it: 1 x 28672 x 4096 in 25.6 us, 2.3 of them the launch, draws 5.0 TB/s, 1 x 128256 x 4096 5.4; smaller weights
+// HBM bounds it: 1 x 28672 x 4096 in 20.8 us, 2.3 of them the launch, draws 6.4 TB/s, 1 x 128256 x 4096 6.5; smaller weights
 // are on their way before the CUs' 128 KB each have come (4096 x 4096 in 6.6 us).
 template <class OUT, int TM, int TN>
-__global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT out, int per) {
+__global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT out, int per, bool once) {
   constexpr int TILES = TM * TN, CH = TILES < 8 ? TILES : 8, COLS = OUT::GATED ? 8 : 16;
   constexpr int SLOTS = 8, PIECE = 16 * GROUP, PPS = TM + TN;   // pieces a stage
   constexpr int XQ = (16 * TM + 63) / 64, WQ = (16 * TN + 63) / 64, WORDS = 64 * (XQ + WQ);   // a stage's words: x's rows, W's
@@ -275,7 +281,8 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
   // the wave's stages: w, w + 8, ..., or the w-th eighth
   const int k0 = TURNS ? w : (int)((int64_t)w * P.nk / 8);
   const int ni = TURNS ? (P.nk - w + 7) / 8 : (int)((int64_t)(w + 1) * P.nk / 8) - k0;
-  auto stage_of = [&](int i) { return TURNS ? w + 8 * i : k0 + i; };
+  const int rot = TURNS && ni > 0 ? (int)(blockIdx.x / 8 % (unsigned)ni) : 0;   // (workgroups go round the 8 XCDs)
+  auto stage_of = [&](int i) { return TURNS ? w + 8 * (i + rot < ni ? i + rot : i + rot - ni) : k0 + i; };
   auto has_words = [&](int i) { return TURNS || i == 0 || (stage_of(i) & 3) == 0; };
   auto place_of = [&](int i) { return (TURNS ? i : stage_of(i) >> 2) & (PLACES - 1); };
   const int M = (int)P.M;
@@ -320,6 +327,7 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (t < TM) dma16_at(xbase + k * GROUP, xoff[t < TM ? t : 0][h], to + 1024 * h);
+      else if (once) dma16_once_at(wbase[h] + k * GROUP, woff[t < TM ? 0 : t - TM][h], to + 1024 * h);
       else dma16_at(wbase[h] + k * GROUP, woff[t < TM ? 0 : t - TM][h], to + 1024 * h);
     }
   };
@@ -487,14 +495,15 @@ template <class OUT, int TM>
 void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
   const dim3 grid((unsigned)((cols + per - 1) / per));
+  const bool once = P.N * P.nk * GROUP >= READ_ONCE;
   if constexpr (OUT::CODES) {
-    if constexpr (TM == 1 && !OUT::GATED) linear_e4m3_stream_kernel<OUT, TM, 8><<<grid, 512, 0, s>>>(P, out, (int)per);
+    if constexpr (TM == 1 && !OUT::GATED) linear_e4m3_stream_kernel<OUT, TM, 8><<<grid, 512, 0, s>>>(P, out, (int)per, once);
   } else {
-    if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per);
-    else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per);
+    if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+    else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per, once);
     else if constexpr (TM > 2) return;   // (not planned)
-    else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per);
-    else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per);
+    else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+    else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per, once);
   }
 }
 template <class OUT>
