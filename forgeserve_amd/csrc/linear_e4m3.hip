@@ -16,10 +16,6 @@ namespace {
 // over the limit 64 x 4096 x 14336 24.4 and 19.8, 96 x 2048 x 8192 14.6 and 13.5; four tiles, 64 x 16384 x 2048, 11.1 and 9.8).
 constexpr int STREAM_ROWS = 128;
 constexpr int64_t STREAM_BYTES = 600 * 1024;
-// Codes leave these kernels by themselves, up to 16 rows and without a gate, a group of 128 columns a workgroup, where there
-// are so many groups that their CUs draw nearly what all of them would (16 x 8192 x 2048 7.6 us, through memory 8.6; 16 x 4096
-// x 4096 10.1 and 9.1; a gate's, twice the bytes a CU: 16 x 28672 x 4096 31.6 and 26.8).
-constexpr int STREAM_CODES = 56 * GROUP;
 // Bytes of W from which they are read past the caches (`nt`): of a weight's size several pass between two calls that read the
 // same one, and then the caches have none of it (1 x 4096 x 14336 12.9 -> 11.8 us; with the next comment's turns 1 x 128256 x
 // 4096 91.4 -> 82.5). Smaller ones may still be there (8 x 6144 x 4096 7.1 us, read past them 8.0; out of HBM 8.0 and 7.3).
@@ -379,12 +375,8 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
   }
   __syncthreads();   // every wave has read its last pieces, and no copy is on its way
   float4_t(*red)[CH][64] = reinterpret_cast<float4_t(*)[CH][64]>(&ring[0][0]);
-  constexpr int PITCH = GROUP + 4;
-  float* rows = reinterpret_cast<float*>(&ring[4][0]);
-  static_assert(!OUT::CODES || (!OUT::GATED && TN * COLS == GROUP && sizeof(red[0]) * 8 <= sizeof(ring) / 2 &&
-                                16 * TM * PITCH * sizeof(float) <= sizeof(ring) / 2), "a group, beside the sums");
-  // CH tiles at a time: wave t joins tile t's eight sums in order (codes': into rows of a group's, behind the ring's first
-  // half); lane (l16, g) has row l16, and of the tile's rows of W (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
+  // CH tiles at a time: wave t joins tile t's eight sums in order; lane (l16, g) has row l16, and of the tile's rows of W
+  // (g = 0, 1 the gate's, 2, 3 the same columns' others) 4 g ..
 #pragma unroll
   for (int first = 0; first < TILES; first += CH) {
     if (first) __syncthreads();
@@ -406,17 +398,9 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
     }
     const int row = 16 * (t / TN) + l16;
     const int64_t col = c0 + COLS * (t % TN) + 4 * g;
-    if constexpr (OUT::CODES) {
-      *reinterpret_cast<float4_t*>(rows + row * PITCH + COLS * (t % TN) + 4 * g) = a;
-      continue;
-    }
     if (row >= M || col >= c1 || (OUT::GATED && g >= 2)) continue;
     if (!OUT::GATED && out.part) *reinterpret_cast<float4_t*>(out.part + row * P.N + col) = a;   // (N % 4 == 0)
-    else if constexpr (!OUT::CODES) out.four(a, b, row, col, cols);
-  }
-  if constexpr (OUT::CODES) {
-    __syncthreads();
-    finish_tile<OUT, 16 * TM, GROUP, PITCH, 512>(out, rows, threadIdx.x, 0, M, c0, cols);
+    else out.four(a, b, row, col, cols);
   }
 }
 
@@ -450,7 +434,6 @@ Plan plan_for(const fs_linear& c) {
   const bool codes = c.out_scales != nullptr;
   if (M <= STREAM_ROWS) {
     const int rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    if (codes && !c.gated && rows == 16 && c.N >= STREAM_CODES) return Plan{rows, GROUP, 1, false, true};
     const int tiles = codes ? stream_tiles(N, false) : stream_tiles(c.N, c.gated != 0);
     if (rows <= 32 || (tiles <= 2 && rows * c.K <= STREAM_BYTES)) return Plan{rows, 16 * tiles, 1, codes, true};
   }
@@ -496,15 +479,11 @@ void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipSt
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
   const dim3 grid((unsigned)((cols + per - 1) / per));
   const bool once = P.N * P.nk * GROUP >= READ_ONCE;
-  if constexpr (OUT::CODES) {
-    if constexpr (TM == 1 && !OUT::GATED) linear_e4m3_stream_kernel<OUT, TM, 8><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-  } else {
-    if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-    else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-    else if constexpr (TM > 2) return;   // (not planned)
-    else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-    else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-  }
+  if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+  else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+  else if constexpr (TM > 2) return;   // (not planned)
+  else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+  else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per, once);
 }
 template <class OUT>
 void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
@@ -560,10 +539,11 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
     else if (p.splits == 4) linear_e4m3_join_kernel<OUT, 4><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else if (p.splits == 2) linear_e4m3_join_kernel<OUT, 2><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else linear_e4m3_join_kernel<OUT, 1><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
-  } else if (p.stream) {
-    launch_stream(P, out, p, OUT::CODES ? GROUP : stream_columns(c.N, c.gated != 0), s);
+  } else if constexpr (OUT::CODES) {
+    launch_tiles<OUT, false>(P, out, p, s);   // (the others' codes go through memory)
   } else {
-    launch_tiles<OUT, false>(P, out, p, s);
+    if (p.stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
+    else launch_tiles<OUT, false>(P, out, p, s);
   }
   return fs::launch_status("linear_e4m3");
 }

@@ -116,65 +116,65 @@ SIZES = {
     (5, 2441, 512, True, False): (16, 32, 1, 0), (9, 2050, 896, True, False): (16, 32, 1, 0),
     (6, 4224, 512, False, True): (16, 32, 1, 1), (5, 2176, 512, True, True): (16, 32, 1, 1),
     (5, 8444, 512, False, False): (16, 64, 1, 0), (5, 4420, 512, True, False): (16, 64, 1, 0),
-    (16, 5003, 512, True, False): (16, 64, 1, 0), (6, 4352, 512, True, True): (16, 64, 1, 1),
-    (5, 16852, 512, False, False): (16, 112, 1, 0), (5, 8954, 512, True, False): (16, 112, 1, 0),
+    (16, 5003, 512, True, False): (16, 64, 1, 0), (6, 8448, 512, False, True): (16, 64, 1, 1),
+    (6, 4352, 512, True, True): (16, 64, 1, 1), (5, 16852, 512, False, False): (16, 112, 1, 0),
+    (5, 8954, 512, True, False): (16, 112, 1, 0), (5, 17024, 640, False, True): (16, 112, 1, 1),
     (16, 14336, 512, True, True): (16, 112, 1, 1), (5, 8704, 512, True, True): (16, 112, 1, 1),
-    (5, 8064, 512, False, True): (16, 128, 1, 0), (31, 1537, 640, False, False): (32, 16, 1, 0),
-    (17, 1, 512, False, False): (32, 16, 1, 0), (17, 1, 512, True, False): (32, 16, 1, 0),
-    (17, 128, 512, False, True): (32, 16, 1, 1), (17, 128, 512, True, True): (32, 16, 1, 1),
-    (17, 4443, 512, False, False): (32, 32, 1, 0), (19, 2097, 512, True, False): (32, 32, 1, 0),
-    (17, 4864, 512, False, True): (32, 32, 1, 1), (17, 2432, 512, True, True): (32, 32, 1, 1),
-    (17, 9604, 512, False, False): (32, 64, 1, 0), (17, 4204, 512, True, False): (32, 64, 1, 0),
-    (18, 8576, 512, False, True): (32, 64, 1, 1), (20, 4224, 512, True, True): (32, 64, 1, 1),
-    (17, 17300, 512, False, False): (32, 112, 1, 0), (19, 8301, 512, True, False): (32, 112, 1, 0),
-    (17, 16640, 512, False, True): (32, 112, 1, 1), (19, 9088, 512, True, True): (32, 112, 1, 1),
-    (34, 1, 512, False, False): (64, 16, 1, 0), (33, 1, 512, True, False): (64, 16, 1, 0),
-    (33, 128, 512, False, True): (64, 16, 1, 1), (33, 128, 512, True, True): (64, 16, 1, 1),
-    (36, 4126, 512, False, False): (64, 32, 1, 0), (35, 2105, 512, True, False): (64, 32, 1, 0),
-    (36, 4736, 512, False, True): (64, 32, 1, 1), (36, 2176, 512, True, True): (64, 32, 1, 1),
-    (134, 1, 512, False, False): (64, 64, 1, 0), (134, 1, 512, True, False): (64, 64, 1, 0),
-    (65, 128, 4864, False, True): (64, 64, 1, 1), (129, 128, 1152, True, True): (64, 64, 1, 1),
-    (35, 4, 11264, False, False): (64, 64, 2, 1), (65, 128, 5120, False, True): (64, 64, 2, 1),
-    (73, 4, 5120, True, False): (64, 64, 2, 1), (129, 128, 1024, True, True): (64, 64, 2, 1),
-    (135, 4, 2048, False, False): (64, 64, 4, 1), (129, 128, 2048, False, True): (64, 64, 4, 1),
-    (134, 4, 2048, True, False): (64, 64, 4, 1), (129, 128, 2048, True, True): (64, 64, 4, 1),
-    (129, 4, 4096, False, False): (64, 64, 8, 1), (33, 128, 12288, False, True): (64, 64, 8, 1),
-    (129, 4, 4096, True, False): (64, 64, 8, 1), (33, 128, 12288, True, True): (64, 64, 8, 1),
-    (71, 16420, 512, False, False): (64, 128, 1, 0), (129, 128, 512, False, True): (64, 128, 1, 0),
-    (65, 8605, 512, True, False): (64, 128, 1, 0), (36, 17292, 4096, False, False): (64, 128, 2, 1),
-    (33, 16768, 4096, False, True): (64, 128, 2, 1), (36, 8724, 4096, True, False): (64, 128, 2, 1),
-    (35, 9644, 4096, False, False): (64, 128, 4, 1), (34, 10240, 2048, False, True): (64, 128, 4, 1),
-    (37, 4244, 4096, True, False): (64, 128, 4, 1), (2110, 68, 4096, False, False): (64, 128, 8, 1),
-    (133, 1408, 4096, False, True): (64, 128, 8, 1), (2205, 36, 4096, True, False): (64, 128, 8, 1),
-    (129, 128, 512, True, True): (64, 256, 1, 0), (65, 1, 512, False, False): (128, 16, 1, 0),
-    (65, 1, 512, True, False): (128, 16, 1, 0), (65, 128, 512, False, True): (128, 16, 1, 1),
-    (65, 128, 512, True, True): (128, 16, 1, 1), (67, 4172, 512, False, False): (128, 32, 1, 0),
-    (66, 2074, 512, True, False): (128, 32, 1, 0), (72, 4224, 512, False, True): (128, 32, 1, 1),
-    (72, 2176, 512, True, True): (128, 32, 1, 1), (75, 16940, 1536, False, False): (128, 128, 1, 0),
-    (130, 12032, 1408, False, True): (128, 128, 1, 0), (70, 9399, 1664, True, False): (128, 128, 1, 0),
-    (79, 8320, 5248, True, True): (128, 128, 1, 1), (72, 8204, 4096, False, False): (128, 128, 2, 1),
-    (66, 8320, 4096, False, True): (128, 128, 2, 1), (76, 4164, 4096, True, False): (128, 128, 2, 1),
-    (70, 5120, 2048, True, True): (128, 128, 2, 1), (133, 2836, 4096, False, False): (128, 128, 4, 1),
-    (132, 2816, 4096, False, True): (128, 128, 4, 1), (2754, 68, 4096, True, False): (128, 128, 4, 1),
-    (135, 1408, 4096, True, True): (128, 128, 4, 1), (2052, 68, 8192, False, False): (128, 128, 8, 1),
-    (69, 2176, 8192, False, True): (128, 128, 8, 1), (2073, 36, 8192, True, False): (128, 128, 8, 1),
-    (75, 1280, 8192, True, True): (128, 128, 8, 1), (71, 17024, 512, True, True): (128, 256, 1, 0),
-    (394, 9433, 1152, False, False): (256, 128, 1, 0), (258, 13184, 1152, False, True): (256, 128, 1, 0),
-    (134, 12083, 1152, True, False): (256, 128, 1, 0), (158, 13364, 9216, False, False): (256, 128, 2, 1),
-    (173, 12288, 7168, False, True): (256, 128, 2, 1), (732, 1372, 7168, True, False): (256, 128, 2, 1),
-    (131, 5632, 4096, True, True): (256, 128, 2, 1), (140, 6116, 8192, False, False): (256, 128, 4, 1),
-    (220, 4352, 6144, False, True): (256, 128, 4, 1), (263, 1652, 8192, True, False): (256, 128, 4, 1),
-    (134, 3200, 8192, True, True): (256, 128, 4, 1), (146, 2884, 16384, False, False): (256, 128, 8, 1),
-    (135, 2816, 16384, False, True): (256, 128, 8, 1), (2797, 68, 16384, True, False): (256, 128, 8, 1),
-    (130, 1408, 16384, True, True): (256, 128, 8, 1), (1713, 4893, 1408, False, False): (256, 256, 1, 0),
-    (1689, 4864, 1408, False, True): (256, 256, 1, 0), (259, 14221, 1408, True, False): (256, 256, 1, 0),
-    (200, 17920, 512, True, True): (256, 256, 1, 0), (1848, 2180, 7168, False, False): (256, 256, 2, 1),
-    (468, 9216, 6144, False, True): (256, 256, 2, 1), (366, 5524, 6144, True, False): (256, 256, 2, 1),
-    (138, 11392, 5120, True, True): (256, 256, 2, 1), (138, 10996, 8192, False, False): (256, 256, 4, 1),
-    (141, 11008, 8192, False, True): (256, 256, 4, 1), (193, 4108, 8192, True, False): (256, 256, 4, 1),
-    (132, 4608, 8192, True, True): (256, 256, 4, 1), (2711, 260, 16384, False, False): (256, 256, 8, 1),
-    (137, 5760, 16384, False, True): (256, 256, 8, 1), (2797, 132, 16384, True, False): (256, 256, 8, 1),
-    (131, 2176, 16384, True, True): (256, 256, 8, 1),
+    (31, 1537, 640, False, False): (32, 16, 1, 0), (17, 1, 512, False, False): (32, 16, 1, 0),
+    (17, 1, 512, True, False): (32, 16, 1, 0), (17, 128, 512, False, True): (32, 16, 1, 1),
+    (17, 128, 512, True, True): (32, 16, 1, 1), (17, 4443, 512, False, False): (32, 32, 1, 0),
+    (19, 2097, 512, True, False): (32, 32, 1, 0), (17, 4864, 512, False, True): (32, 32, 1, 1),
+    (17, 2432, 512, True, True): (32, 32, 1, 1), (17, 9604, 512, False, False): (32, 64, 1, 0),
+    (17, 4204, 512, True, False): (32, 64, 1, 0), (18, 8576, 512, False, True): (32, 64, 1, 1),
+    (20, 4224, 512, True, True): (32, 64, 1, 1), (17, 17300, 512, False, False): (32, 112, 1, 0),
+    (19, 8301, 512, True, False): (32, 112, 1, 0), (17, 16640, 512, False, True): (32, 112, 1, 1),
+    (19, 9088, 512, True, True): (32, 112, 1, 1), (34, 1, 512, False, False): (64, 16, 1, 0),
+    (33, 1, 512, True, False): (64, 16, 1, 0), (33, 128, 512, False, True): (64, 16, 1, 1),
+    (33, 128, 512, True, True): (64, 16, 1, 1), (36, 4126, 512, False, False): (64, 32, 1, 0),
+    (35, 2105, 512, True, False): (64, 32, 1, 0), (36, 4736, 512, False, True): (64, 32, 1, 1),
+    (36, 2176, 512, True, True): (64, 32, 1, 1), (134, 1, 512, False, False): (64, 64, 1, 0),
+    (134, 1, 512, True, False): (64, 64, 1, 0), (65, 128, 4864, False, True): (64, 64, 1, 1),
+    (129, 128, 1152, True, True): (64, 64, 1, 1), (35, 4, 11264, False, False): (64, 64, 2, 1),
+    (65, 128, 5120, False, True): (64, 64, 2, 1), (73, 4, 5120, True, False): (64, 64, 2, 1),
+    (129, 128, 1024, True, True): (64, 64, 2, 1), (135, 4, 2048, False, False): (64, 64, 4, 1),
+    (129, 128, 2048, False, True): (64, 64, 4, 1), (134, 4, 2048, True, False): (64, 64, 4, 1),
+    (129, 128, 2048, True, True): (64, 64, 4, 1), (129, 4, 4096, False, False): (64, 64, 8, 1),
+    (33, 128, 12288, False, True): (64, 64, 8, 1), (129, 4, 4096, True, False): (64, 64, 8, 1),
+    (33, 128, 12288, True, True): (64, 64, 8, 1), (71, 16420, 512, False, False): (64, 128, 1, 0),
+    (129, 128, 512, False, True): (64, 128, 1, 0), (65, 8605, 512, True, False): (64, 128, 1, 0),
+    (36, 17292, 4096, False, False): (64, 128, 2, 1), (33, 16768, 4096, False, True): (64, 128, 2, 1),
+    (36, 8724, 4096, True, False): (64, 128, 2, 1), (35, 9644, 4096, False, False): (64, 128, 4, 1),
+    (34, 10240, 2048, False, True): (64, 128, 4, 1), (37, 4244, 4096, True, False): (64, 128, 4, 1),
+    (2110, 68, 4096, False, False): (64, 128, 8, 1), (133, 1408, 4096, False, True): (64, 128, 8, 1),
+    (2205, 36, 4096, True, False): (64, 128, 8, 1), (129, 128, 512, True, True): (64, 256, 1, 0),
+    (65, 1, 512, False, False): (128, 16, 1, 0), (65, 1, 512, True, False): (128, 16, 1, 0),
+    (65, 128, 512, False, True): (128, 16, 1, 1), (65, 128, 512, True, True): (128, 16, 1, 1),
+    (67, 4172, 512, False, False): (128, 32, 1, 0), (66, 2074, 512, True, False): (128, 32, 1, 0),
+    (72, 4224, 512, False, True): (128, 32, 1, 1), (72, 2176, 512, True, True): (128, 32, 1, 1),
+    (75, 16940, 1536, False, False): (128, 128, 1, 0), (130, 12032, 1408, False, True): (128, 128, 1, 0),
+    (70, 9399, 1664, True, False): (128, 128, 1, 0), (79, 8320, 5248, True, True): (128, 128, 1, 1),
+    (72, 8204, 4096, False, False): (128, 128, 2, 1), (66, 8320, 4096, False, True): (128, 128, 2, 1),
+    (76, 4164, 4096, True, False): (128, 128, 2, 1), (70, 5120, 2048, True, True): (128, 128, 2, 1),
+    (133, 2836, 4096, False, False): (128, 128, 4, 1), (132, 2816, 4096, False, True): (128, 128, 4, 1),
+    (2754, 68, 4096, True, False): (128, 128, 4, 1), (135, 1408, 4096, True, True): (128, 128, 4, 1),
+    (2052, 68, 8192, False, False): (128, 128, 8, 1), (69, 2176, 8192, False, True): (128, 128, 8, 1),
+    (2073, 36, 8192, True, False): (128, 128, 8, 1), (75, 1280, 8192, True, True): (128, 128, 8, 1),
+    (71, 17024, 512, True, True): (128, 256, 1, 0), (394, 9433, 1152, False, False): (256, 128, 1, 0),
+    (258, 13184, 1152, False, True): (256, 128, 1, 0), (134, 12083, 1152, True, False): (256, 128, 1, 0),
+    (158, 13364, 9216, False, False): (256, 128, 2, 1), (173, 12288, 7168, False, True): (256, 128, 2, 1),
+    (732, 1372, 7168, True, False): (256, 128, 2, 1), (131, 5632, 4096, True, True): (256, 128, 2, 1),
+    (140, 6116, 8192, False, False): (256, 128, 4, 1), (220, 4352, 6144, False, True): (256, 128, 4, 1),
+    (263, 1652, 8192, True, False): (256, 128, 4, 1), (134, 3200, 8192, True, True): (256, 128, 4, 1),
+    (146, 2884, 16384, False, False): (256, 128, 8, 1), (135, 2816, 16384, False, True): (256, 128, 8, 1),
+    (2797, 68, 16384, True, False): (256, 128, 8, 1), (130, 1408, 16384, True, True): (256, 128, 8, 1),
+    (1713, 4893, 1408, False, False): (256, 256, 1, 0), (1689, 4864, 1408, False, True): (256, 256, 1, 0),
+    (259, 14221, 1408, True, False): (256, 256, 1, 0), (200, 17920, 512, True, True): (256, 256, 1, 0),
+    (1848, 2180, 7168, False, False): (256, 256, 2, 1), (468, 9216, 6144, False, True): (256, 256, 2, 1),
+    (366, 5524, 6144, True, False): (256, 256, 2, 1), (138, 11392, 5120, True, True): (256, 256, 2, 1),
+    (138, 10996, 8192, False, False): (256, 256, 4, 1), (141, 11008, 8192, False, True): (256, 256, 4, 1),
+    (193, 4108, 8192, True, False): (256, 256, 4, 1), (132, 4608, 8192, True, True): (256, 256, 4, 1),
+    (2711, 260, 16384, False, False): (256, 256, 8, 1), (137, 5760, 16384, False, True): (256, 256, 8, 1),
+    (2797, 132, 16384, True, False): (256, 256, 8, 1), (131, 2176, 16384, True, True): (256, 256, 8, 1),
 }
 
 
