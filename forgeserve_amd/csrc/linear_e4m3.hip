@@ -33,7 +33,8 @@ FS_DEVICE float over_one_plus_exp(float z, float y) {
 }
 // z Phi(z) with Phi(-a) = erfc(a / sqrt 2) / 2 = e^(-a^2 / 2) t Q(t) / 2, t = 1 / (1 + 0.4 a / sqrt 2): Q, of degree 6, is
 // the polynomial whose largest relative error over 0 <= a <= 19.8 is least (3.5e-6, fitted to scipy's erfcx). The result is
-// within 8e-6 of itself in both tails, a thirtieth of f16's rounding.
+// within 8e-6 of itself in both tails, a thirtieth of f16's rounding. About 22 instructions of a lane, 2.5 us of 333 x 8192's
+// 17.2, which the vector units set.
 FS_DEVICE float gelu_erf(float z) {
   const float a = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(a, 0.282842712f, 1.f));
   float q = -0.0880692603f;
@@ -206,7 +207,8 @@ struct LinearOut {
 };
 
 // The SPLITS sums in memory added in order and finished, eight columns of the results a thread (N % 4 == 0: rows of W); every
-// load ahead of the first addition.
+// load ahead of the first addition, for what it takes is their latency: 160 x 2048 of eight splits, 10 MB out of the caches, 4.1
+// us, the gate of 1 x 28672 4.0 (one load after another 160 x 2048 x 8192 took 1.6 us more).
 template <class OUT, int SPLITS>
 __global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __restrict__ part, int64_t M, int64_t N,
                                                                uint32_t pieces, OUT out) {
