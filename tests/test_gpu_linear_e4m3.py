@@ -209,6 +209,23 @@ def test_linear(size, dtype):
         assert (back[:, : 8 + shift] == 3).all() and (back[:, 8 + shift + n:] == 3).all()
 
 
+@pytest.mark.parametrize("m,n,k,gated", [(3, 4100, 8320, False), (17, 20000, 1792, False), (8, 12000, 2944, True), (33, 4096, 8192, False),
+                                         (100, 8192, 4096, False), (2, 9000, 128, False), (2, 9000, 640, False), (1, 9003, 1152, True)])
+@gpu
+def test_wide_and_large_weights_of_short_batches(m, n, k, gated):
+    """Weights of more than 32 MB are read past the caches; where a workgroup has many rows of W its waves begin at different
+    stages, with one more stage for some waves, or none for some."""
+    assert plan(m, n, k, gated, False)[0] in (16, 32, 64, 128)
+    x, w, bias, r = operands(m, n, k, gated, BF16)
+    a, a_scales = ops.quantize_e4m3(x)
+    want = wanted(decoded(a, a_scales), decoded(*w), bias, "silu", gated, r)
+    y = ops.linear_e4m3(a, *w, a_scales=a_scales, bias=bias, activation="silu", gated=gated, residual=r)
+    close(y, *want)
+    # rows do not depend on which of the batch they are, nor on what lies behind them
+    assert torch.equal(ops.linear_e4m3(a.flip(0), *w, a_scales=a_scales.flip(1).contiguous(), bias=bias, activation="silu",
+                                       gated=gated, residual=r.flip(0)).flip(0), y)
+
+
 def test_the_sizes_take_every_kernel():
     assert {size: plan(*size) for size in SIZES} == SIZES
 
