@@ -208,7 +208,7 @@ struct LinearOut {
 
 // The SPLITS sums in memory added in order and finished, eight columns of the results a thread (N % 4 == 0: rows of W); every
 // load ahead of the first addition, for what it takes is their latency: 160 x 2048 of eight splits, 10 MB out of the caches, 4.1
-// us, the gate of 1 x 28672 4.0 (one load after another 160 x 2048 x 8192 took 1.6 us more).
+// us, of four 3.8, the gate of 1 x 28672 4.0 (one load after another 160 x 2048 of eight took 1.6 us more).
 template <class OUT, int SPLITS>
 __global__ void __launch_bounds__(256) linear_e4m3_join_kernel(const float* __restrict__ part, int64_t M, int64_t N,
                                                                uint32_t pieces, OUT out) {
@@ -428,7 +428,7 @@ int stream_tiles(int64_t cols, bool gated) {
 }
 
 // Tiles: the cheapest of what a sweep over 26 shapes of 40 to 4000 rows fits (us; by 4 to 12 % rms, and its choice is within
-// 1.4 % of the best one's time on average, 9 % at most): `first` for a grid, `round` for each further round of the CUs' places
+// 1 % of the best one's time on average, 7 % at most): `first` for a grid, `round` for each further round of the CUs' places
 // (two of the smaller tiles share a CU: stage2 for both), a stage of 128, and a MB of results or of sums in memory. Codes
 // leave tiles of 128 columns by themselves, a gate's tiles of 256; other sums go through memory, as those of K splits do.
 Plan plan_for(const fs_linear& c) {
@@ -464,7 +464,7 @@ Plan plan_for(const fs_linear& c) {
       const double two = t.stage2 > 0.0 ? (double)(wgs / places + (rest > 256)) : 0.0;
       const double out_mb = (double)M * (double)N * 2e-6, sums_mb = 2.0 * s * out_mb;
       const double us = t.first + t.round * (one + two - 1.0) + (double)(nk / s) * (one * t.stage + two * t.stage2) +
-                        (join ? t.sums_mb * sums_mb + 2.9 + 0.125 * sums_mb + 0.05 * out_mb : t.out_mb * out_mb);
+                        (join ? t.sums_mb * sums_mb + (s == 8 ? 3.9 : 2.9) + 0.125 * sums_mb + 0.05 * out_mb : t.out_mb * out_mb);
       if (us < least) least = us, best = Plan{t.bm, t.bn, s, join, false};
     }
   }

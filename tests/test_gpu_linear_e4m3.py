@@ -145,8 +145,8 @@ SIZES = {
     (36, 17292, 4096, False, False): (64, 128, 2, 1), (33, 16768, 4096, False, True): (64, 128, 2, 1),
     (36, 8724, 4096, True, False): (64, 128, 2, 1), (35, 9644, 4096, False, False): (64, 128, 4, 1),
     (34, 10240, 2048, False, True): (64, 128, 4, 1), (37, 4244, 4096, True, False): (64, 128, 4, 1),
-    (2110, 68, 4096, False, False): (64, 128, 8, 1), (133, 1408, 4096, False, True): (64, 128, 8, 1),
-    (2205, 36, 4096, True, False): (64, 128, 8, 1), (129, 128, 512, True, True): (64, 256, 1, 0),
+    (37, 4356, 16384, False, False): (64, 128, 8, 1), (39, 4608, 12288, False, True): (64, 128, 8, 1),
+    (40, 2068, 16384, True, False): (64, 128, 8, 1), (129, 128, 512, True, True): (64, 256, 1, 0),
     (65, 1, 512, False, False): (128, 16, 1, 0), (65, 1, 512, True, False): (128, 16, 1, 0),
     (65, 128, 512, False, True): (128, 16, 1, 1), (65, 128, 512, True, True): (128, 16, 1, 1),
     (67, 4172, 512, False, False): (128, 32, 1, 0), (66, 2074, 512, True, False): (128, 32, 1, 0),
