@@ -1016,14 +1016,15 @@ constexpr int PF_MIN_QTILES = 5; // a call with at least this many query tiles p
 // One 16-byte copy per lane straight into LDS from sbase + voff (a wave-uniform base in SGPRs and a
 // 32-bit unsigned per-lane byte offset; lane l lands at lds + 16 * l, the same base for the whole
 // wave). The copy is counted by vmcnt like any vector load; the waits below are explicit.
+// (s_nop: a copy may read m0 one wait state behind its writing, and inside the asm the compiler puts none.)
 FS_DEVICE void pf_dma16(const void* sbase, uint32_t voff, uint32_t lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(l) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(l) : "memory", "m0");
 }
 // 4 bytes per lane from an address of its own; lane l lands at lds + 4 * l.
 FS_DEVICE void pf_dma4(const void* src, uint32_t lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(l) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(l) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 template <int N>

@@ -148,15 +148,16 @@ __global__ void __launch_bounds__(256) gemm_bf16_kernel(const uint16_t* __restri
 // ------------------------------------------------------------------------------------------------
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+// (s_nop: a copy may read m0 one wait state behind its writing, and inside the asm the compiler puts none.)
 FS_DEVICE void dma16(const void* g, uint32_t lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane(lds);  // the LDS base is the same for the whole wave
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(l) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(l) : "memory", "m0");
 }
 // the same copy marked non-temporal: the weights stream through once, and keeping them out of the way
 // in L2 leaves the activation panel (re-read by every column tile) resident (about 3% at M = 448)
 FS_DEVICE void dma16_nt(const void* g, uint32_t lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(g), "s"(l) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(g), "s"(l) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN) gemm_bf16_lds_kernel(const uin
 #pragma clang diagnostic ignored "-Winline-asm"
 // dma16 from a wave-uniform base and a 32-bit byte offset per lane
 FS_DEVICE void dma16_at(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
