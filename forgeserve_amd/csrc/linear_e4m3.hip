@@ -579,8 +579,8 @@ int check(const fs_linear* c, const char* what, Plan& p) {
   // a copy's offset inside its tile of rows, and a row's scale word inside its group of K, are 32 bits
   FS_CHECK_ARG(c->K <= (1 << 22) && c->M < (1 << 29) && c->N < (1 << 28), "%s: M %lld N %lld K %lld", what, (long long)c->M,
                (long long)c->N, (long long)c->K);
-  // 2^32 threads a launch: 64 for a row's 512 columns that are encoded, 512 a tile, one for eight columns from memory
-  FS_CHECK_ARG(c->x_scales || c->M * ((c->K + 511) / 512) < (1 << 26), "%s: M %lld K %lld", what, (long long)c->M,
+  // below 2^32 threads a launch: 64 for a row's 512 columns that are encoded, 512 a tile, one for eight columns from memory
+  FS_CHECK_ARG(c->x_scales || waves_fit(c->M * ((c->K + 511) / 512)), "%s: M %lld K %lld", what, (long long)c->M,
                (long long)c->K);
   FS_CHECK_ARG(!c->out_scales || c->N % GROUP == 0, "%s: codes of %lld columns (a multiple of %d)", what, (long long)c->N, GROUP);
   p = plan_for(*c);

@@ -236,7 +236,8 @@ extern "C" int fs_add_rmsnorm_e4m3(const void* x, int64_t ldx, const void* delta
   FS_CHECK_ARG(dtype_ok(dtype), "add_rmsnorm_e4m3: dtype %d", dtype);
   FS_CHECK_ARG(M >= 0 && N > 0 && N % GROUP == 0 && N < 0x7fff0000, "add_rmsnorm_e4m3: M %lld N %lld (a multiple of %d)",
                (long long)M, (long long)N, GROUP);
-  FS_CHECK_ARG(M < (N <= 1024 ? 1 << 26 : 1 << 22), "add_rmsnorm_e4m3: M %lld N %lld", (long long)M, (long long)N);   // (2^32 threads)
+  // (below 2^32 threads: a wave a row, or up to 1024 threads)
+  FS_CHECK_ARG(N <= 1024 ? waves_fit(M) : M < (1 << 22), "add_rmsnorm_e4m3: M %lld N %lld", (long long)M, (long long)N);
   FS_CHECK_ARG(ldx >= N && ldc >= N && (!delta || (ldd >= N && ldxo >= N)), "add_rmsnorm_e4m3: leading dimensions");
   FS_CHECK_ARG(ldc % 16 == 0 && al16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
                "add_rmsnorm_e4m3: codes need 16-byte aligned rows, scales whole words");
@@ -261,7 +262,7 @@ extern "C" int fs_dequantize_e4m3(const void* codes, int64_t ldc, const void* sc
                (long long)rows, (long long)K, GROUP);
   FS_CHECK_ARG(ldc % 16 == 0 && al16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
                "dequantize_e4m3: codes need 16-byte aligned rows, scales whole words");
-  FS_CHECK_ARG(rows < (1 << 26) && rows * ((K + 511) / 512) < (1 << 26), "dequantize_e4m3: rows %lld K %lld", (long long)rows, (long long)K);
+  FS_CHECK_ARG(rows < (1 << 26) && waves_fit(rows * ((K + 511) / 512)), "dequantize_e4m3: rows %lld K %lld", (long long)rows, (long long)K);
   if (rows == 0) return 0;
   const int64_t kw = (K + 511) / 512;
   const dim3 grid((unsigned)((rows * kw + 3) / 4));

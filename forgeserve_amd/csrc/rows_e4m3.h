@@ -145,6 +145,8 @@ inline bool rows_by_8(const void* C, int64_t ldc, const void* R, int64_t ldr) {
 }
 
 inline int64_t scale_bytes(int64_t rows, int64_t K) { return (K + 511) / 512 * rows * 4; }
+// Whether a launch of so many waves, four a workgroup, stays below 2^32 threads.
+inline bool waves_fit(int64_t waves) { return waves <= (1 << 26) - 4; }
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
