@@ -136,6 +136,16 @@ int short_tiles(int64_t N) {
   const int64_t tiles = (N + 15) / 16;
   return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4;
 }
+// Whether a call's launches stay below 2^32 threads: a wave for a row's 512 columns that are encoded, a workgroup a tile
+// (these in eights), a thread for four columns of joined splits.
+bool launches_fit(int64_t M, int64_t N, int64_t K, bool in_one) {
+  constexpr int64_t LIMIT = 1LL << 32;
+  if (in_one) return ((N + 15) / 16 + short_tiles(N) - 1) / short_tiles(N) * 512 < LIMIT;
+  const Plan p = plan_for(M, N, K);
+  const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
+  return waves_fit(M * ((K + 511) / 512)) && (tiles + 7) / 8 * 8 * (p.bm == 64 ? 256 : 512) < LIMIT &&
+         (p.splits == 1 || M * N / 4 + 256 <= LIMIT);
+}
 
 }  // namespace
 
@@ -218,7 +228,7 @@ extern "C" int fs_quantize_e4m3(const void* X, int64_t ldx, int64_t rows, int64_
                (long long)rows, (long long)K, GROUP);
   FS_CHECK_ARG(ldc % 16 == 0 && al16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
                "quantize_e4m3: codes need 16-byte aligned rows, scales whole words");
-  FS_CHECK_ARG(rows * ((K + 511) / 512) < 0x7fffffffLL, "quantize_e4m3: rows %lld K %lld", (long long)rows, (long long)K);
+  FS_CHECK_ARG(rows < (1 << 26) && waves_fit(rows * ((K + 511) / 512)), "quantize_e4m3: rows %lld K %lld", (long long)rows, (long long)K);
   if (rows == 0) return 0;
   fs::quantize_rows_e4m3(X, ldx, rows, K, dtype, reinterpret_cast<uint8_t*>(codes), ldc, reinterpret_cast<uint32_t*>(scales), fs::as_stream(stream));
   return fs::launch_status("quantize_e4m3");
@@ -255,6 +265,8 @@ extern "C" int fs_gemm_e4m3(const void* X, int64_t ldx, const void* W, int64_t l
   FS_CHECK_ARG(K <= (1 << 22) && ldw < (1 << 23) && M < (1 << 29) && N < (1 << 29), "gemm_e4m3: M %lld N %lld K %lld ldw %lld",
                (long long)M, (long long)N, (long long)K, (long long)ldw);
   if (M == 0) return 0;
+  FS_CHECK_ARG(launches_fit(M, N, K, short_call(M, N, K, X, ldx)), "gemm_e4m3: M %lld N %lld K %lld", (long long)M, (long long)N,
+               (long long)K);
   const int64_t need = fs_gemm_e4m3_workspace_size(M, N, K);
   FS_CHECK_ARG(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "gemm_e4m3: workspace %lld < %lld bytes (or not 256-byte aligned)", (long long)workspace_bytes, (long long)need);

@@ -39,3 +39,17 @@ def test_norm(lib, m, n):
 def test_values(lib, rows, k):
     assert lib.fs_dequantize_e4m3(256, k, 256, rows, k, _lib.BF16, 256, k, None) == -1
     assert b"dequantize_e4m3: rows" in lib.fs_last_error()
+
+
+@pytest.mark.parametrize("rows,k", [(MOST + 1, 128), (MOST + 3, 512), (MOST // 2 + 1, 640), (1 << 29, 128)])
+def test_encoding(lib, rows, k):
+    assert lib.fs_quantize_e4m3(256, k, rows, k, _lib.BF16, 256, k, 256, None) == -1
+    assert b"quantize_e4m3: rows" in lib.fs_last_error()
+
+
+@pytest.mark.parametrize("m,n,k", [(MOST + 1, 1, 128), (MOST + 3, 1, 512), (MOST // 2 + 1, 1, 640), (1 << 28, 1, 128), (1 << 25, 1 << 20, 128),
+                                   (1, (1 << 29) - 1, 128)])
+def test_product(lib, m, n, k):
+    """Its rows' encoding, and its tiles."""
+    assert lib.fs_gemm_e4m3(256, k, 256, k, 256, 256, n, None, 0, m, n, k, _lib.BF16, 256, 1 << 62, None) == -1
+    assert b"gemm_e4m3: M" in lib.fs_last_error()
