@@ -476,41 +476,54 @@ int64_t sums_bytes(const fs_linear& c, const Plan& p) {
   return p.join ? (int64_t)p.splits * c.M * weight_rows(c) * (int64_t)sizeof(float) : 0;
 }
 
+// The launchers: false, with nothing launched, of a plan that no kernel here takes.
 template <class OUT, int TM>
-void launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
+bool launch_stream(const Operands& P, const OUT& out, int tn, int64_t per, hipStream_t s) {
   const int64_t cols = OUT::GATED ? P.N / 2 : P.N;
+  if (P.M > 16 * TM || per > tn * (OUT::GATED ? 8 : 16)) return false;   // (rows or columns that nobody takes)
   const dim3 grid((unsigned)((cols + per - 1) / per));
   const bool once = P.N * P.nk * GROUP >= READ_ONCE;
   if (tn == 1) linear_e4m3_stream_kernel<OUT, TM, 1><<<grid, 512, 0, s>>>(P, out, (int)per, once);
   else if (tn == 2) linear_e4m3_stream_kernel<OUT, TM, 2><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-  else if constexpr (TM > 2) return;   // (not planned)
+  else if constexpr (TM > 2) return false;
   else if (tn == 4) linear_e4m3_stream_kernel<OUT, TM, 4><<<grid, 512, 0, s>>>(P, out, (int)per, once);
-  else linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+  else if (tn == 7) linear_e4m3_stream_kernel<OUT, TM, 7><<<grid, 512, 0, s>>>(P, out, (int)per, once);
+  else return false;
+  return true;
 }
 template <class OUT>
-void launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
+bool launch_stream(const Operands& P, const OUT& out, const Plan& p, int64_t per, hipStream_t s) {
   const int tn = p.bn / 16;
-  if (p.bm == 16) launch_stream<OUT, 1>(P, out, tn, per, s);
-  else if (p.bm == 32) launch_stream<OUT, 2>(P, out, tn, per, s);
-  else if (p.bm == 64) launch_stream<OUT, 4>(P, out, tn, per, s);
-  else launch_stream<OUT, 8>(P, out, tn, per, s);
+  switch (p.splits == 1 ? p.bm : 0) {
+    case 16: return launch_stream<OUT, 1>(P, out, tn, per, s);
+    case 32: return launch_stream<OUT, 2>(P, out, tn, per, s);
+    case 64: return launch_stream<OUT, 4>(P, out, tn, per, s);
+    case 128: return launch_stream<OUT, 8>(P, out, tn, per, s);
+    default: return false;
+  }
 }
 
 // PARTS: a class of which only the sums in memory are asked for.
 template <class OUT, bool PARTS>
-void launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t s) {
+bool launch_tiles(const Operands& P, const OUT& out, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(8 * ((P.ntiles + 7) / 8)), (unsigned)p.splits);
-  if (p.bn == 256 && p.bm == 256) {
+  const auto tile = [&](int bm, int bn) { return p.bm == bm && p.bn == bn; };
+  if (p.stream || (!PARTS && p.splits != 1)) return false;
+  if (tile(256, 256)) {
     gemm_e4m3_long_kernel<OUT, PARTS><<<grid, 512, 0, s>>>(P, out);
   } else if constexpr (OUT::CODES && OUT::GATED) {
-    if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 256, 2, 4, 3><<<grid, 512, 0, s>>>(P, out);
-    else gemm_e4m3_tile_kernel<OUT, 64, 256, 1, 8, 3><<<grid, 512, 0, s>>>(P, out);
+    if (tile(128, 256)) gemm_e4m3_tile_kernel<OUT, 128, 256, 2, 4, 3><<<grid, 512, 0, s>>>(P, out);
+    else if (tile(64, 256)) gemm_e4m3_tile_kernel<OUT, 64, 256, 1, 8, 3><<<grid, 512, 0, s>>>(P, out);
+    else return false;
   } else {
-    if (p.bm == 256) gemm_e4m3_tile_kernel<OUT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, out);
-    else if (p.bm == 128) gemm_e4m3_tile_kernel<OUT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, out);
-    else if (p.bn == 128) gemm_e4m3_tile_kernel<OUT, 64, 128, 2, 2, 3><<<grid, 256, 0, s>>>(P, out);
-    else if constexpr (!OUT::CODES) gemm_e4m3_tile_kernel<OUT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, out);
+    if (tile(256, 128)) gemm_e4m3_tile_kernel<OUT, 256, 128, 4, 2, 3><<<grid, 512, 0, s>>>(P, out);
+    else if (tile(128, 128)) gemm_e4m3_tile_kernel<OUT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(P, out);
+    else if (tile(64, 128)) gemm_e4m3_tile_kernel<OUT, 64, 128, 2, 2, 3><<<grid, 256, 0, s>>>(P, out);
+    else if constexpr (OUT::CODES) return false;
+    else if (tile(64, 64)) gemm_e4m3_tile_kernel<OUT, 64, 64, 2, 2, 4><<<grid, 256, 0, s>>>(P, out);
+    else return false;
   }
+  return true;
 }
 
 template <class OUT>
@@ -529,23 +542,27 @@ int run(const fs_linear& c, Operands P, const Plan& p, float* part, hipStream_t 
   out.scales = reinterpret_cast<uint8_t*>(c.out_scales);
   out.rows = c.M;
   out.part = nullptr;
+  bool done = false;
   if (p.join) {
     typedef LinearOut<false, false> Sums;
     Sums sums{};
     sums.part = part;
-    if (p.stream) launch_stream(P, sums, p, stream_columns(P.N, false), s);   // (rows of W in their order, gated or not)
-    else launch_tiles<Sums, true>(P, sums, p, s);
+    if (p.splits == 1 || p.splits == 2 || p.splits == 4 || p.splits == 8)   // (what the join takes)
+      done = p.stream ? launch_stream(P, sums, p, stream_columns(P.N, false), s)   // (rows of W in their order, gated or not)
+                      : launch_tiles<Sums, true>(P, sums, p, s);
+  } else if constexpr (OUT::CODES) {
+    done = launch_tiles<OUT, false>(P, out, p, s);   // (the others' codes go through memory)
+  } else {
+    done = p.stream ? launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s) : launch_tiles<OUT, false>(P, out, p, s);
+  }
+  FS_CHECK_ARG(done, "linear_e4m3: no kernel of %d x %d, %d splits, %d %d", p.bm, p.bn, p.splits, p.join, p.stream);
+  if (p.join) {
     const uint32_t pieces = (uint32_t)((c.N + 7) / 8);
     const dim3 grid((unsigned)((c.M * pieces + 255) / 256));
     if (p.splits == 8) linear_e4m3_join_kernel<OUT, 8><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else if (p.splits == 4) linear_e4m3_join_kernel<OUT, 4><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else if (p.splits == 2) linear_e4m3_join_kernel<OUT, 2><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
     else linear_e4m3_join_kernel<OUT, 1><<<grid, 256, 0, s>>>(part, P.M, P.N, pieces, out);
-  } else if constexpr (OUT::CODES) {
-    launch_tiles<OUT, false>(P, out, p, s);   // (the others' codes go through memory)
-  } else {
-    if (p.stream) launch_stream(P, out, p, stream_columns(c.N, c.gated != 0), s);
-    else launch_tiles<OUT, false>(P, out, p, s);
   }
   return fs::launch_status("linear_e4m3");
 }
