@@ -11,14 +11,19 @@
 
 namespace {
 
-// Rows that the kernels without tiles in LDS may take, and, of more than 32, their codes: every workgroup reads them, for one
-// or two tiles of W (64 x 4096 x 4096 8.2 us, in tiles 11.9; 128 x 6144 x 4096 13.5 and 14.5; 64 x 2048 x 8192 10.3 and 13.2;
-// over the limit 64 x 4096 x 14336 24.4 and 19.8, 96 x 2048 x 8192 14.6 and 13.5; four tiles, 64 x 16384 x 2048, 11.1 and 9.8).
+// Rows that the streaming kernels may take, and, of more than 32, the bytes of their codes: every workgroup copies them all,
+// beside one or two tiles of W. us, streamed and in tiles, of one weight called again and again / of 1 GB of weights in turn:
+// 64 x 4096 x 4096 8.2 and 10.4 / 9.5 and 11.3; 100 x 4096 x 4096 10.7 and 12.6 / 11.5 and 14.3; 128 x 6144 x 4096 13.8 and 15.3 /
+// 15.3 and 14.5; 64 x 2048 x 8192 10.6 and 10.4 / 12.6 and 11.3; over the limit 64 x 4096 x 14336 23.3 and 17.3 / 22.2 and 18.9, 96
+// x 2048 x 8192 14.7 and 12.4 / 16.6 and 12.4; with four tiles 64 x 16384 x 2048 11.1 and 9.8.
 constexpr int STREAM_ROWS = 128;
 constexpr int64_t STREAM_BYTES = 600 * 1024;
 // Bytes of W from which they are read past the caches (`nt`): of a weight's size several pass between two calls that read the
-// same one, and then the caches have none of it (1 x 4096 x 14336 12.9 -> 11.8 us; with the next comment's turns 1 x 128256 x
-// 4096 91.4 -> 82.5). Smaller ones may still be there (8 x 6144 x 4096 7.1 us, read past them 8.0; out of HBM 8.0 and 7.3).
+// same one, and then the caches have none of it. us, past them and through them, of one weight called again and again / of 1 GB
+// of weights in turn: 1 x 4096 x 14336 11.5 and 12.5 / 12.1 and 13.0; 1 x 28672 x 4096 20.3 and 21.8 / 21.5 and 23.8; 1 x 128256 x
+// 4096 82.6 and 91.9 / 81.4 and 89.5. Smaller ones are read through them, for they may still be there; that wins nothing to speak
+// of (64 x 4096 x 4096 8.8 and 8.5, 8 x 6144 x 4096 5.8 both), and costs 4 to 8 % where a model's other layers pass in between, as
+// in its decode steps (9.0 and 9.4; 7.7 and 8.3).
 constexpr int64_t READ_ONCE = 32 << 20;
 
 // ------------------------------------------------------------------------------------------------
@@ -412,11 +417,11 @@ __global__ void __launch_bounds__(512) linear_e4m3_stream_kernel(Operands P, OUT
 struct Plan {
   int bm, bn, splits;
   bool join;     // the sums through memory
-  bool stream;   // no tiles in LDS
+  bool stream;   // the streaming kernel: every wave its own part of K, no tile in LDS that waves share
 };
 int64_t weight_rows(const fs_linear& c) { return c.gated ? 2 * c.N : c.N; }
 
-// Columns of the results that a workgroup of the kernel without tiles takes, of `cols`: a multiple of eight, so many that the
+// Columns of the results that a workgroup of the streaming kernel takes, of `cols`: a multiple of eight, so many that the
 // grid is one round of the 256 CUs, or the fewest rounds where that is more than seven tiles; and the tiles of its kernel.
 int64_t stream_columns(int64_t cols, bool gated) {
   const int64_t most = 256 * (gated ? 56 : 112), rounds = (cols + most - 1) / most;
@@ -430,7 +435,12 @@ int stream_tiles(int64_t cols, bool gated) {
 // Tiles: the cheapest of what a sweep over 26 shapes of 40 to 4000 rows fits (us; by 4 to 12 % rms, and its choice is within
 // 1 % of the best one's time on average, 7 % at most): `first` for a grid, `round` for each further round of the CUs' places
 // (two of the smaller tiles share a CU: stage2 for both), a stage of 128, and a MB of results or of sums in memory. Codes
-// leave tiles of 128 columns by themselves, a gate's tiles of 256; other sums go through memory, as those of K splits do.
+// leave tiles of 128 columns by themselves, a gate's tiles of 256; other sums go through memory, as those of K splits do. Eight
+// splits pay 1 us beside their bytes: of 19 shapes of 80 to 640 rows that this leaves with four, 16 are the faster for it (160 x
+// 2048 x 8192 15.6 us for 17.5, 512 x 1024 x 8192 16.1 for 19.1, 129 x 1024 x 4096 9.5 for 10.2), three the slower by up to 3 % (200 x
+// 6144 x 16384 43.8 for 42.6). Beyond the sweep's 4000 rows, and for many tiles below, the fit is off by up to a fifth (8005 x 28672 x
+// 4096 863 us for 730, 2777 x 28672 x 4096 302 for 262, 8005 x 4096 x 4096 117 for 126, 2777 x 4096 x 14336 128 for 142); the largest
+// tile is ahead of the next there by as much or more.
 Plan plan_for(const fs_linear& c) {
   const int64_t M = c.M, N = weight_rows(c), nk = c.K / GROUP;
   const bool codes = c.out_scales != nullptr;

@@ -206,7 +206,9 @@ bool dtype_ok(int32_t dt) { return dt == FS_F32 || dt == FS_BF16 || dt == FS_F16
 
 // Up to four rows a CU are held by their latency: one piece a thread (64 x 4096 bf16 with delta 3.7 us, two pieces 4.2; 64 x
 // 8192 4.5, four pieces 5.7); longer batches by HBM, where fewer, larger threads draw more (8005 x 4096 21.0 us without delta,
-// one piece 25.9; with delta 38.7, 5.9 TB/s). The results are the same.
+// one piece 25.9; with delta 38.7, 5.9 TB/s). The results are the same. Rows of more than 16384 columns, which no configuration
+// here has, are not held and read twice (2000 x 20480 bf16 with delta 60.7 us, 4.7 TB/s of the bytes that it cannot do without;
+// 2000 x 16384 39.3, 5.8).
 template <int DT, bool VEC, bool DELTA>
 void launch_norm(const NormArgs& a, hipStream_t s) {
   const unsigned rows = (unsigned)a.M, rows4 = (unsigned)((a.M + 3) / 4);

@@ -178,7 +178,9 @@ def gemm_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Opt
     little: three launches). Sums are float32 (of each eight
     products the matrix instruction drops what lies more than 13 binary places below the largest); product and residual
     are rounded once, to a's dtype. A row's last bit may depend on how many rows the call has. out may be the
-    residual itself, but shares no memory with a or w."""
+    residual itself, but shares no memory with a or w. linear_e4m3 computes the same product with kernels and an order of its
+    own (a last bit may differ), also from rows in codes, and is mostly the faster from about 8 rows to 1000, by up to a third;
+    this call is for fewer rows of small weights, by up to a fifth."""
     require_device(a, w, w_scales)
     if not a.device == w.device == w_scales.device or any(t is not None and t.device != a.device for t in (out, residual)):
         raise ValueError("gemm_e4m3: tensors on different devices")
@@ -379,9 +381,11 @@ def linear_e4m3(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, a_scal
     add_rmsnorm_e4m3 or linear_e4m3_codes), or rows of float32, bfloat16 or float16, which are encoded within the call.
     activation: None, "relu", "silu", "gelu" (with the normal distribution's function) or "gelu_tanh". bias: float32,
     bfloat16 or float16. The result is bfloat16 or float16: dtype, or out's, the residual's or a's, in that order, or
-    bfloat16; the residual has the same. K is a multiple of 128. Sums as gemm_e4m3's, the rest in float32, rounded once. A
-    row's last bit may depend on how many rows the call has. out may be the residual itself, but shares no memory with a
-    or w."""
+    bfloat16; the residual has the same. K is a multiple of 128. Sums are float32, but of each eight products the matrix
+    instruction drops what lies more than 13 binary places below the largest: 2.5e-5 of a random result's norm. (With every
+    product in full: dequantize_e4m3 both to bfloat16, which holds them exactly, and gemm.) The rest is float32, rounded
+    once. A row's last bit may depend on how many rows the call has. out may be the residual itself, but shares no memory
+    with a or w."""
     if dtype is None:
         dtype = (out.dtype if out is not None else residual.dtype if residual is not None else
                  a.dtype if a.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16)
@@ -394,7 +398,8 @@ def linear_e4m3_codes(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, 
                       bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
                       gated: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """linear_e4m3 with its result left in 8-bit floating point for the next product: (codes, scales) as quantize_e4m3 lays
-    them out, rounded once. The result's columns are a multiple of 128."""
+    them out, rounded once. The result's columns are a multiple of 128. What the sums drop turns a value next to the middle
+    between two codes to the other one: 1e-3 of a random result's norm, where the codes' own rounding is 2.7e-2."""
     return _linear_e4m3("linear_e4m3_codes", a, w, w_scales, a_scales, bias, activation, gated, None, None, torch.float8_e4m3fn)
 
 

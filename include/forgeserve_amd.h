@@ -323,7 +323,8 @@ int fs_add_rmsnorm_e4m3(const void* x, int64_t ldx, const void* delta, int64_t l
 /* A projection over codes and what follows it. With z = x . w^T + bias:
  *   out = act(z) + residual, or, gated (w and bias hold the gate's N rows, then N others),
  *   out = act(z[:, :N]) * z[:, N:] + residual                                     (SwiGLU.forward, model.py:88-93)
- * Sums as fs_gemm_e4m3's, the rest in f32, rounded once: to rows of `dtype`, or, with out_scales, to codes.
+ * Sums as fs_gemm_e4m3's (f32, but for what the matrix instruction drops of each eight products), the rest in f32, rounded
+ * once: to rows of `dtype`, or, with out_scales, to codes.
  * x_scales NULL: x holds rows of x_dtype, which are encoded within the call. bias (contiguous), residual: or NULL. The
  * residual has `dtype`; none is added to codes. */
 typedef struct fs_linear {
